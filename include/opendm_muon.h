@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define MUON_ABI_VERSION 4
+#define MUON_ABI_VERSION 5
 
 enum muon_status {
   MUON_OK = 0,
@@ -52,6 +52,17 @@ enum muon_dtype {
   MUON_F16 = 3,  /* float16 storage (NS operands, scaled by powers of two) */
   MUON_F16X3 = 4 /* NS operands as float16 pairs hi + lo (hi = fp16(x), lo = fp16(x - hi)), each
                     product as hi*hi + hi*lo + lo*hi: ~22-bit operands for 3x the MMA work */
+};
+
+enum muon_index_dtype {
+  MUON_I32 = 16, /* 32-bit signed token ids */
+  MUON_I64 = 17  /* 64-bit signed token ids */
+};
+
+enum muon_norm_kind {
+  MUON_NORM_2 = 0,
+  MUON_NORM_1 = 1,
+  MUON_NORM_INF = 2
 };
 
 enum muon_ns_algo {
@@ -414,6 +425,97 @@ int muon_adamw(const muon_adamw_seg* segs_dev, int n_segs, int64_t total_chunks,
  * (gradient-norm clipping, section (e)). */
 int muon_adamw_scaled(const muon_adamw_seg* segs_dev, int n_segs, int64_t total_chunks, double beta1, double beta2,
                       float eps, float wd_factor, const float* grad_scale_dev, void* stream);
+
+/* muon_adamw for a rows x dim parameter whose gradient is zero outside `count`
+ * rows (what muon_embedding_grad's row form writes): the results equal
+ * muon_adamw_scaled's on the dense gradient, which is neither made nor read.
+ * `seg` is host memory, read before the call returns. ids: [cap] ascending
+ * row numbers, of which the first *count (all, when count is NULL; never more
+ * than cap) are used; an id outside [0, rows) matches no row. values:
+ * [cap][dim] of grad_dtype. exp_avg and exp_avg_sq are fp32, updated in place
+ * like param. */
+typedef struct muon_adamw_rows_seg {
+  void* param;           /* [rows][dim] of param_dtype */
+  float* exp_avg;        /* [rows][dim] */
+  float* exp_avg_sq;     /* [rows][dim] */
+  const int64_t* ids;    /* [cap] device */
+  const void* values;    /* [cap][dim] of grad_dtype, device */
+  const int64_t* count;  /* device, or NULL */
+  int64_t rows;
+  int64_t dim;
+  int64_t cap;
+  float step_size;
+  float bc2_sqrt;
+  int32_t param_dtype;
+  int32_t grad_dtype;
+} muon_adamw_rows_seg;
+
+int muon_adamw_rows(const muon_adamw_rows_seg* seg, double beta1, double beta2, float eps, float wd_factor,
+                    const float* grad_scale_dev /* or NULL */, void* stream);
+
+/* ------------------------------- (f) token embedding and its gradient
+ * No counterpart in the reference's optimizer: the lookup whose gradient is
+ * the largest tensor of the AdamW group (a vocabulary of 151936 rows against
+ * the few thousand distinct tokens of a step), and that gradient in the form
+ * muon_adamw_rows takes.
+ *
+ * muon_embedding:  out[t] = round(scale * weight[ids[t]])   for t in [0, tokens)
+ * weight: [rows][ld] (ld >= dim), out: [tokens][dim]; MUON_BF16 or MUON_F32
+ * each, the product in fp32, rounded once to out_dtype. An id outside
+ * [0, rows) gives a row of zeros and records MUON_DEV_BAD_INDEX in *err_dev. */
+#define MUON_DEV_BAD_INDEX 0x201
+int muon_embedding(const void* weight, int weight_dtype, int64_t rows, int64_t dim, int64_t ld, const void* ids,
+                   int ids_dtype, int64_t tokens, float scale, void* out, int out_dtype, int* err_dev, void* stream);
+
+/* muon_embedding_grad:  dW[v] = round(scale * sum over t with ids[t] == v of grad[t])
+ * by sorting the tokens by id: fp32 sums in an order fixed by the sorted
+ * tokens (two calls give the same bits). grad: [tokens][dim], MUON_BF16 or
+ * MUON_F32. Tokens whose id is padding_idx (-1: none) are left out; ids outside
+ * [0, rows) are left out and record MUON_DEV_BAD_INDEX in *err_dev.
+ *   dense form (out_ids NULL): out is [rows][dim] of out_dtype, every row
+ *     written, zeros for a row without tokens; count is not used.
+ *   row form: out is [cap][dim] and out_ids [cap], cap = min(tokens, rows):
+ *     the distinct ids, ascending, and their rows, *count of them; the rows
+ *     past *count are written as zeros with id 0, so that (out_ids, out) is a
+ *     valid coordinate list whatever *count is.
+ * workspace: muon_embedding_grad_workspace_bytes() bytes, 256-byte aligned
+ * (-1 for sizes the call refuses: tokens or rows >= 2^31 - 1). One workspace
+ * serves one call at a time. */
+int64_t muon_embedding_grad_workspace_bytes(int64_t tokens, int64_t rows, int64_t dim);
+int muon_embedding_grad(const void* grad, int grad_dtype, const void* ids, int ids_dtype, int64_t tokens,
+                        int64_t rows, int64_t dim, int64_t padding_idx, float scale, void* out, int out_dtype,
+                        int64_t* out_ids, int64_t* count, void* workspace, int64_t workspace_bytes, int* err_dev,
+                        void* stream);
+
+/* ------------------------- (g) norm and clipping of a list of gradients
+ * The in-place form of section (e) (opendm/trainer/trainer.py:213 clips
+ * before each step), for gradients that something other than this library's
+ * step reads, without (e)'s roundings to the gradients' dtype:
+ *   total = (sum over all elements of |g|^p)^(1/p), p = 1, 2 or inf
+ *   coef  = min(max_norm / (total + 1e-6), 1)       (NaN when total is)
+ *   out   = round(grad * coef)                      (out may be grad itself)
+ * Products in fp32, joined in double in a fixed order; elements whose squares leave
+ * fp32's range are summed in double, so total overflows or underflows only
+ * where its own fp32 value does. `segs` is host memory, read before the call
+ * returns; segments must not overlap other segments' outputs. workspace:
+ * muon_clip_workspace_bytes(n_segs) bytes, 16-byte aligned. total_dev: one
+ * device float, written by muon_total_norm and muon_clip_grads, read by
+ * muon_scale_grads (which applies the coefficient of a norm known already). */
+typedef struct muon_clip_seg {
+  const void* grad;    /* numel elements of grad_dtype */
+  void* out;           /* numel elements of out_dtype (unused by muon_total_norm) */
+  int64_t numel;
+  int32_t grad_dtype;  /* MUON_BF16 or MUON_F32 */
+  int32_t out_dtype;
+} muon_clip_seg;
+
+int64_t muon_clip_workspace_bytes(int64_t n_segs);
+int muon_total_norm(const muon_clip_seg* segs, int64_t n_segs, int norm_kind, void* workspace, float* total_dev,
+                    void* stream);
+int muon_clip_grads(const muon_clip_seg* segs, int64_t n_segs, int norm_kind, float max_norm, void* workspace,
+                    float* total_dev, void* stream);
+int muon_scale_grads(const muon_clip_seg* segs, int64_t n_segs, float max_norm, const float* total_dev,
+                     void* stream);
 
 #ifdef __cplusplus
 }

@@ -30,7 +30,14 @@ MUON_NS_STANDARD = 0
 MUON_NS_GRAM = 1
 MUON_NS_INPUT_SCALED = 1  # muon_ns_class.flags
 
-ABI_VERSION = 4
+MUON_I32 = 16
+MUON_I64 = 17
+MUON_NORM_2 = 0
+MUON_NORM_1 = 1
+MUON_NORM_INF = 2
+MUON_DEV_BAD_INDEX = 0x201  # device error word: a token id outside the vocabulary
+
+ABI_VERSION = 5
 
 
 class MomentumSeg(Structure):
@@ -116,6 +123,29 @@ class AdamwSeg(Structure):
     ]
 
 
+class AdamwRowsSeg(Structure):
+    _fields_ = [
+        ("param", c_void_p),
+        ("exp_avg", c_void_p),
+        ("exp_avg_sq", c_void_p),
+        ("ids", c_void_p),
+        ("values", c_void_p),
+        ("count", c_void_p),
+        ("rows", c_int64),
+        ("dim", c_int64),
+        ("cap", c_int64),
+        ("step_size", c_float),
+        ("bc2_sqrt", c_float),
+        ("param_dtype", c_int32),
+        ("grad_dtype", c_int32),
+    ]
+
+
+class ClipSeg(Structure):
+    _fields_ = [("grad", c_void_p), ("out", c_void_p), ("numel", c_int64), ("grad_dtype", c_int32),
+                ("out_dtype", c_int32)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/opendm_muon.h.
 SIGNATURES = {
     "muon_version": (c_int, []),
@@ -151,6 +181,16 @@ SIGNATURES = {
     "muon_ns_class_layout": (c_int, [POINTER(NsClass), c_void_p, c_int]),
     "muon_adamw_chunks": (c_int64, [c_int64]),
     "muon_adamw": (c_int, [c_void_p, c_int, c_int64, c_double, c_double, c_float, c_float, c_void_p]),
+    "muon_adamw_rows": (c_int, [POINTER(AdamwRowsSeg), c_double, c_double, c_float, c_float, c_void_p, c_void_p]),
+    "muon_embedding": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_float, c_void_p,
+                               c_int, c_void_p, c_void_p]),
+    "muon_embedding_grad_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64]),
+    "muon_embedding_grad": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_float,
+                                    c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "muon_clip_workspace_bytes": (c_int64, [c_int64]),
+    "muon_total_norm": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
+    "muon_clip_grads": (c_int, [c_void_p, c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p]),
+    "muon_scale_grads": (c_int, [c_void_p, c_int64, c_float, c_void_p, c_void_p]),
 }
 
 _LIB = None

@@ -135,6 +135,202 @@ __global__ void __launch_bounds__(ADAM_THREADS) adamw_kernel(const muon_adamw_se
   }
 }
 
+// ------------------------------------------------------------ row gradients
+// The same update of a [rows][dim] parameter whose gradient is zero outside
+// the rows listed in ids (ascending). A block takes ADAM_CHUNK consecutive elements,
+// finds the listed rows among its own by a 32-way search of ids and keeps
+// their slots in shared memory; elements of the other rows take g = 0, so
+// the results equal adamw_kernel's on the dense gradient, at the bytes of
+// param and moments plus those of the listed rows.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float (&v)[4]) {
+  if constexpr (sizeof(T) == 2) {
+    const uint2 raw = *reinterpret_cast<const uint2*>(p);
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+    const float2 a = __bfloat1622float2(h[0]), b = __bfloat1622float2(h[1]);
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+  } else {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float (&v)[4]) {
+  if constexpr (sizeof(T) == 2) {
+    uint2 raw;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&raw);
+    h[0] = __floats2bfloat162_rn(v[0], v[1]);
+    h[1] = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(p) = raw;
+  } else {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float load1(const T* p) {
+  if constexpr (sizeof(T) == 2)
+    return __bfloat162float(*p);
+  else
+    return *p;
+}
+template <typename T>
+__device__ __forceinline__ void store1(T* p, float v) {
+  if constexpr (sizeof(T) == 2)
+    *p = __float2bfloat16_rn(v);
+  else
+    *p = v;
+}
+
+// First index in ids[0, n) with ids[index] >= row, by a whole warp: 32
+// probes a step, so four dependent loads for a million rows.
+__device__ __forceinline__ int64_t warp_lower_bound(const int64_t* ids, int64_t n, int64_t row) {
+  const int lane = threadIdx.x & 31;
+  int64_t lo = 0, hi = n;
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 31) / 32;
+    const int64_t at = lo + int64_t(lane) * step;
+    const bool below = at < hi && ids[at] < row;
+    const int k = __popc(__ballot_sync(0xffffffffu, below));  // the probes below `row` come first
+    if (k == 0) return lo;
+    const int64_t last_below = lo + int64_t(k - 1) * step;
+    hi = min(hi, last_below + step);
+    lo = last_below + 1;
+  }
+  return lo;
+}
+
+struct AdamwRowsArgs {
+  float* exp_avg;
+  float* exp_avg_sq;
+  const int64_t* ids;
+  const int64_t* count;
+  int64_t rows, dim, cap, numel;
+  float beta1w, beta2, one_minus_beta2, eps, wd_factor, neg_step, bc2_sqrt;
+  const float* grad_scale;
+};
+
+template <typename P, typename G, bool kVector>
+__global__ void __launch_bounds__(ADAM_THREADS) adamw_rows_kernel(P* __restrict__ param, const G* __restrict__ values,
+                                                                  const AdamwRowsArgs a) {
+  // slot of each of the block's rows (at most ADAM_CHUNK + 1, when dim is 1), or -1
+  extern __shared__ int32_t slots[];
+  constexpr int kPer = kVector ? ADAM_VEC : 1;
+  const int64_t e0 = int64_t(blockIdx.x) * ADAM_CHUNK;
+  const int64_t e1 = min(e0 + ADAM_CHUNK, a.numel);
+  const int64_t row0 = e0 / a.dim, row1 = (e1 - 1) / a.dim + 1;
+  const uint32_t col0 = static_cast<uint32_t>(e0 - row0 * a.dim), dim = static_cast<uint32_t>(a.dim);
+  const int n_rows = static_cast<int>(row1 - row0);
+  for (int r = threadIdx.x; r < n_rows; r += ADAM_THREADS) slots[r] = -1;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int64_t n = a.count ? min(max(*a.count, int64_t(0)), a.cap) : a.cap;
+    const int64_t first = warp_lower_bound(a.ids, n, row0);
+    for (int64_t i = first + threadIdx.x;; i += 32) {
+      const int64_t id = i < n ? a.ids[i] : row1;
+      const bool mine = id >= row0 && id < row1;
+      if (mine) slots[id - row0] = static_cast<int32_t>(i);
+      if (!__all_sync(0xffffffffu, mine)) break;
+    }
+  }
+  __syncthreads();
+  const bool pbf = sizeof(P) == 2, gbf = sizeof(G) == 2;
+  const float coef = a.grad_scale ? *a.grad_scale : 1.f;
+  const int len = static_cast<int>(e1 - e0);
+  for (int o = threadIdx.x * kPer; o < len; o += ADAM_THREADS * kPer) {
+    const int64_t e = e0 + o;
+    float p[kPer], m[kPer], v[kPer], g[kPer];
+    if constexpr (kVector) {
+      load4(param + e, p);
+      load4(a.exp_avg + e, m);
+      load4(a.exp_avg_sq + e, v);
+    } else {
+      p[0] = load1(param + e);
+      m[0] = a.exp_avg[e];
+      v[0] = a.exp_avg_sq[e];
+    }
+    const uint32_t at = col0 + o, r = at / dim, col = at - r * dim;
+    const int32_t slot = slots[r];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) g[i] = 0.f;
+    if (slot >= 0) {
+      if constexpr (kVector)
+        load4(values + int64_t(slot) * a.dim + col, g);
+      else
+        g[0] = load1(values + int64_t(slot) * a.dim + col);
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (a.grad_scale) g[i] = clip_grad_adam(g[i], coef, gbf);
+      p[i] = adam_elem(p[i], g[i], m[i], v[i], a.beta1w, a.beta2, a.one_minus_beta2, a.eps, a.wd_factor, a.neg_step,
+                       a.bc2_sqrt, pbf);
+    }
+    if constexpr (kVector) {
+      store4(a.exp_avg + e, m);
+      store4(a.exp_avg_sq + e, v);
+      store4(param + e, p);
+    } else {
+      a.exp_avg[e] = m[0];
+      a.exp_avg_sq[e] = v[0];
+      store1(param + e, p[0]);
+    }
+  }
+}
+
+template <typename P, typename G>
+int run_adamw_rows(const muon_adamw_rows_seg& sg, const AdamwRowsArgs& a, cudaStream_t stream) {
+  const bool vec = sg.dim % ADAM_VEC == 0 &&
+                   ((reinterpret_cast<uintptr_t>(sg.param) | reinterpret_cast<uintptr_t>(sg.values) |
+                     reinterpret_cast<uintptr_t>(sg.exp_avg) | reinterpret_cast<uintptr_t>(sg.exp_avg_sq)) & 15u) == 0;
+  const int64_t blocks = (a.numel + ADAM_CHUNK - 1) / ADAM_CHUNK;
+  if (blocks > 0x7fffffffLL) return set_error(MUON_ERR_ARG, "too many AdamW chunks");
+  const size_t smem = sizeof(int32_t) * size_t(ADAM_CHUNK / sg.dim + 2);
+  P* p = static_cast<P*>(sg.param);
+  const G* g = static_cast<const G*>(sg.values);
+  if (vec)
+    adamw_rows_kernel<P, G, true><<<unsigned(blocks), ADAM_THREADS, smem, stream>>>(p, g, a);
+  else
+    adamw_rows_kernel<P, G, false><<<unsigned(blocks), ADAM_THREADS, smem, stream>>>(p, g, a);
+  return check_cuda(cudaGetLastError(), "adamw rows launch");
+}
+
+int launch_adamw_rows(const muon_adamw_rows_seg* seg, double beta1, double beta2, float eps, float wd_factor,
+                      const float* grad_scale, cudaStream_t stream) {
+  if (!seg) return set_error(MUON_ERR_ARG, "null AdamW row segment");
+  const muon_adamw_rows_seg& sg = *seg;
+  if (sg.rows < 0 || sg.dim < 0 || sg.cap < 0 || sg.cap > 0x7fffffffLL || sg.dim > 0x7fff0000LL ||
+      (sg.dim > 0 && sg.rows > (int64_t(1) << 43) / sg.dim))
+    return set_error(MUON_ERR_ARG, "AdamW row sizes out of range");
+  if ((sg.param_dtype != MUON_BF16 && sg.param_dtype != MUON_F32) ||
+      (sg.grad_dtype != MUON_BF16 && sg.grad_dtype != MUON_F32))
+    return set_error(MUON_ERR_ARG, "AdamW row dtypes must be MUON_BF16 or MUON_F32");
+  if (sg.rows == 0 || sg.dim == 0) return MUON_OK;
+  if (!sg.param || !sg.exp_avg || !sg.exp_avg_sq || (sg.cap > 0 && (!sg.ids || !sg.values)))
+    return set_error(MUON_ERR_ARG, "null AdamW row pointer");
+  AdamwRowsArgs a{};
+  a.exp_avg = sg.exp_avg;
+  a.exp_avg_sq = sg.exp_avg_sq;
+  a.ids = sg.ids;
+  a.count = sg.count;
+  a.rows = sg.rows;
+  a.dim = sg.dim;
+  a.cap = sg.cap;
+  a.numel = sg.rows * sg.dim;
+  a.beta1w = static_cast<float>(1.0 - beta1);
+  a.beta2 = static_cast<float>(beta2);
+  a.one_minus_beta2 = static_cast<float>(1.0 - beta2);
+  a.eps = eps;
+  a.wd_factor = wd_factor;
+  a.neg_step = -sg.step_size;
+  a.bc2_sqrt = sg.bc2_sqrt;
+  a.grad_scale = grad_scale;
+  using bf = __nv_bfloat16;
+  const bool pb = sg.param_dtype == MUON_BF16, gb = sg.grad_dtype == MUON_BF16;
+  if (pb && gb) return run_adamw_rows<bf, bf>(sg, a, stream);
+  if (pb) return run_adamw_rows<bf, float>(sg, a, stream);
+  if (gb) return run_adamw_rows<float, bf>(sg, a, stream);
+  return run_adamw_rows<float, float>(sg, a, stream);
+}
+
 int launch_adamw(const muon_adamw_seg* segs_dev, int n_segs, int64_t total_chunks, double beta1, double beta2,
                  float eps, float wd_factor, const float* grad_scale, cudaStream_t stream) {
   if (n_segs <= 0 || total_chunks <= 0) return MUON_OK;

@@ -75,7 +75,8 @@ int muon_read_error(int* err_dev, int* host_code, void* stream) {
     if (muon::check_cuda(cudaMemsetAsync(err_dev, 0, sizeof(int), s), "clear error word"))
       return MUON_ERR_CUDA;
     char buf[128];
-    snprintf(buf, sizeof(buf), "kernel reported error code 0x%x (bounded wait expired)", code);
+    snprintf(buf, sizeof(buf), "kernel reported error code 0x%x (%s)", code,
+             code == MUON_DEV_BAD_INDEX ? "token id out of range" : "bounded wait expired");
     return set_error(MUON_ERR_KERNEL, buf);
   }
   return MUON_OK;
@@ -187,6 +188,48 @@ int muon_clip_grad_norm(const muon_norm_seg* segs_dev, int n_segs, int64_t total
                         float* partials_dev, float* out_dev, void* stream) {
   return muon::launch_clip_grad_norm(segs_dev, n_segs, total_chunks, max_norm, partials_dev, out_dev,
                                      static_cast<cudaStream_t>(stream));
+}
+
+int muon_adamw_rows(const muon_adamw_rows_seg* seg, double beta1, double beta2, float eps, float wd_factor,
+                    const float* grad_scale_dev, void* stream) {
+  return muon::launch_adamw_rows(seg, beta1, beta2, eps, wd_factor, grad_scale_dev, static_cast<cudaStream_t>(stream));
+}
+
+int muon_embedding(const void* weight, int weight_dtype, int64_t rows, int64_t dim, int64_t ld, const void* ids,
+                   int ids_dtype, int64_t tokens, float scale, void* out, int out_dtype, int* err_dev, void* stream) {
+  return muon::launch_embedding(weight, weight_dtype, rows, dim, ld, ids, ids_dtype, tokens, scale, out, out_dtype,
+                                err_dev, static_cast<cudaStream_t>(stream));
+}
+
+int64_t muon_embedding_grad_workspace_bytes(int64_t tokens, int64_t rows, int64_t dim) {
+  return muon::embedding_grad_workspace_bytes(tokens, rows, dim);
+}
+
+int muon_embedding_grad(const void* grad, int grad_dtype, const void* ids, int ids_dtype, int64_t tokens,
+                        int64_t rows, int64_t dim, int64_t padding_idx, float scale, void* out, int out_dtype,
+                        int64_t* out_ids, int64_t* count, void* workspace, int64_t workspace_bytes, int* err_dev,
+                        void* stream) {
+  return muon::launch_embedding_grad(grad, grad_dtype, ids, ids_dtype, tokens, rows, dim, padding_idx, scale, out,
+                                     out_dtype, out_ids, count, workspace, workspace_bytes, err_dev,
+                                     static_cast<cudaStream_t>(stream));
+}
+
+int64_t muon_clip_workspace_bytes(int64_t n_segs) { return muon::clip_workspace_bytes(n_segs); }
+
+int muon_total_norm(const muon_clip_seg* segs, int64_t n_segs, int norm_kind, void* workspace, float* total_dev,
+                    void* stream) {
+  return muon::launch_total_norm(segs, n_segs, norm_kind, workspace, total_dev, static_cast<cudaStream_t>(stream));
+}
+
+int muon_clip_grads(const muon_clip_seg* segs, int64_t n_segs, int norm_kind, float max_norm, void* workspace,
+                    float* total_dev, void* stream) {
+  return muon::launch_clip_grads(segs, n_segs, norm_kind, max_norm, workspace, total_dev,
+                                 static_cast<cudaStream_t>(stream));
+}
+
+int muon_scale_grads(const muon_clip_seg* segs, int64_t n_segs, float max_norm, const float* total_dev,
+                     void* stream) {
+  return muon::launch_scale_grads(segs, n_segs, max_norm, total_dev, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -50,4 +50,24 @@ int launch_flags_wait(const muon_flag_list* list, uint32_t value, int64_t timeou
 int launch_momentum_f16(const muon_momentum_f16_seg* segs_dev, int n_segs, int64_t total_chunks, int grad_dtype,
                         float momentum, int nesterov, float eps, float* partials_dev, float* pscale_dev,
                         float* scales_dev, int* redo_dev, const float* grad_scale, cudaStream_t stream);
+
+int launch_adamw_rows(const muon_adamw_rows_seg* seg, double beta1, double beta2, float eps, float wd_factor,
+                      const float* grad_scale, cudaStream_t stream);
+
+int launch_embedding(const void* weight, int weight_dtype, int64_t rows, int64_t dim, int64_t ld, const void* ids,
+                     int ids_dtype, int64_t tokens, float scale, void* out, int out_dtype, int* err,
+                     cudaStream_t stream);
+int64_t embedding_grad_workspace_bytes(int64_t tokens, int64_t rows, int64_t dim);
+int launch_embedding_grad(const void* grad, int grad_dtype, const void* ids, int ids_dtype, int64_t tokens,
+                          int64_t rows, int64_t dim, int64_t padding_idx, float scale, void* out, int out_dtype,
+                          int64_t* out_ids, int64_t* count, void* workspace, int64_t workspace_bytes, int* err,
+                          cudaStream_t stream);
+
+int64_t clip_workspace_bytes(int64_t n_segs);
+int launch_total_norm(const muon_clip_seg* segs, int64_t n_segs, int norm_kind, void* workspace, float* total,
+                      cudaStream_t stream);
+int launch_clip_grads(const muon_clip_seg* segs, int64_t n_segs, int norm_kind, float max_norm, void* workspace,
+                      float* total, cudaStream_t stream);
+int launch_scale_grads(const muon_clip_seg* segs, int64_t n_segs, float max_norm, const float* total,
+                       cudaStream_t stream);
 }  // namespace muon

@@ -35,6 +35,7 @@ import torch
 
 from . import _native as N
 from . import trace
+from .embedding import RowGrad
 
 _DTYPE_CODE = {torch.bfloat16: N.MUON_BF16, torch.float32: N.MUON_F32}
 PRECISIONS = {"tf32": N.MUON_TF32, "fp16": N.MUON_F16, "bf16": N.MUON_BF16, "parity": N.MUON_F16X3}
@@ -59,7 +60,7 @@ class MatrixItem:
 @dataclass
 class AdamItem:
     param: torch.Tensor
-    grad: torch.Tensor
+    grad: torch.Tensor | RowGrad
     exp_avg: torch.Tensor
     exp_avg_sq: torch.Tensor
     step: float  # step count after this step's increment
@@ -743,7 +744,12 @@ class CudaMuonEngine:
 
     def adamw(self, items: list[AdamItem], *, lr: float, beta1: float, beta2: float, eps: float,
               weight_decay: float) -> None:
-        """Fused AdamW over all items (reference muon_adamw.py:333-343)."""
+        """Fused AdamW over all items (reference muon_adamw.py:333-343); an
+        item whose gradient is a RowGrad gets a launch of its own."""
+        for it in items:
+            if isinstance(it.grad, RowGrad):
+                self._adamw_rows(it, lr=lr, beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay)
+        items = [it for it in items if not isinstance(it.grad, RowGrad)]
         if not items:
             return
         segs = []
@@ -793,6 +799,44 @@ class CudaMuonEngine:
                                            c_float(eps), c_float(wd_factor),
                                            c_void_p(gs.data_ptr() if gs is not None else None), _stream_handle()),
                 "muon_adamw_scaled")
+        self._event_end(ev)
+        self.kernel_launches += 1
+
+    def _adamw_rows(self, it: AdamItem, *, lr: float, beta1: float, beta2: float, eps: float,
+                    weight_decay: float) -> None:
+        """AdamW of one parameter whose gradient is zero outside some rows."""
+        g = it.grad
+        tensors = (it.param, it.exp_avg, it.exp_avg_sq, g.ids, g.values)
+        for t in tensors + ((g.count,) if g.count is not None else ()):
+            if t.device != self.device:
+                raise RuntimeError("AdamW tensors must be on the engine's device")
+        if not all(t.is_contiguous() for t in tensors):
+            raise RuntimeError("AdamW parameters, moments and row gradients must be contiguous")
+        shape = it.param.shape
+        if it.param.ndim < 2 or g.num_rows != shape[0] or g.values.shape[1:] != shape[1:]:
+            raise RuntimeError(f"row gradient of {g.num_rows} rows of {tuple(g.values.shape[1:])} does not match a "
+                               f"parameter of shape {tuple(shape)}")
+        if it.exp_avg.shape != shape or it.exp_avg_sq.shape != shape:
+            raise RuntimeError("AdamW moments must have their parameter's shape")
+        if it.exp_avg.dtype != torch.float32 or it.exp_avg_sq.dtype != torch.float32:
+            raise RuntimeError("AdamW moments must be float32")
+        if g.ids.dtype != torch.int64 or g.ids.ndim != 1 or g.ids.numel() != g.values.shape[0]:
+            raise RuntimeError("a row gradient needs one int64 id per row of values")
+        if g.count is not None and (g.count.dtype != torch.int64 or g.count.numel() != 1):
+            raise RuntimeError("a row gradient's count is one int64 value")
+        s = N.AdamwRowsSeg()
+        s.param, s.exp_avg, s.exp_avg_sq = it.param.data_ptr(), it.exp_avg.data_ptr(), it.exp_avg_sq.data_ptr()
+        s.ids, s.values = g.ids.data_ptr(), g.values.data_ptr()
+        s.count = g.count.data_ptr() if g.count is not None else None
+        s.rows, s.dim, s.cap = shape[0], math.prod(shape[1:]), g.ids.numel()
+        s.step_size, s.bc2_sqrt = lr / (1 - beta1 ** it.step), (1 - beta2 ** it.step) ** 0.5
+        s.param_dtype, s.grad_dtype = _dtype_code(it.param), _dtype_code(g.values)
+        wd_factor = 1.0 - lr * weight_decay if weight_decay != 0 else 1.0
+        ev = self._event_pair("adamw")
+        gs = self.grad_scale
+        N.check(self.lib.muon_adamw_rows(byref(s), float(beta1), float(beta2), c_float(eps), c_float(wd_factor),
+                                         c_void_p(gs.data_ptr() if gs is not None else None), _stream_handle()),
+                "muon_adamw_rows")
         self._event_end(ev)
         self.kernel_launches += 1
 

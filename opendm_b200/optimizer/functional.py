@@ -1,0 +1,303 @@
+"""Gradient norm, clipping and AdamW over lists of tensors.
+
+``clip_grad_norm_``, ``get_total_norm`` and ``clip_grads_with_norm_`` take the
+arguments of their ``torch.nn.utils`` namesakes; ``clip_grads`` is the form
+over the gradients themselves, in place or into other tensors (fp32
+accumulators into bf16 gradients, say). Norms of type 1, 2 and inf; the norm is
+returned in fp32 whatever the gradients' dtype, sums are held in fp32 and
+double, and a clipped gradient is rounded once. (``MuonAdamW.clip_grad_norm_``
+is the form that folds the clip into the optimizer's step, with torch's
+roundings.) ``adamw`` is the optimizer's fused AdamW over lists, for dense
+gradients and for row gradients (``opendm_b200.embedding.RowGrad``).
+
+All run sm_100a kernels on the current stream of the tensors' device; CPU
+tensors raise. No call reads anything back unless asked to
+(``error_if_nonfinite``), so all of them can be captured into a CUDA graph.
+"""
+
+from __future__ import annotations
+
+import math
+from array import array
+from collections.abc import Iterable
+
+import torch
+
+from .. import _native as N
+from ..embedding import RowGrad, _device_index, _on_device, embedding_row_grad
+from ..engine import AdamItem
+
+_CODE = {torch.bfloat16: N.MUON_BF16, torch.float32: N.MUON_F32}
+_NORMS = {2.0: N.MUON_NORM_2, 1.0: N.MUON_NORM_1, math.inf: N.MUON_NORM_INF}
+
+
+def _norm_kind(norm_type: float) -> int:
+    kind = _NORMS.get(float(norm_type))
+    if kind is None:
+        raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type}")
+    return kind
+
+
+def _dense_storage(t: torch.Tensor) -> bool:
+    """True when the tensor's elements fill one block of memory, in any order."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _check_grads(grads: list[torch.Tensor], what: str) -> int:
+    """Device index of the list; raises for layouts, dtypes and devices the kernels do not take."""
+    index = _device_index(grads[0])
+    device = grads[0].device
+    for g in grads:
+        if g.layout is not torch.strided:
+            raise RuntimeError(f"{what} must be dense tensors, got layout {g.layout}")
+        if g.device != device:
+            raise RuntimeError(f"{what} must be on one device; got {device} and {g.device}")
+        if g.dtype not in _CODE:
+            raise RuntimeError(f"unsupported dtype {g.dtype}: the kernels take bfloat16 or float32")
+    return index
+
+
+def _table(src: list[torch.Tensor], dst: list[torch.Tensor]) -> array:
+    """The list as muon_clip_seg structures: pointers, size and the two 32-bit dtypes of each."""
+    flat = array("q")
+    for s, d in zip(src, dst):
+        flat.extend((s.data_ptr(), d.data_ptr(), s.numel(), _CODE[s.dtype] | _CODE[d.dtype] << 32))
+    return flat
+
+
+def _refuse_overlap(src: list[torch.Tensor], dst: list[torch.Tensor]) -> None:
+    """Every output must own its memory: blocks write them in no fixed order."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in dst if t.numel())
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise RuntimeError("gradients to be clipped overlap in memory")
+    if src is dst:
+        return
+    starts = [s[0] for s in spans]
+    from bisect import bisect_left
+
+    for s, d in zip(src, dst):
+        if not s.numel() or s.data_ptr() == d.data_ptr():
+            continue
+        lo, hi = s.data_ptr(), s.data_ptr() + s.numel() * s.element_size()
+        at = bisect_left(starts, hi) - 1
+        if at >= 0 and spans[at][1] > lo:
+            raise RuntimeError("gradients overlap the tensors they are clipped into")
+
+
+def _unique(tensors: Iterable[torch.Tensor]) -> list[torch.Tensor]:
+    seen: set[int] = set()
+    return [t for t in tensors if not (id(t) in seen or seen.add(id(t)))]
+
+
+def _workspace(n: int, device: torch.device) -> torch.Tensor:
+    return torch.empty(int(N.lib().muon_clip_workspace_bytes(n)), dtype=torch.uint8, device=device)
+
+
+def _raise_nonfinite(total: torch.Tensor, norm_type: float) -> None:
+    if not torch.isfinite(total).item():
+        raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients from `parameters` is "
+                           "non-finite, so it cannot be clipped. To disable this error and scale the "
+                           "gradients by the non-finite norm anyway, set `error_if_nonfinite=False`")
+
+
+@torch.no_grad()
+def get_total_norm(tensors: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2.0,
+                   error_if_nonfinite: bool = False, foreach: bool | None = None) -> torch.Tensor:
+    """Norm of all elements of ``tensors`` together, a 0-d fp32 tensor.
+    ``foreach`` is accepted for torch's signature and changes nothing."""
+    kind = _norm_kind(norm_type)
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not tensors:
+        return torch.tensor(0.0)
+    index = _check_grads(tensors, "tensors")
+    tensors = [t if _dense_storage(t) else t.contiguous() for t in tensors]
+
+    def call():
+        total = torch.empty((), dtype=torch.float32, device=tensors[0].device)
+        table, work = _table(tensors, tensors), _workspace(len(tensors), total.device)
+        N.check(N.lib().muon_total_norm(table.buffer_info()[0], len(tensors), kind, work.data_ptr(), total.data_ptr(),
+                                        torch.cuda.current_stream().cuda_stream), "muon_total_norm")
+        return total
+
+    total = _on_device(index, call)
+    if error_if_nonfinite:
+        _raise_nonfinite(total, norm_type)
+    return total
+
+
+def _apply(grads: list[torch.Tensor], outs: list[torch.Tensor], max_norm: float, norm_type: float | None,
+           total: torch.Tensor | None) -> torch.Tensor:
+    """Norm (unless given) and scaling of dense-storage tensors."""
+    index = _check_grads(grads, "gradients")
+    if outs is not grads:
+        _check_grads(outs, "outputs")
+        if outs[0].device != grads[0].device:
+            raise RuntimeError("gradients and outputs must be on one device")
+    _refuse_overlap(grads, outs)
+
+    def call():
+        lib, stream = N.lib(), torch.cuda.current_stream().cuda_stream
+        table = _table(grads, outs)
+        if total is not None:
+            N.check(lib.muon_scale_grads(table.buffer_info()[0], len(grads), max_norm, total.data_ptr(), stream),
+                    "muon_scale_grads")
+            return total
+        norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+        work = _workspace(len(grads), norm.device)
+        N.check(lib.muon_clip_grads(table.buffer_info()[0], len(grads), _norm_kind(norm_type), max_norm,
+                                    work.data_ptr(), norm.data_ptr(), stream), "muon_clip_grads")
+        return norm
+
+    return _on_device(index, call)
+
+
+def _max_norm(max_norm: float) -> float:
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must be >= 0, got {max_norm}")
+    return max_norm
+
+
+def _clip(grads: list[torch.Tensor], outs: list[torch.Tensor] | None, max_norm: float, norm_type: float | None,
+          total: torch.Tensor | None) -> torch.Tensor:
+    if outs is None:
+        outs = grads
+    if all(g.is_contiguous() for g in grads) and (outs is grads or all(o.is_contiguous() for o in outs)):
+        return _apply(grads, outs, max_norm, norm_type, total)
+    # Other strides: elementwise work needs only that both sides agree on the
+    # order of elements, else a contiguous copy is scaled and copied back.
+    src, dst, back = [], [], []
+    for g, o in zip(grads, outs):
+        if any(n > 1 and s == 0 for s, n in zip(o.stride(), o.shape)):
+            raise RuntimeError("an expanded tensor cannot be clipped in place: several elements share memory")
+        if g.stride() == o.stride() and _dense_storage(g):
+            src.append(g)
+            dst.append(o)
+            continue
+        src.append(g.contiguous())
+        if o.is_contiguous():
+            dst.append(o)
+        else:
+            dst.append(torch.empty(o.shape, dtype=o.dtype, device=o.device))
+            back.append((o, dst[-1]))
+    norm = _apply(src, dst, max_norm, norm_type, total)
+    for o, d in back:
+        o.copy_(d)
+    return norm
+
+
+@torch.no_grad()
+def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *, norm_type: float = 2.0,
+               out: Iterable[torch.Tensor] | None = None) -> torch.Tensor:
+    """Scale ``grads`` by min(max_norm / (total + 1e-6), 1), in place or into
+    ``out`` (same shapes, bfloat16 or float32 each), and return the total
+    norm of ``grads``, a 0-d fp32 tensor. In place, a tensor that appears
+    twice counts and is scaled once."""
+    max_norm = _max_norm(max_norm)
+    _norm_kind(norm_type)
+    grads = list(grads)
+    if out is None:
+        grads = _unique(grads)
+    else:
+        out = list(out)
+        if len(out) != len(grads) or any(o.shape != g.shape for o, g in zip(out, grads)):
+            raise ValueError("out must match the gradients in number and shapes")
+    if not grads:
+        return torch.tensor(0.0)
+    return _clip(grads, out, max_norm, norm_type, None)
+
+
+def _parameter_grads(parameters) -> list[torch.Tensor]:
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    return _unique(p.grad for p in _unique(parameters) if p.grad is not None)
+
+
+def _merged(grad: torch.Tensor) -> torch.Tensor:
+    """Values of a sparse gradient with each row's entries added up."""
+    return rows_of(grad).values
+
+
+def rows_of(grad: torch.Tensor) -> RowGrad:
+    """A sparse COO gradient (sparse in its first dimension) as a RowGrad:
+    entries of the same row, as accumulated passes or ``nn.Embedding(sparse=
+    True)`` leave them, are added by the sorted-token kernel."""
+    if grad.layout is not torch.sparse_coo or grad.sparse_dim() != 1 or grad.dense_dim() < 1:
+        raise RuntimeError("sparse gradients must be COO tensors, sparse in their first dimension only")
+    ids, values = grad._indices()[0], grad._values()
+    if grad.is_coalesced():
+        return RowGrad(grad.shape[0], ids.contiguous(), values.contiguous())
+    flat = values.reshape(values.shape[0], math.prod(values.shape[1:]))
+    rows = embedding_row_grad(flat, ids, grad.shape[0])
+    rows.values = rows.values.view(rows.values.shape[0], *values.shape[1:])
+    return rows
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False, foreach: bool | None = None) -> torch.Tensor:
+    """``torch.nn.utils.clip_grad_norm_`` in two kernel launches: clips the
+    parameters' gradients in place and returns their total norm (fp32). A
+    sparse COO gradient counts with its entries of one row added up, and has
+    its values scaled."""
+    max_norm = _max_norm(max_norm)
+    _norm_kind(norm_type)
+    grads = _parameter_grads(parameters)
+    if not grads:
+        return torch.tensor(0.0)
+    sparse = any(g.layout is not torch.strided for g in grads)
+    if not sparse and not error_if_nonfinite:
+        return _clip(grads, None, max_norm, norm_type, None)
+    total = get_total_norm([g if g.layout is torch.strided else _merged(g) for g in grads], norm_type,
+                           error_if_nonfinite)
+    _clip([g if g.layout is torch.strided else g._values() for g in grads], None, max_norm, None, total)
+    return total
+
+
+@torch.no_grad()
+def clip_grads_with_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float,
+                          total_norm: torch.Tensor, foreach: bool | None = None) -> None:
+    """Scale the parameters' gradients in place by min(max_norm / (total_norm
+    + 1e-6), 1), for a norm known already (one reduced over ranks, say).
+    ``total_norm``: a one-element fp32 tensor on the gradients' device."""
+    max_norm = _max_norm(max_norm)
+    grads = _parameter_grads(parameters)
+    if not grads:
+        return
+    if total_norm.numel() != 1 or total_norm.dtype != torch.float32 or total_norm.device != grads[0].device:
+        raise RuntimeError("total_norm must be one float32 value on the gradients' device")
+    _clip([g if g.layout is torch.strided else g._values() for g in grads], None, max_norm, None, total_norm)
+
+
+@torch.no_grad()
+def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor], exp_avg_sqs: list[torch.Tensor],
+          steps: list[float], *, lr: float, beta1: float, beta2: float, eps: float, weight_decay: float) -> None:
+    """One AdamW update of each parameter, in place with its fp32 moments
+    (``MuonAdamW``'s AdamW group, decoupled weight decay). ``grads``: dense
+    tensors, or RowGrads for parameters whose gradient is zero outside some
+    rows: the same results at the cost of those rows. ``steps``: the step
+    count of each, this step included."""
+    from .muon_adamw import _engine_for
+
+    if not len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(steps):
+        raise ValueError("adamw lists must have one entry per parameter")
+    if not params:
+        return
+    for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
+        if isinstance(g, RowGrad):
+            continue  # checked by the engine
+        if not isinstance(g, torch.Tensor) or g.layout is not torch.strided or g.shape != p.shape:
+            raise RuntimeError("adamw takes a dense gradient of its parameter's shape, or a RowGrad")
+        if any(t.dtype != torch.float32 or t.shape != p.shape or not t.is_contiguous() for t in (m, v)):
+            raise RuntimeError("AdamW moments must be contiguous float32 tensors of their parameter's shape")
+    items = [AdamItem(*it) for it in zip(params, grads, exp_avgs, exp_avg_sqs, map(float, steps))]
+    index = _device_index(params[0])
+    engine = _engine_for(params[0].device, "fp16")
+    _on_device(index, lambda: engine.adamw(items, lr=float(lr), beta1=float(beta1), beta2=float(beta2),
+                                           eps=float(eps), weight_decay=float(weight_decay)))

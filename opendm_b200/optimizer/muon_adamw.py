@@ -64,6 +64,13 @@ The arithmetic runs in the sm_100a kernels of ``libopendm_muon.so`` through
   on request; ``last_grad_norm`` holds the total norm of the last clip. With
   Muon matrices in FSDP shards ``step()`` refuses ``max_grad_norm``: the norm
   must then be reduced across ranks, which FSDP's own ``clip_grad_norm_`` does.
+* ``sparse_grads``: False (default: a sparse gradient raises, as in the
+  reference) or True: AdamW-group parameters may have sparse COO gradients,
+  sparse in their first dimension (``opendm_b200.embedding`` or
+  ``torch.nn.Embedding`` with ``sparse=True``). Entries of one row are added
+  by the sorted-token kernel, and the update equals the one on the dense
+  gradient, which is never formed: rows without entries take a zero gradient,
+  so their moments decay and weight decay applies as ever.
 * ``allgather``: "nccl" (default) or "p2p": the flat parameter buckets live
   in peer-mapped memory and each rank pulls its peers' buckets with
   copy-engine memcpys ordered by cross-GPU flags (``opendm_b200.p2p``), so
@@ -86,9 +93,11 @@ from dataclasses import dataclass
 import torch
 import torch.distributed as dist
 
+from .. import embedding as emb
 from .. import trace
 from ..engine import AdamItem, CudaMuonEngine, MatrixItem, effective_lr
 from ..sharding import FlatAdamShards, FlatParamBuckets, assign_owners, assign_waves
+from .functional import clip_grad_norm_, rows_of
 
 _MUON_SHAPE = "_opendm_muon_shape"
 _MUON_NAME = "_opendm_muon_name"
@@ -224,7 +233,7 @@ class MuonAdamW(torch.optim.Optimizer):
                  allgather_waves: int | None = None, allgather_wave_ratio: float = 0.7, comm_sms: int = 32,
                  allgather: str = "nccl",
                  fsdp_owner_ns: bool = True, max_grad_norm: float | None = None, adamw_sharding: bool = False,
-                 _engine=None) -> None:
+                 sparse_grads: bool = False, _engine=None) -> None:
         adamw_params, muon_params, muon_shapes, muon_names = [], [], [], []
         for param in model.parameters():
             if not param.requires_grad:
@@ -282,6 +291,10 @@ class MuonAdamW(torch.optim.Optimizer):
             raise ValueError("adamw_sharding needs state_sharding=True (each rank keeps only its range of the "
                              "AdamW moments current)")
         self.adamw_sharding = bool(adamw_sharding)
+        if sparse_grads and adamw_sharding:
+            raise ValueError("sparse_grads needs adamw_sharding=False (ranges of rows are not split over ranks)")
+        self.sparse_grads = bool(sparse_grads)
+        self._row_grads: dict = {}  # parameter -> RowGrad, of the step under way
         self._adam_shards: dict[int, FlatAdamShards | None] = {}
         self._adam_pending: list[FlatAdamShards] = []  # ranges updated this step, all-gather not yet queued
         self._adam_handles: list = []
@@ -373,7 +386,18 @@ class MuonAdamW(torch.optim.Optimizer):
         return self._engine
 
     def _grads_for_clip(self) -> list[torch.Tensor]:
-        return [p.grad for g in self.param_groups for p in g["params"] if p.grad is not None]
+        """Every gradient; of a sparse one (``sparse_grads``), its merged rows."""
+        rows = self._row_grads or self._merge_row_grads()
+        return [rows[p].values if p in rows else p.grad
+                for g in self.param_groups for p in g["params"] if p.grad is not None]
+
+    def _merge_row_grads(self) -> dict:
+        """RowGrads of the AdamW parameters with sparse gradients."""
+        if not self.sparse_grads:
+            return {}
+        emb.poll_errors(self._device_for_params(self.param_groups[0]["params"]))
+        return {p: rows_of(p.grad) for g in self.param_groups if not g.get("use_muon", False)
+                for p in g["params"] if p.grad is not None and p.grad.is_sparse}
 
     @torch.no_grad()
     def clip_grad_norm_(self, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False,
@@ -387,14 +411,18 @@ class MuonAdamW(torch.optim.Optimizer):
         tensor, bf16 when every gradient is bf16, as torch's). Other norm
         types, or parameters split over ranks (FSDP, whose own
         ``clip_grad_norm_`` reduces across ranks), run torch's function."""
-        grads = self._grads_for_clip()
+        grads = [p.grad for g in self.param_groups for p in g["params"] if p.grad is not None]
         if not grads:
             return torch.tensor(0.0)
         fused = float(norm_type) == 2.0 and grads[0].device.type == "cuda" and not self._split_over_ranks()
         if not fused:
             params = [p for g in self.param_groups for p in g["params"]]
+            if self.sparse_grads and any(g.is_sparse for g in grads) and not self._split_over_ranks():
+                return clip_grad_norm_(params, max_norm, norm_type, error_if_nonfinite, foreach)
             return torch.nn.utils.clip_grad_norm_(params, max_norm, norm_type, error_if_nonfinite, foreach)
         engine = self._get_engine(grads[0].device)
+        if self.sparse_grads:
+            grads = self._grads_for_clip()
         out = engine.clip_grad_norm(grads, float(max_norm))
         res_dtype = torch.bfloat16 if all(g.dtype == torch.bfloat16 for g in grads) else torch.float32
         total = out[0].to(res_dtype)
@@ -417,6 +445,16 @@ class MuonAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        try:
+            self._row_grads = self._merge_row_grads()
+            self._clipped_step()
+        finally:
+            self._row_grads = {}
+        if self.sparse_grads:
+            emb.record_error_check(self._device_for_params(self.param_groups[0]["params"]))
+        return loss
+
+    def _clipped_step(self) -> None:
         if self.max_grad_norm is not None and self._pending_clip is None:
             if self._split_over_ranks():
                 raise RuntimeError("max_grad_norm needs parameters replicated on every rank; with FSDP shards "
@@ -433,7 +471,6 @@ class MuonAdamW(torch.optim.Optimizer):
         finally:
             if engine is not None:
                 engine.grad_scale = None
-        return loss
 
     def _step_groups(self) -> None:
         # Muon groups first, then AdamW: the groups update disjoint parameters,
@@ -498,14 +535,16 @@ class MuonAdamW(torch.optim.Optimizer):
             grad = param.grad
             if grad is None:
                 continue
-            if grad.is_sparse:
+            rows = self._row_grads.get(param)
+            if grad.is_sparse and rows is None:
                 raise RuntimeError("MuonAdamW does not support sparse gradients.")
             state = self._state_for_param(param, self.state[param])
             hs = self._host_step(param, state) + 1.0
             self._host_steps[param] = hs
             step_tensors.append(state["step"])
             if pieces is None:
-                items.append(AdamItem(param.data, grad.detach(), state["exp_avg"], state["exp_avg_sq"], hs))
+                items.append(AdamItem(param.data, grad.detach() if rows is None else rows, state["exp_avg"],
+                                      state["exp_avg_sq"], hs))
                 continue
             if grad.numel() != param.numel():
                 raise RuntimeError("AdamW gradient shape mismatch.")
@@ -1004,5 +1043,7 @@ class MuonAdamW(torch.optim.Optimizer):
 
     def check_device_errors(self) -> None:
         """Synchronise and raise if a kernel recorded a device error."""
+        if self.sparse_grads:
+            emb.check_errors()
         if self._engine is not None and hasattr(self._engine, "check_errors"):
             self._engine.check_errors(block=True)
