@@ -209,12 +209,13 @@ struct AdamwRowsArgs {
   const float* grad_scale;
 };
 
-template <typename P, typename G, bool kVector>
+// kVector: param and moments are 16-byte aligned; four consecutive elements
+// may span rows. kGradVector: they never do, and rows of values are aligned too.
+template <typename P, typename G, bool kVector, bool kGradVector>
 __global__ void __launch_bounds__(ADAM_THREADS) adamw_rows_kernel(P* __restrict__ param, const G* __restrict__ values,
                                                                   const AdamwRowsArgs a) {
   // slot of each of the block's rows (at most ADAM_CHUNK + 1, when dim is 1), or -1
   extern __shared__ int32_t slots[];
-  constexpr int kPer = kVector ? ADAM_VEC : 1;
   const int64_t e0 = int64_t(blockIdx.x) * ADAM_CHUNK;
   const int64_t e1 = min(e0 + ADAM_CHUNK, a.numel);
   const int64_t row0 = e0 / a.dim, row1 = (e1 - 1) / a.dim + 1;
@@ -236,60 +237,70 @@ __global__ void __launch_bounds__(ADAM_THREADS) adamw_rows_kernel(P* __restrict_
   const bool pbf = sizeof(P) == 2, gbf = sizeof(G) == 2;
   const float coef = a.grad_scale ? *a.grad_scale : 1.f;
   const int len = static_cast<int>(e1 - e0);
-  for (int o = threadIdx.x * kPer; o < len; o += ADAM_THREADS * kPer) {
-    const int64_t e = e0 + o;
-    float p[kPer], m[kPer], v[kPer], g[kPer];
-    if constexpr (kVector) {
-      load4(param + e, p);
-      load4(a.exp_avg + e, m);
-      load4(a.exp_avg_sq + e, v);
-    } else {
-      p[0] = load1(param + e);
-      m[0] = a.exp_avg[e];
-      v[0] = a.exp_avg_sq[e];
-    }
-    const uint32_t at = col0 + o, r = at / dim, col = at - r * dim;
+  auto element = [&](int o) {  // gradient of element o of the block
+    const uint32_t at = col0 + o, r = at / dim;
     const int32_t slot = slots[r];
+    return slot < 0 ? 0.f : load1(values + int64_t(slot) * a.dim + (at - r * dim));
+  };
+  auto update = [&](float& p, float g, float& m, float& v) {
+    if (a.grad_scale) g = clip_grad_adam(g, coef, gbf);
+    p = adam_elem(p, g, m, v, a.beta1w, a.beta2, a.one_minus_beta2, a.eps, a.wd_factor, a.neg_step, a.bc2_sqrt, pbf);
+  };
+  const int body = kVector ? len / ADAM_VEC * ADAM_VEC : 0;
+  for (int o = threadIdx.x * ADAM_VEC; o < body; o += ADAM_THREADS * ADAM_VEC) {
+    const int64_t e = e0 + o;
+    float p[4], m[4], v[4], g[4] = {};
+    load4(param + e, p);
+    load4(a.exp_avg + e, m);
+    load4(a.exp_avg_sq + e, v);
+    const uint32_t at = col0 + o, r = at / dim, col = at - r * dim;
+    if (kGradVector || col + 3 < dim) {
+      const int32_t slot = slots[r];
+      if (slot >= 0) {
+        const G* row = values + int64_t(slot) * a.dim + col;
+        if constexpr (kGradVector) {
+          load4(row, g);
+        } else {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) g[i] = 0.f;
-    if (slot >= 0) {
-      if constexpr (kVector)
-        load4(values + int64_t(slot) * a.dim + col, g);
-      else
-        g[0] = load1(values + int64_t(slot) * a.dim + col);
-    }
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if (a.grad_scale) g[i] = clip_grad_adam(g[i], coef, gbf);
-      p[i] = adam_elem(p[i], g[i], m[i], v[i], a.beta1w, a.beta2, a.one_minus_beta2, a.eps, a.wd_factor, a.neg_step,
-                       a.bc2_sqrt, pbf);
-    }
-    if constexpr (kVector) {
-      store4(a.exp_avg + e, m);
-      store4(a.exp_avg_sq + e, v);
-      store4(param + e, p);
+          for (int i = 0; i < 4; ++i) g[i] = load1(row + i);
+        }
+      }
     } else {
-      a.exp_avg[e] = m[0];
-      a.exp_avg_sq[e] = v[0];
-      store1(param + e, p[0]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) g[i] = element(o + i);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) update(p[i], g[i], m[i], v[i]);
+    store4(a.exp_avg + e, m);
+    store4(a.exp_avg_sq + e, v);
+    store4(param + e, p);
+  }
+  for (int o = body + threadIdx.x; o < len; o += ADAM_THREADS) {
+    const int64_t e = e0 + o;
+    float p = load1(param + e), m = a.exp_avg[e], v = a.exp_avg_sq[e];
+    update(p, element(o), m, v);
+    a.exp_avg[e] = m;
+    a.exp_avg_sq[e] = v;
+    store1(param + e, p);
   }
 }
 
 template <typename P, typename G>
 int run_adamw_rows(const muon_adamw_rows_seg& sg, const AdamwRowsArgs& a, cudaStream_t stream) {
-  const bool vec = sg.dim % ADAM_VEC == 0 &&
-                   ((reinterpret_cast<uintptr_t>(sg.param) | reinterpret_cast<uintptr_t>(sg.values) |
-                     reinterpret_cast<uintptr_t>(sg.exp_avg) | reinterpret_cast<uintptr_t>(sg.exp_avg_sq)) & 15u) == 0;
+  const bool vec = ((reinterpret_cast<uintptr_t>(sg.param) | reinterpret_cast<uintptr_t>(sg.exp_avg) |
+                     reinterpret_cast<uintptr_t>(sg.exp_avg_sq)) & 15u) == 0;
+  const bool grad_vec = vec && sg.dim % ADAM_VEC == 0 && (reinterpret_cast<uintptr_t>(sg.values) & 15u) == 0;
   const int64_t blocks = (a.numel + ADAM_CHUNK - 1) / ADAM_CHUNK;
   if (blocks > 0x7fffffffLL) return set_error(MUON_ERR_ARG, "too many AdamW chunks");
   const size_t smem = sizeof(int32_t) * size_t(ADAM_CHUNK / sg.dim + 2);
   P* p = static_cast<P*>(sg.param);
   const G* g = static_cast<const G*>(sg.values);
-  if (vec)
-    adamw_rows_kernel<P, G, true><<<unsigned(blocks), ADAM_THREADS, smem, stream>>>(p, g, a);
+  if (grad_vec)
+    adamw_rows_kernel<P, G, true, true><<<unsigned(blocks), ADAM_THREADS, smem, stream>>>(p, g, a);
+  else if (vec)
+    adamw_rows_kernel<P, G, true, false><<<unsigned(blocks), ADAM_THREADS, smem, stream>>>(p, g, a);
   else
-    adamw_rows_kernel<P, G, false><<<unsigned(blocks), ADAM_THREADS, smem, stream>>>(p, g, a);
+    adamw_rows_kernel<P, G, false, false><<<unsigned(blocks), ADAM_THREADS, smem, stream>>>(p, g, a);
   return check_cuda(cudaGetLastError(), "adamw rows launch");
 }
 

@@ -4,13 +4,13 @@
 //   gradient  dW[v]  = round(scale * sum_{t: ids[t] = v} dY[t])
 //
 // Lookup: a gather bound by HBM (rows in, rows out) for a batch, by latency for a
-// few tokens. A block takes 1024 groups of 8 elements in output order, each
-// thread four of them with their loads in flight together.
+// few tokens.
 //
 // Gradient. The tokens are sorted by id (stable, so a row's tokens keep their
 // order), then summed:
 //   1. sort. Ids left out (padding, out of range) get the key `rows`, which
-//      sorts last and is dropped.
+//      sorts last and is dropped. Up to 1024 tokens in one block, up to
+//      32768 in a cluster of eight, more by tiles over the GPU.
 //   2. sum. The sorted tokens are cut into chunks of C positions; a warp takes
 //      one chunk and 256 columns and adds the rows of dY in sorted order in
 //      fp32 registers, writing a row of dW where the key changes. A run of
@@ -20,6 +20,8 @@
 //   3. join. Each long run's partial rows are added in chunk order.
 // Every sum's order depends on the sorted tokens alone: no floating-point
 // atomics, two calls give the same bits.
+
+#include <cooperative_groups.h>
 
 #include "common.cuh"
 #include "internal.h"
@@ -74,45 +76,74 @@ __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 constexpr int LK_THREADS = 256;
 constexpr int LK_PER = 4;
 
-// `group` consecutive elements per unit: 8 (vector path) or 1.
-template <typename W, typename O, bool kVector>
+// Rows of whole 8-element groups (16-byte aligned): a block takes 1024
+// groups in output order.
+template <typename W, typename O>
 __global__ void __launch_bounds__(LK_THREADS) lookup_kernel(const W* __restrict__ weight, int64_t rows, int64_t ld,
                                                             const void* __restrict__ ids, bool wide, int64_t tokens,
-                                                            uint32_t units, int64_t dim, float scale,
-                                                            O* __restrict__ out, int* err) {
+                                                            uint32_t groups, float scale, O* __restrict__ out,
+                                                            int* err) {
+  constexpr int kWords = sizeof(W) / 2;  // 16-byte words of a group
   const int64_t base = int64_t(blockIdx.x) * (LK_THREADS * LK_PER);
-  const int64_t row0 = base / units;
-  const uint32_t col0 = uint32_t(base - row0 * units);
-  float v[LK_PER][kVector ? kVec : 1];
-  int64_t dst[LK_PER];
+  const int64_t row0 = base / groups;
+  const uint32_t col0 = uint32_t(base - row0 * groups);
+  const int64_t left = tokens * groups - base;
+  uint4 raw[LK_PER][kWords];
 #pragma unroll
   for (int i = 0; i < LK_PER; ++i) {
-    const uint32_t c = col0 + i * LK_THREADS + threadIdx.x;
-    const uint32_t over = c / units;
-    const int64_t t = row0 + over;
-    const int64_t col = int64_t(c - over * units) * (kVector ? kVec : 1);
-    dst[i] = t < tokens ? t * dim + col : -1;
-    if (t >= tokens) continue;
-    const int64_t id = load_id(ids, wide, t);
+    const uint32_t o = i * LK_THREADS + threadIdx.x, c = col0 + o, over = c / groups;
+    if (o >= left) continue;
+    const uint32_t group = c - over * groups;
+    const int64_t id = load_id(ids, wide, row0 + over);
     if (id < 0 || id >= rows) {
 #pragma unroll
-      for (int k = 0; k < (kVector ? kVec : 1); ++k) v[i][k] = 0.f;
-      if (col == 0) record_error(err, MUON_DEV_BAD_INDEX);
-    } else if constexpr (kVector) {
-      load8(weight + id * ld + col, v[i]);
+      for (int q = 0; q < kWords; ++q) raw[i][q] = make_uint4(0, 0, 0, 0);
+      if (group == 0) record_error(err, MUON_DEV_BAD_INDEX);
     } else {
-      v[i][0] = load1(weight + id * ld + col);
+      const uint4* src = reinterpret_cast<const uint4*>(weight + id * ld) + int64_t(group) * kWords;
+#pragma unroll
+      for (int q = 0; q < kWords; ++q) raw[i][q] = src[q];
     }
   }
 #pragma unroll
   for (int i = 0; i < LK_PER; ++i) {
-    if (dst[i] < 0) continue;
+    const uint32_t o = i * LK_THREADS + threadIdx.x;
+    if (o >= left) continue;
+    float v[kVec];
+    load8(reinterpret_cast<const W*>(raw[i]), v);
 #pragma unroll
-    for (int k = 0; k < (kVector ? kVec : 1); ++k) v[i][k] *= scale;
-    if constexpr (kVector)
-      store8(out + dst[i], v[i]);
-    else
-      store1(out + dst[i], v[i][0]);
+    for (int k = 0; k < kVec; ++k) v[k] *= scale;
+    store8(out + (base + o) * kVec, v);
+  }
+}
+
+// Other rows: a warp takes up to 1024 columns of one token, eight single
+// elements a lane at a time (no division per element).
+constexpr int LK_COLS = 1024;
+
+template <typename W, typename O>
+__global__ void __launch_bounds__(LK_THREADS) lookup_rows_kernel(const W* __restrict__ weight, int64_t rows,
+                                                                 int64_t ld, const void* __restrict__ ids, bool wide,
+                                                                 int64_t tokens, int64_t dim, int64_t parts,
+                                                                 float scale, O* __restrict__ out, int* err) {
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = int64_t(blockIdx.x) * (LK_THREADS / 32) + (threadIdx.x >> 5);
+  const int64_t t = unit / parts, part = unit - t * parts;
+  if (t >= tokens) return;
+  const int64_t id = load_id(ids, wide, t);
+  const bool ok = id >= 0 && id < rows;
+  if (!ok && part == 0 && lane == 0) record_error(err, MUON_DEV_BAD_INDEX);
+  const int64_t c0 = part * LK_COLS;
+  const int n = static_cast<int>(min(int64_t(LK_COLS), dim - c0));
+  const W* src = weight + (ok ? id * ld : 0) + c0;
+  O* dst = out + t * dim + c0;
+  for (int base = lane; base < n; base += 32 * kVec) {
+    float v[kVec];
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) v[k] = ok && base + 32 * k < n ? load1(src + base + 32 * k) : 0.f;
+#pragma unroll
+    for (int k = 0; k < kVec; ++k)
+      if (base + 32 * k < n) store1(dst + base + 32 * k, v[k] * scale);
   }
 }
 
@@ -121,43 +152,43 @@ int run_lookup(const void* weight, int64_t rows, int64_t dim, int64_t ld, const 
                float scale, void* out, int* err, cudaStream_t stream) {
   const bool vec = dim % kVec == 0 && ld % kVec == 0 &&
                    ((reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
-  const int64_t units = vec ? dim / kVec : dim;
-  const int64_t blocks = (tokens * units + LK_THREADS * LK_PER - 1) / (LK_THREADS * LK_PER);
+  const int64_t groups = dim / kVec, parts = (dim + LK_COLS - 1) / LK_COLS;
+  const int64_t units = vec ? tokens * groups : tokens * parts, per = vec ? LK_THREADS * LK_PER : LK_THREADS / 32;
+  const int64_t blocks = (units + per - 1) / per;
   if (blocks > 0x7fffffffLL) return set_error(MUON_ERR_ARG, "embedding output too large");
   const unsigned grid = static_cast<unsigned>(blocks);
+  const W* w = static_cast<const W*>(weight);
+  O* o = static_cast<O*>(out);
   if (vec)
-    lookup_kernel<W, O, true><<<grid, LK_THREADS, 0, stream>>>(static_cast<const W*>(weight), rows, ld, ids, wide,
-                                                               tokens, static_cast<uint32_t>(units), dim, scale,
-                                                               static_cast<O*>(out), err);
+    lookup_kernel<W, O><<<grid, LK_THREADS, 0, stream>>>(w, rows, ld, ids, wide, tokens,
+                                                         static_cast<uint32_t>(groups), scale, o, err);
   else
-    lookup_kernel<W, O, false><<<grid, LK_THREADS, 0, stream>>>(static_cast<const W*>(weight), rows, ld, ids, wide,
-                                                                tokens, static_cast<uint32_t>(units), dim, scale,
-                                                                static_cast<O*>(out), err);
+    lookup_rows_kernel<W, O><<<grid, LK_THREADS, 0, stream>>>(w, rows, ld, ids, wide, tokens, dim, parts, scale, o,
+                                                              err);
   return check_cuda(cudaGetLastError(), "embedding launch");
 }
 
 // -------------------------------------------------------------------- sort
 // Least-significant-digit radix sort of (key, position), digits of at most 9
-// bits: 2 passes for vocabularies below 2^18. A pass is three launches: digit
-// counts per tile, their scan, and the stable scatter.
-constexpr int RS_THREADS = 256;
-constexpr int RS_WARPS = RS_THREADS / 32;
-constexpr int RS_PER = 8;
-constexpr int RS_TILE = RS_THREADS * RS_PER;
+// bits: two passes for vocabularies below 2^18. A warp ranks its keys 32 at a
+// time: equal digits find each other with a ballot per bit (16384 tokens in one
+// block took 44 us so, and 49 us with match_any), so the order of equal keys
+// is kept.
 constexpr int RS_BITS = 9;
 constexpr int RS_BINS = 1 << RS_BITS;
+constexpr int RS_THREADS = 1024;
+constexpr int RS_WARPS = RS_THREADS / 32;
+constexpr int RS_MAX_PASSES = 4;
 
-struct SortSource {
-  const void* ids;  // pass 0: token ids
+struct TokenSource {
+  const void* ids;
   bool wide;
   int64_t rows;
   int64_t padding;
-  const uint32_t* keys;  // later passes
-  const uint32_t* pos;
 };
 
 // Key of token t: its id, or `rows` when it takes no part.
-__device__ __forceinline__ uint32_t token_key(const SortSource& s, int64_t t, int* err) {
+__device__ __forceinline__ uint32_t token_key(const TokenSource& s, int64_t t, int* err) {
   const int64_t id = load_id(s.ids, s.wide, t);
   if (id < 0 || id >= s.rows) {
     if (err) record_error(err, MUON_DEV_BAD_INDEX);
@@ -166,159 +197,420 @@ __device__ __forceinline__ uint32_t token_key(const SortSource& s, int64_t t, in
   return id == s.padding ? static_cast<uint32_t>(s.rows) : static_cast<uint32_t>(id);
 }
 
-__global__ void __launch_bounds__(RS_THREADS) radix_count_kernel(SortSource s, int64_t n, int shift, int bits,
-                                                                 uint32_t* __restrict__ hist, uint32_t* long_count,
-                                                                 int* err) {
+__device__ __forceinline__ uint32_t warp_inclusive(uint32_t x) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint32_t up = __shfl_up_sync(0xffffffffu, x, off);
+    if (lane >= off) x += up;
+  }
+  return x;
+}
+
+// Exclusive prefix over a block of RS_THREADS threads; `sums` holds RS_WARPS words.
+__device__ __forceinline__ uint32_t block_exclusive(uint32_t x, uint32_t* sums, uint32_t* total = nullptr) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t inc = warp_inclusive(x);
+  if (lane == 31) sums[warp] = inc;
+  __syncthreads();
+  const uint32_t mine = sums[lane];
+  const uint32_t all = warp_inclusive(mine);
+  const uint32_t before = __shfl_sync(0xffffffffu, all - mine, warp);
+  if (total) *total = __shfl_sync(0xffffffffu, all, 31);
+  __syncthreads();
+  return before + inc - x;
+}
+
+// Lanes whose `d` (of RS_BITS bits) equals this lane's.
+__device__ __forceinline__ uint32_t equal_digits(uint32_t d) {
+  uint32_t peers = 0xffffffffu;
+#pragma unroll
+  for (int b = 0; b < RS_BITS; ++b) {
+    const bool set = (d >> b) & 1u;
+    const uint32_t votes = __ballot_sync(0xffffffffu, set);
+    peers &= set ? votes : ~votes;
+  }
+  return peers;
+}
+
+// Stable ranks of a warp's kPer x 32 digits within the warp; counts[digit] ends as the warp's count.
+template <int kPer, typename Get>
+__device__ __forceinline__ void warp_ranks(uint16_t* counts, uint32_t (&rank)[kPer], Get&& digit) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t d = digit(i);
+    const uint32_t peers = equal_digits(d);
+    const uint32_t before = __popc(peers & ((1u << lane) - 1u));
+    const uint32_t count = counts[d];
+    __syncwarp();
+    if (before == 0) counts[d] = static_cast<uint16_t>(count + __popc(peers));
+    __syncwarp();
+    rank[i] = count + before;
+  }
+}
+
+// counts[warp][bin] -> how many keys of that bin the warps before hold; returns the bin's total (threads below
+// RS_BINS; 0 otherwise).
+__device__ __forceinline__ uint32_t scan_warps(uint16_t (*counts)[RS_BINS]) {
+  uint32_t run = 0;
+  if (threadIdx.x < RS_BINS) {
+    uint16_t c[RS_WARPS];
+#pragma unroll
+    for (int w = 0; w < RS_WARPS; ++w) c[w] = counts[w][threadIdx.x];
+#pragma unroll
+    for (int w = 0; w < RS_WARPS; ++w) {
+      counts[w][threadIdx.x] = static_cast<uint16_t>(run);
+      run += c[w];
+    }
+  }
+  return run;
+}
+
+__device__ __forceinline__ void clear_counts(uint16_t (*counts)[RS_BINS]) {
+  uint32_t* words = reinterpret_cast<uint32_t*>(counts);
+#pragma unroll
+  for (int i = 0; i < RS_WARPS * RS_BINS / 2 / RS_THREADS; ++i) words[i * RS_THREADS + threadIdx.x] = 0;
+}
+
+constexpr int HD_TILE = 4096;  // positions that share one entry of tile_base
+
+// Run starts among a block's sorted keys (element e0 + 32 i of the warp), as
+// ballots; `prev` gives the key before a position.
+template <int kPer, typename Prev>
+__device__ __forceinline__ uint32_t run_heads(const uint32_t (&key)[kPer], uint32_t rows, uint32_t (&heads)[kPer],
+                                              Prev&& prev) {
+  uint32_t mine = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t before = prev(i);
+    heads[i] = __ballot_sync(0xffffffffu, key[i] != before && key[i] < rows);
+    mine += __popc(heads[i]);
+  }
+  return mine;
+}
+
+// Sort of up to RS_THREADS tokens in one block, with the run starts counted
+// on the way out.
+__global__ void __launch_bounds__(RS_THREADS) block_sort_kernel(TokenSource src, int n, int passes, int bits,
+                                                                int chunk, uint32_t* __restrict__ out_keys,
+                                                                uint32_t* __restrict__ out_pos,
+                                                                uint32_t* __restrict__ chunk_base,
+                                                                uint32_t* __restrict__ tile_base,
+                                                                uint32_t* __restrict__ long_count,
+                                                                int64_t* __restrict__ row_count, int* err) {
+  __shared__ uint32_t skey[RS_THREADS];
+  __shared__ uint16_t spos[RS_THREADS];
+  __shared__ uint16_t counts[RS_WARPS][RS_BINS];
+  __shared__ uint16_t base[RS_BINS];
+  __shared__ uint32_t sums[RS_WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = threadIdx.x;
+  const uint32_t rows = static_cast<uint32_t>(src.rows), mask = (1u << bits) - 1u;
+  uint32_t key[1] = {e < n ? token_key(src, e, err) : 0xffffffffu};  // places past n sort last: all digits highest
+  uint32_t pos = e;
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * bits;
+    clear_counts(counts);
+    __syncthreads();
+    uint32_t rank[1];
+    const uint32_t d = (key[0] >> shift) & mask;
+    warp_ranks<1>(counts[warp], rank, [&](int) { return d; });
+    __syncthreads();
+    const uint32_t first = block_exclusive(scan_warps(counts), sums);
+    if (threadIdx.x < RS_BINS) base[threadIdx.x] = static_cast<uint16_t>(first);
+    __syncthreads();
+    const uint32_t to = base[d] + counts[warp][d] + rank[0];
+    skey[to] = key[0];
+    spos[to] = static_cast<uint16_t>(pos);
+    __syncthreads();
+    key[0] = skey[e];
+    pos = spos[e];
+  }
+  uint32_t heads[1], total;
+  const uint32_t mine = run_heads<1>(key, rows, heads, [&](int) { return e > 0 ? skey[e - 1] : 0xffffffffu; });
+  if (e < n) {
+    out_keys[e] = key[0];
+    out_pos[e] = pos;
+  }
+  uint32_t before = block_exclusive(lane == 0 ? mine : 0, sums, &total);
+  before = __shfl_sync(0xffffffffu, before, 0);  // run starts before this warp's first position
+  if (e < n && e % chunk == 0) chunk_base[e / chunk] = before + __popc(heads[0] & ((1u << lane) - 1u));
+  if (threadIdx.x == 0) {
+    tile_base[0] = 0;
+    *long_count = 0;
+    if (row_count) *row_count = total;
+  }
+}
+
+// The same by a cluster of eight blocks for up to 8 x RS_THREADS x kPer
+// tokens: the digit totals cross the blocks through distributed shared
+// memory, the scattered keys through L2 (one block alone needs 44 us for
+// 16384 tokens, bound by its instruction issue).
+constexpr int CL_BLOCKS = 8;
+
+template <int kPer>
+__global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(RS_THREADS)
+    cluster_sort_kernel(TokenSource src, int n, int passes, int bits, int chunk, uint32_t* keys0, uint32_t* pos0,
+                        uint32_t* keys1, uint32_t* pos1, uint32_t* __restrict__ chunk_base,
+                        uint32_t* __restrict__ tile_base, uint32_t* __restrict__ long_count,
+                        int64_t* __restrict__ row_count, int* err) {
+  __shared__ uint16_t counts[RS_WARPS][RS_BINS];
+  __shared__ uint32_t totals[RS_BINS];
+  __shared__ uint32_t base[RS_BINS];
+  __shared__ uint32_t sums[RS_WARPS];
+  __shared__ uint32_t block_heads;
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const unsigned block = cluster.block_rank();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int e0 = int(block) * RS_THREADS * kPer + warp * 32 * kPer + lane;
+  const uint32_t rows = static_cast<uint32_t>(src.rows), mask = (1u << bits) - 1u;
+  uint32_t key[kPer], pos[kPer];  // element e0 + 32 i
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = e0 + 32 * i;
+    key[i] = e < n ? token_key(src, e, err) : 0xffffffffu;
+    pos[i] = e;
+  }
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * bits;
+    clear_counts(counts);
+    __syncthreads();
+    uint32_t rank[kPer];
+    warp_ranks<kPer>(counts[warp], rank, [&](int i) { return (key[i] >> shift) & mask; });
+    __syncthreads();
+    const uint32_t mine = scan_warps(counts);
+    if (threadIdx.x < RS_BINS) totals[threadIdx.x] = mine;
+    cluster.sync();
+    uint32_t all = 0, before = 0;
+    if (threadIdx.x < RS_BINS) {
+#pragma unroll
+      for (unsigned q = 0; q < CL_BLOCKS; ++q) {
+        const uint32_t c = *cluster.map_shared_rank(&totals[threadIdx.x], q);
+        all += c;
+        if (q < block) before += c;
+      }
+    }
+    const uint32_t first = block_exclusive(all, sums);
+    if (threadIdx.x < RS_BINS) base[threadIdx.x] = first + before;
+    __syncthreads();
+    uint32_t* out_keys = p & 1 ? keys1 : keys0;
+    uint32_t* out_pos = p & 1 ? pos1 : pos0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t d = (key[i] >> shift) & mask;
+      const uint32_t to = base[d] + counts[warp][d] + rank[i];
+      if (to < uint32_t(n)) {  // the places past n stay behind
+        out_keys[to] = key[i];
+        out_pos[to] = pos[i];
+      }
+    }
+    cluster.sync();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {  // written by other SMs: past this one's L1
+      const int e = e0 + 32 * i;
+      key[i] = e < n ? __ldcg(out_keys + e) : 0xffffffffu;
+      if (p + 1 < passes) pos[i] = e < n ? __ldcg(out_pos + e) : 0;
+    }
+  }
+  const uint32_t* sorted = (passes - 1) & 1 ? keys1 : keys0;
+  uint32_t heads[kPer], total = 0, before_block = 0;
+  const uint32_t mine = run_heads<kPer>(key, rows, heads, [&](int i) {
+    const int e = e0 + 32 * i;
+    const uint32_t up = __shfl_up_sync(0xffffffffu, key[i], 1);
+    return lane > 0 ? up : (e > 0 && e < n ? __ldcg(sorted + e - 1) : 0xffffffffu);
+  });
+  uint32_t before = block_exclusive(lane == 0 ? mine : 0, sums, &total);
+  if (threadIdx.x == 0) block_heads = total;
+  cluster.sync();
+  total = 0;
+#pragma unroll
+  for (unsigned q = 0; q < CL_BLOCKS; ++q) {
+    const uint32_t h = *cluster.map_shared_rank(&block_heads, q);
+    total += h;
+    if (q < block) before_block += h;
+  }
+  before = __shfl_sync(0xffffffffu, before, 0) + before_block;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = e0 + 32 * i;
+    if (e < n && e % chunk == 0) chunk_base[e / chunk] = before + __popc(heads[i] & ((1u << lane) - 1u));
+    before += __popc(heads[i]);
+  }
+  if (block == 0) {
+    if (int(threadIdx.x) * HD_TILE < n) tile_base[threadIdx.x] = 0;
+    if (threadIdx.x == 0) {
+      *long_count = 0;
+      if (row_count) *row_count = total;
+    }
+  }
+  cluster.sync();  // no block leaves while another reads its shared memory
+}
+
+// Larger sorts: digit counts of every tile for the first pass, then one
+// scatter a pass. A scatter block adds the tiles' counts itself (its first
+// positions are the sums over the smaller digits and the tiles before it)
+// and counts the next pass's digits by destination tile as it writes.
+constexpr int RS_PER = 4;
+constexpr int RS_TILE = RS_THREADS * RS_PER;
+
+__global__ void __launch_bounds__(RS_THREADS) radix_count_kernel(TokenSource src, int64_t n, int bits, int passes,
+                                                                 int64_t tiles, uint32_t* __restrict__ hist,
+                                                                 uint32_t* __restrict__ zeroed, int* err) {
   __shared__ uint32_t h[RS_BINS];
-  const int bins = 1 << bits;
-  for (int b = threadIdx.x; b < bins; b += RS_THREADS) h[b] = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *long_count = 0;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x < RS_BINS) {
+    h[threadIdx.x] = 0;
+    for (int p = 1; p < passes; ++p) hist[(p * tiles + blockIdx.x) * RS_BINS + threadIdx.x] = 0;
+  }
+  if (blockIdx.x == 0 && threadIdx.x < 2) zeroed[threadIdx.x] = 0;
   __syncthreads();
   const int64_t base = int64_t(blockIdx.x) * RS_TILE;
 #pragma unroll
   for (int i = 0; i < RS_PER; ++i) {
     const int64_t t = base + i * RS_THREADS + threadIdx.x;
-    if (t < n) {
-      const uint32_t key = s.keys ? s.keys[t] : token_key(s, t, err);
-      atomicAdd(&h[(key >> shift) & (bins - 1)], 1u);
-    }
+    const uint32_t d = t < n ? token_key(src, t, err) & ((1u << bits) - 1u) : 0;
+    const uint32_t peers = equal_digits(d) & __ballot_sync(0xffffffffu, t < n);
+    if (t < n && lane == __ffs(peers) - 1)  // one add for the warp's equal digits
+      atomicAdd(&h[d], static_cast<uint32_t>(__popc(peers)));
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < bins; b += RS_THREADS) hist[int64_t(blockIdx.x) * RS_BINS + b] = h[b];
+  if (threadIdx.x < RS_BINS) hist[int64_t(blockIdx.x) * RS_BINS + threadIdx.x] = h[threadIdx.x];
 }
 
-// hist[tile][bin] -> first output position of that tile's keys of that bin.
-__global__ void __launch_bounds__(RS_BINS) radix_scan_kernel(uint32_t* __restrict__ hist, int64_t tiles, int bits) {
-  __shared__ uint32_t warp_sum[RS_BINS / 32];
-  const int bin = threadIdx.x, bins = 1 << bits, lane = bin & 31, warp = bin >> 5;
-  uint32_t total = 0;
-  if (bin < bins)
-    for (int64_t t = 0; t < tiles; ++t) total += hist[t * RS_BINS + bin];
-  uint32_t inc = total;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const uint32_t up = __shfl_up_sync(0xffffffffu, inc, off);
-    if (lane >= off) inc += up;
-  }
-  if (lane == 31) warp_sum[warp] = inc;
-  __syncthreads();
-  uint32_t run = inc - total;
-  for (int w = 0; w < warp; ++w) run += warp_sum[w];
-  if (bin < bins)
-    for (int64_t t = 0; t < tiles; ++t) {
-      const uint32_t c = hist[t * RS_BINS + bin];
-      hist[t * RS_BINS + bin] = run;
-      run += c;
-    }
-}
-
-__global__ void __launch_bounds__(RS_THREADS) radix_scatter_kernel(SortSource s, int64_t n, int shift, int bits,
-                                                                   const uint32_t* __restrict__ first,
+__global__ void __launch_bounds__(RS_THREADS) radix_scatter_kernel(TokenSource src, const uint32_t* __restrict__ keys,
+                                                                   const uint32_t* __restrict__ positions, int64_t n,
+                                                                   int shift, int bits, int64_t tiles,
+                                                                   const uint32_t* __restrict__ hist,
+                                                                   uint32_t* __restrict__ next_hist,
                                                                    uint32_t* __restrict__ out_keys,
                                                                    uint32_t* __restrict__ out_pos) {
-  __shared__ uint32_t h[RS_WARPS][RS_BINS];
-  const int bins = 1 << bits, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int b = lane; b < bins; b += 32) h[warp][b] = 0;
-  __syncwarp();
-  const int64_t base = int64_t(blockIdx.x) * RS_TILE + warp * (32 * RS_PER) + lane;
+  __shared__ uint16_t counts[RS_WARPS][RS_BINS];
+  __shared__ uint32_t half[2][RS_BINS];
+  __shared__ uint32_t base[RS_BINS];
+  __shared__ uint32_t sums[RS_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t e0 = int64_t(blockIdx.x) * RS_TILE + warp * 32 * RS_PER + lane;
+  const uint32_t mask = (1u << bits) - 1u;
   uint32_t key[RS_PER], pos[RS_PER], rank[RS_PER];
 #pragma unroll
   for (int i = 0; i < RS_PER; ++i) {
-    const int64_t t = base + i * 32;
-    if (t < n) {
-      key[i] = s.keys ? s.keys[t] : token_key(s, t, nullptr);
-      pos[i] = s.keys ? s.pos[t] : static_cast<uint32_t>(t);
+    const int64_t e = e0 + 32 * i;
+    key[i] = 0xffffffffu;
+    pos[i] = static_cast<uint32_t>(e);
+    if (e < n) {
+      key[i] = keys ? keys[e] : token_key(src, e, nullptr);
+      if (keys) pos[i] = positions[e];
     }
   }
-#pragma unroll
-  for (int i = 0; i < RS_PER; ++i) {
-    const bool in = base + i * 32 < n;
-    const uint32_t d = in ? (key[i] >> shift) & (bins - 1) : 0xffffffffu;
-    const uint32_t peers = __match_any_sync(0xffffffffu, d);
-    const uint32_t before = __popc(peers & ((1u << lane) - 1u));
-    uint32_t count = 0;
-    if (in) count = h[warp][d];
-    __syncwarp();
-    if (in && before == 0) h[warp][d] = count + __popc(peers);
-    __syncwarp();
-    rank[i] = count + before;
+  clear_counts(counts);
+  // this tile's first position of every digit: two threads a bin, half of the tiles each
+  const int bin = threadIdx.x & (RS_BINS - 1), part = threadIdx.x / RS_BINS;
+  uint32_t before = 0, total = 0;
+  const int64_t mid = (tiles + 1) / 2;
+#pragma unroll 8
+  for (int64_t t = part ? mid : 0; t < (part ? tiles : mid); ++t) {
+    const uint32_t c = hist[t * RS_BINS + bin];
+    total += c;
+    if (t < int64_t(blockIdx.x)) before += c;
   }
+  if (part) half[0][bin] = before, half[1][bin] = total;
   __syncthreads();
-  for (int b = threadIdx.x; b < bins; b += RS_THREADS) {
-    uint32_t run = first[int64_t(blockIdx.x) * RS_BINS + b];
-#pragma unroll
-    for (int w = 0; w < RS_WARPS; ++w) {
-      const uint32_t c = h[w][b];
-      h[w][b] = run;
-      run += c;
-    }
-  }
+  if (!part) before += half[0][bin], total += half[1][bin];
+  warp_ranks<RS_PER>(counts[warp], rank, [&](int i) { return (key[i] >> shift) & mask; });
+  const uint32_t first = block_exclusive(part ? 0 : total, sums);
+  if (!part) base[bin] = first + before;
+  scan_warps(counts);
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < RS_PER; ++i) {
-    if (base + i * 32 >= n) continue;
-    const uint32_t to = h[warp][(key[i] >> shift) & (bins - 1)] + rank[i];
-    out_keys[to] = key[i];
-    out_pos[to] = pos[i];
+    const bool in = e0 + 32 * i < n;
+    const uint32_t d = (key[i] >> shift) & mask;
+    const uint32_t to = base[d] + counts[warp][d] + rank[i];
+    if (in) {
+      out_keys[to] = key[i];
+      out_pos[to] = pos[i];
+    }
+    if (next_hist) {  // one add for the lanes whose next digit and tile are those of the first lane of that digit
+      const uint32_t d2 = (key[i] >> (shift + bits)) & mask, tile = to / RS_TILE;
+      const uint32_t peers = equal_digits(d2) & __ballot_sync(0xffffffffu, in);
+      const int leader = in ? __ffs(peers) - 1 : lane;
+      const bool same = __shfl_sync(0xffffffffu, tile, leader) == tile;
+      const uint32_t joined = peers & __ballot_sync(0xffffffffu, in && same);
+      if (in && (lane == leader || !same))
+        atomicAdd(&next_hist[tile * RS_BINS + d2], lane == leader ? static_cast<uint32_t>(__popc(joined)) : 1u);
+    }
   }
 }
 
-// ------------------------------------------------------------------- heads
-// Row form: how many runs start before each chunk. chunk_base[c] counts the
-// run starts between the chunk's tile of HD_TILE positions and the chunk;
-// tile_heads[t] the run starts in tile t.
-constexpr int HD_THREADS = 256;
-constexpr int HD_TILE = 4096;
+// How many runs start before each chunk: chunk_base[c] within the chunk's
+// tile of HD_TILE positions, tile_base[t] before the tile (by the last block to
+// finish), and their number.
+constexpr int HD_THREADS = 1024;
 
 __global__ void __launch_bounds__(HD_THREADS) heads_kernel(const uint32_t* __restrict__ keys, int64_t n,
                                                            uint32_t rows, int chunk, uint32_t* __restrict__ chunk_base,
-                                                           uint32_t* __restrict__ tile_heads) {
-  constexpr int kPer = HD_TILE / HD_THREADS;  // consecutive positions per thread
-  __shared__ uint32_t warp_sum[HD_THREADS / 32];
+                                                           uint32_t* tile_base, uint32_t* ticket,
+                                                           int64_t* __restrict__ row_count) {
+  constexpr int kWarps = HD_THREADS / 32, kRounds = HD_TILE / HD_THREADS;
+  __shared__ uint32_t warp_sum[kWarps];
+  __shared__ uint32_t last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t base = int64_t(blockIdx.x) * HD_TILE + int64_t(threadIdx.x) * kPer;
-  uint32_t flags = 0;
-  uint32_t prev = base > 0 && base < n ? keys[base - 1] : 0xffffffffu;
-  for (int i = 0; i < kPer && base + i < n; ++i) {
-    const uint32_t k = keys[base + i];
-    if (k != prev && k < rows) flags |= 1u << i;
-    prev = k;
-  }
-  const uint32_t mine = __popc(flags);
-  uint32_t inc = mine;
+  const int64_t e0 = int64_t(blockIdx.x) * HD_TILE + warp * 32 * kRounds + lane;
+  uint32_t heads[kRounds], key[kRounds];
 #pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const uint32_t up = __shfl_up_sync(0xffffffffu, inc, off);
-    if (lane >= off) inc += up;
-  }
-  if (lane == 31) warp_sum[warp] = inc;
+  for (int i = 0; i < kRounds; ++i) key[i] = e0 + 32 * i < n ? keys[e0 + 32 * i] : 0xffffffffu;
+  const uint32_t edge = lane == 0 && e0 > 0 && e0 <= n ? keys[e0 - 1] : 0xffffffffu;  // before the warp's first
+  const uint32_t mine = run_heads<kRounds>(key, rows, heads, [&](int i) {
+    const uint32_t up = __shfl_up_sync(0xffffffffu, key[i], 1);
+    const uint32_t wrap = i > 0 ? __shfl_sync(0xffffffffu, key[i > 0 ? i - 1 : 0], 31) : edge;
+    return lane > 0 ? up : wrap;
+  });
+  if (lane == 0) warp_sum[warp] = mine;
   __syncthreads();
-  uint32_t before = inc - mine;
-  for (int w = 0; w < warp; ++w) before += warp_sum[w];
-  for (int i = 0; i < kPer; ++i)
-    if (base + i < n && (base + i) % chunk == 0)
-      chunk_base[(base + i) / chunk] = before + __popc(flags & ((1u << i) - 1u));
-  if (threadIdx.x == HD_THREADS - 1) tile_heads[blockIdx.x] = before + mine;
+  uint32_t before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += warp_sum[w];
+    total += warp_sum[w];
+  }
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const int64_t e = e0 + 32 * i;
+    if (e < n && e % chunk == 0) chunk_base[e / chunk] = before + __popc(heads[i] & ((1u << lane) - 1u));
+    before += __popc(heads[i]);
+  }
+  if (threadIdx.x == 0) {
+    tile_base[blockIdx.x] = total;
+    __threadfence();
+    last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  uint32_t run = 0;
+  for (unsigned t0 = 0; t0 < gridDim.x; t0 += HD_THREADS) {
+    const unsigned t = t0 + threadIdx.x;
+    const uint32_t x = t < gridDim.x ? *reinterpret_cast<volatile uint32_t*>(tile_base + t) : 0;
+    const uint32_t inc = warp_inclusive(x);
+    __syncthreads();
+    if (lane == 31) warp_sum[warp] = inc;
+    __syncthreads();
+    uint32_t pre = run + inc - x;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) pre += warp_sum[w];
+      run += warp_sum[w];
+    }
+    if (t < gridDim.x) tile_base[t] = pre;
+  }
+  if (threadIdx.x == 0 && row_count) *row_count = run;
 }
 
 // --------------------------------------------------------------------- sum
 constexpr int SUM_THREADS = 256;
 constexpr int SUM_WARPS = SUM_THREADS / 32;
-
-template <bool kVector, typename T>
-__device__ __forceinline__ void load_cols(const T* row, int64_t col, int64_t dim, int lane, float (&v)[kVec]) {
-  if constexpr (kVector) {
-    if (col < dim) {
-      load8(row + col, v);
-    } else {
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) v[k] = 0.f;
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) v[k] = col + 32 * k < dim ? load1(row + col + 32 * k) : 0.f;
-  }
-}
+constexpr int SUM_STAGE_BYTES = 4096;  // rows in flight of one warp
+constexpr int ZERO_ROWS = 16;          // rows one warp of the zero part looks after
 
 template <bool kVector, typename T>
 __device__ __forceinline__ void store_cols(T* row, int64_t col, int64_t dim, const float (&v)[kVec]) {
@@ -340,139 +632,229 @@ struct SumArgs {
   int chunk;
   int64_t chunks;
   int64_t slices;
+  int64_t sum_blocks;
   float scale;
-  const uint32_t* chunk_base;  // row form
-  const uint32_t* tile_heads;
+  const uint32_t* chunk_base;
+  const uint32_t* tile_base;
   int64_t cap;
   int64_t* out_ids;  // NULL: dense form
-  int64_t* count;
+  const int64_t* count;
   float* partial;  // [chunks][2][slices * kSlice]: a run from an earlier chunk; a long run starting here
   uint32_t* long_list;
   uint32_t* long_count;
 };
 
+// First index in keys[lo, hi) whose key is >= `key`, by a whole warp: 32
+// probes a step, four dependent loads for a million tokens.
+__device__ __forceinline__ int64_t warp_lower_bound(const uint32_t* keys, int64_t lo, int64_t hi, int64_t key) {
+  const int lane = threadIdx.x & 31;
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 31) / 32;
+    const int64_t at = lo + int64_t(lane) * step;
+    const bool below = at < hi && int64_t(keys[at]) < key;
+    const int k = __popc(__ballot_sync(0xffffffffu, below));  // the probes below `key` come first
+    if (k == 0) return lo;
+    const int64_t last_below = lo + int64_t(k - 1) * step;
+    hi = min(hi, last_below + step);
+    lo = last_below + 1;
+  }
+  return lo;
+}
+
+// Zeros elements [begin, end) of out, by a warp.
+template <typename O>
+__device__ __forceinline__ void zero_span(O* out, int64_t begin, int64_t end) {
+  constexpr int kPer = 16 / sizeof(O);
+  const int lane = threadIdx.x & 31;
+  const int64_t skew = (reinterpret_cast<uintptr_t>(out) / sizeof(O)) % kPer;  // elements past a 16-byte boundary
+  const int64_t body = min(end, (begin + skew + kPer - 1) / kPer * kPer - skew);
+  for (int64_t e = begin + lane; e < body; e += 32) store1(out + e, 0.f);
+  const int64_t vectors = (end - body) / kPer;
+  uint4* v = reinterpret_cast<uint4*>(out + body);
+  for (int64_t i = lane; i < vectors; i += 32) v[i] = make_uint4(0, 0, 0, 0);
+  for (int64_t e = body + vectors * kPer + lane; e < end; e += 32) store1(out + e, 0.f);
+}
+
+// Rows no token has: in the dense form the gaps between the sorted keys, in
+// the row form those past the count.
+template <typename O>
+__device__ __forceinline__ void zero_rows(O* out, const SumArgs& a, int64_t unit) {
+  const int64_t r0 = unit * ZERO_ROWS;
+  if (a.out_ids) {
+    const int64_t from = max(r0, *a.count), to = min(r0 + ZERO_ROWS, a.cap);
+    if (from >= to) return;
+    zero_span(out, from * a.dim, to * a.dim);
+    const int lane = threadIdx.x & 31;
+    if (from + lane < to) a.out_ids[from + lane] = 0;
+    return;
+  }
+  const int64_t r1 = min(r0 + ZERO_ROWS, a.rows);
+  if (r0 >= r1) return;
+  int64_t at = warp_lower_bound(a.keys, 0, a.n, r0);
+  int64_t row = r0;
+  while (true) {
+    const int64_t key = at < a.n ? min(int64_t(a.keys[at]), r1) : r1;
+    if (key > row) zero_span(out, row * a.dim, key * a.dim);
+    if (key == r1) break;
+    row = key + 1;
+    if (at + 1 < a.n && int64_t(a.keys[at + 1]) != key)
+      ++at;
+    else
+      at = warp_lower_bound(a.keys, at, a.n, row);
+  }
+}
+
+__device__ __forceinline__ void copy_async16(uint32_t shared, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+// Blocks below sum_blocks: one chunk and 256 columns a warp. The rows of dY
+// come through a ring in shared memory (4 KB a warp, filled by asynchronous
+// copies that each lane makes and reads for itself), so few registers are
+// held and seven blocks fit an SM. The other blocks write the zeros.
 template <typename G, typename O, bool kVector>
-__global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ grad, O* __restrict__ out, SumArgs a) {
-  constexpr int kUnroll = sizeof(G) == 2 ? 8 : 4;
-  __shared__ uint32_t red[2][SUM_WARPS];
+__global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ grad, O* __restrict__ out,
+                                                          const SumArgs a) {
+  constexpr int kStages = SUM_STAGE_BYTES / (kSlice * int(sizeof(G)));
+  constexpr int kCopies = kVec * sizeof(G) / 16;
+  __shared__ __align__(16) unsigned char ring[kVector ? SUM_WARPS : 1][kVector ? SUM_STAGE_BYTES : 16];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (int64_t(blockIdx.x) >= a.sum_blocks) {
+    zero_rows(out, a, (int64_t(blockIdx.x) - a.sum_blocks) * SUM_WARPS + warp);
+    return;
+  }
   const int64_t unit = int64_t(blockIdx.x) * SUM_WARPS + warp;
   const int64_t c = unit / a.slices;
+  if (c >= a.chunks) return;
   const int64_t slice = unit - c * a.slices;
   const int64_t s0 = c * a.chunk;
-  uint32_t slot = 0, total = 0;
-  if (a.out_ids) {
-    // distinct rows before this block's first tile, and in all
-    const int64_t tile0 = (int64_t(blockIdx.x) * SUM_WARPS / a.slices) * a.chunk / HD_TILE;
-    const int64_t tiles = (a.n + HD_TILE - 1) / HD_TILE;
-    uint32_t low = 0, all = 0;
-    for (int64_t t = threadIdx.x; t < tiles; t += SUM_THREADS) {
-      const uint32_t h = a.tile_heads[t];
-      all += h;
-      if (t < tile0) low += h;
-    }
-    low = __reduce_add_sync(0xffffffffu, low);
-    all = __reduce_add_sync(0xffffffffu, all);
-    if (lane == 0) red[0][warp] = low, red[1][warp] = all;
-    __syncthreads();
-    for (int w = 0; w < SUM_WARPS; ++w) slot += red[0][w], total += red[1][w];
-    if (c < a.chunks) {
-      for (int64_t t = tile0; t < s0 / HD_TILE; ++t) slot += a.tile_heads[t];
-      slot += a.chunk_base[c];
-    }
-    if (unit == 0 && lane == 0) *a.count = total;
-  }
-  if (c >= a.chunks) return;
   const int len = static_cast<int>(min(int64_t(a.chunk), a.n - s0));
-  const int64_t col = slice * kSlice + (kVector ? lane * kVec : lane);
-  const uint32_t none = 0xffffffffu;
-  // keys and positions of this chunk and the next, one per lane each
-  const uint32_t dropped = static_cast<uint32_t>(a.rows);
   const int64_t s1 = s0 + len;
-  uint32_t key_a = lane < len ? a.keys[s0 + lane] : none;
-  uint32_t pos_a = lane < len ? a.pos[s0 + lane] : 0;
   const int next = static_cast<int>(min(int64_t(a.chunk), a.n - s1));
-  uint32_t key_b = lane < next ? a.keys[s1 + lane] : none;
-  uint32_t pos_b = lane < next ? a.pos[s1 + lane] : 0;
-  if (a.out_ids) {  // this chunk's share of the rows past the count
-    float zero[kVec] = {};
-    for (int i = 0; i < a.chunk; ++i) {
-      const int64_t r = s0 + i;
-      if (r >= int64_t(total) && r < a.cap) {
-        store_cols<kVector>(out + r * a.dim, col, a.dim, zero);
-        if (slice == 0 && lane == 0) a.out_ids[r] = 0;
-      }
-    }
-  }
+  const uint32_t none = 0xffffffffu;
+  const uint32_t dropped = static_cast<uint32_t>(a.rows);
+  // keys and positions of this chunk and the next, one per lane each
+  const uint32_t key_a = lane < len ? a.keys[s0 + lane] : none;
+  const uint32_t key_b = lane < next ? a.keys[s1 + lane] : none;
+  const uint32_t pos_a = lane < len ? a.pos[s0 + lane] : 0;
+  const uint32_t pos_b = lane < next ? a.pos[s1 + lane] : 0;
+  const uint32_t before = s0 > 0 ? a.keys[s0 - 1] : none;
+  const uint32_t before_last = s0 > a.chunk ? a.keys[s0 - a.chunk - 1] : none;
+  uint32_t slot = a.chunk_base[c] + a.tile_base[s0 / HD_TILE];
   const uint32_t first = __shfl_sync(0xffffffffu, key_a, 0);
   const uint32_t last = __shfl_sync(0xffffffffu, key_a, len - 1);
-  const uint32_t before = s0 > 0 ? a.keys[s0 - 1] : none;
+  const uint32_t next_first = __shfl_sync(0xffffffffu, key_b, 0);
+  const uint32_t next_last = __shfl_sync(0xffffffffu, key_b, a.chunk - 1);  // `none` unless the next chunk is full
+  const int valid = __popc(__ballot_sync(0xffffffffu, key_a < dropped));
   const bool whole = len == a.chunk && first == last;
-  int begin = 0;           // first position this warp adds
-  bool lead_partial = false;  // ... belonging to a long run of an earlier chunk
+  int begin = 0;  // first position this warp adds
+  int lead = 0;   // positions of a long run of an earlier chunk
   if (s0 > 0 && before == first) {
-    const bool starts_before_last = s0 - a.chunk > 0 && a.keys[s0 - a.chunk - 1] == first;
-    if (whole || starts_before_last)
-      lead_partial = true;
-    else  // the warp of the chunk before finishes this run
-      begin = __popc(__ballot_sync(0xffffffffu, key_a == first));
+    const int run = __popc(__ballot_sync(0xffffffffu, key_a == first));
+    if (whole || before_last == first)
+      lead = run;
+    else
+      begin = run;  // the warp of the chunk before finishes this run
   }
   // end of the rows this warp adds: the chunk, plus the rest of a run that does not cover the next chunk
   int end = len;
-  bool tail_partial = false;
-  const uint32_t next_first = __shfl_sync(0xffffffffu, key_b, 0);
-  if (begin < len && next > 0 && next_first == last) {
-    const bool from_here = !(lead_partial && whole);  // the last run starts in this chunk
-    const bool next_whole = next == a.chunk && __shfl_sync(0xffffffffu, key_b, a.chunk - 1) == last;
-    if (next_whole)
-      tail_partial = from_here;
-    else if (from_here)
+  bool tail = false;  // a long run starts here
+  if (begin < len && lead < len && next_first == last) {
+    if (next_last == last)
+      tail = true;
+    else
       end = len + __popc(__ballot_sync(0xffffffffu, key_b == last));
   }
-  if (tail_partial && slice == 0 && lane == 0 && last != dropped) a.long_list[atomicAdd(a.long_count, 1u)] = uint32_t(c);
+  if (valid < len) end = valid, tail = false;
+  if (begin >= end) return;
+  if (tail && slice == 0 && lane == 0) a.long_list[atomicAdd(a.long_count, 1u)] = uint32_t(c);
+  // where a run ends
+  const uint32_t after_a = __shfl_down_sync(0xffffffffu, key_a, 1), after_b = __shfl_down_sync(0xffffffffu, key_b, 1);
+  const uint32_t ends_a =
+      __ballot_sync(0xffffffffu, lane < len && key_a != (lane == len - 1 ? next_first : after_a));
+  const uint32_t ends_b = __ballot_sync(0xffffffffu, lane < next && (lane == next - 1 || key_b != after_b));
+  const int64_t col = slice * kSlice + (kVector ? lane * kVec : lane);
   const int64_t pitch = a.slices * kSlice;
-  float* part = a.partial + c * 2 * pitch;
+  float* part = a.partial + c * 2 * pitch + slice * kSlice + lane * kVec;
+
   float acc[kVec] = {};
-  for (int r0 = begin; r0 < end; r0 += kUnroll) {
-    float v[kUnroll][kVec];
-    uint32_t k[kUnroll + 1];
+  auto row_of = [&](int r) {
+    const uint32_t pa = __shfl_sync(0xffffffffu, pos_a, r & 31), pb = __shfl_sync(0xffffffffu, pos_b, (r - len) & 31);
+    return grad + int64_t(r < len ? pa : pb) * a.dim;
+  };
+  auto finish = [&](int r) {  // row r is added: write the sum if its run or this warp's part of it ends here
+    const bool run_ends = r < len ? (ends_a >> r) & 1u : (ends_b >> (r - len)) & 1u;
+    if (!run_ends && r + 1 < end) return;
+    if (r < lead) {
+      store8(part, acc);
+    } else if (tail && r == end - 1) {
+      store8(part + pitch, acc);
+    } else {
 #pragma unroll
-    for (int i = 0; i <= kUnroll; ++i) {
-      const int r = r0 + i;
-      const bool in_b = r >= len;
-      const uint32_t ka = __shfl_sync(0xffffffffu, key_a, r & 31), kb = __shfl_sync(0xffffffffu, key_b, (r - len) & 31);
-      k[i] = in_b ? (r - len < next ? kb : none) : ka;
+      for (int j = 0; j < kVec; ++j) acc[j] *= a.scale;
+      const uint32_t ka = __shfl_sync(0xffffffffu, key_a, r & 31);
+      const uint32_t key = r < len ? ka : last;
+      const int64_t row = a.out_ids ? int64_t(slot) : int64_t(key);
+      store_cols<kVector>(out + row * a.dim, col, a.dim, acc);
+      if (a.out_ids && slice == 0 && lane == 0) a.out_ids[slot] = key;
+      ++slot;
     }
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      const int r = r0 + i;
-      const uint32_t pa = __shfl_sync(0xffffffffu, pos_a, r & 31), pb = __shfl_sync(0xffffffffu, pos_b, (r - len) & 31);
-      if (r < end && k[i] != dropped) load_cols<kVector>(grad + int64_t(r < len ? pa : pb) * a.dim, col, a.dim, lane, v[i]);
-    }
+    for (int j = 0; j < kVec; ++j) acc[j] = 0.f;
+  };
+  if constexpr (kVector) {
+    const bool on = col < a.dim;
+    const uint32_t mine = smem_u32(ring[warp]) + lane * 16;
+    const uint4* mine_read = reinterpret_cast<const uint4*>(ring[warp]) + lane;
+    auto fetch = [&](int r) {
+      const G* row = row_of(r);
+      if (on) {
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      const int r = r0 + i;
-      if (r >= end || k[i] == dropped) continue;
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) acc[j] += v[i][j];
-      const bool run_ends = k[i + 1] != k[i];
-      if (!run_ends && r + 1 < end) continue;
-      if (lead_partial && k[i] == first) {
-        store_cols<true>(part, slice * kSlice + lane * kVec, pitch, acc);
-      } else if (tail_partial && k[i] == last) {
-        store_cols<true>(part + pitch, slice * kSlice + lane * kVec, pitch, acc);
-        ++slot;
-      } else {
-        float w[kVec];
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) w[j] = acc[j] * a.scale;
-        const int64_t row = a.out_ids ? int64_t(slot) : int64_t(k[i]);
-        store_cols<kVector>(out + row * a.dim, col, a.dim, w);
-        if (a.out_ids && slice == 0 && lane == 0) a.out_ids[slot] = k[i];
-        ++slot;
+        for (int q = 0; q < kCopies; ++q)
+          copy_async16(mine + ((r % kStages) * kCopies + q) * 512, row + col + q * (16 / int(sizeof(G))));
       }
+    };
+    for (int r = begin; r < begin + kStages; ++r) {
+      if (r < end) fetch(r);
+      copy_async_commit();
+    }
+    for (int r = begin; r < end; ++r) {
+      copy_async_wait<kStages - 1>();
+      if constexpr (sizeof(G) == 2) {
+        const uint4 x = mine_read[(r % kStages) * 32];
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&x);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) acc[j] = 0.f;
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = __bfloat1622float2(h[j]);
+          acc[2 * j] += f.x;
+          acc[2 * j + 1] += f.y;
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint4 x = mine_read[((r % kStages) * 2 + q) * 32];
+          acc[4 * q] += __uint_as_float(x.x);
+          acc[4 * q + 1] += __uint_as_float(x.y);
+          acc[4 * q + 2] += __uint_as_float(x.z);
+          acc[4 * q + 3] += __uint_as_float(x.w);
+        }
+      }
+      if (r + kStages < end) fetch(r + kStages);
+      copy_async_commit();
+      finish(r);
+    }
+  } else {
+    for (int r = begin; r < end; ++r) {
+      const G* row = row_of(r);
+#pragma unroll
+      for (int k = 0; k < kVec; ++k)
+        if (col + 32 * k < a.dim) acc[k] += load1(row + col + 32 * k);
+      finish(r);
     }
   }
 }
@@ -481,7 +863,7 @@ __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ 
 // One block per (long run, slice): the run's partial rows, split evenly over
 // the warps in chunk order, then the warps' sums in order.
 template <typename O, bool kVector>
-__global__ void __launch_bounds__(SUM_THREADS) join_kernel(O* __restrict__ out, SumArgs a) {
+__global__ void __launch_bounds__(SUM_THREADS) join_kernel(O* __restrict__ out, const SumArgs a) {
   __shared__ float red[SUM_WARPS][kSlice];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t pitch = a.slices * kSlice;
@@ -490,23 +872,17 @@ __global__ void __launch_bounds__(SUM_THREADS) join_kernel(O* __restrict__ out, 
     const int64_t c0 = a.long_list[job / a.slices];
     const int64_t slice = job % a.slices;
     const uint32_t key = a.keys[(c0 + 1) * a.chunk];
-    // last chunk the run reaches: the last c1 whose first key is the run's
-    int64_t lo = c0 + 1, hi = a.chunks - 1;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi + 1) >> 1;
-      if (a.keys[mid * a.chunk] == key)
-        lo = mid;
-      else
-        hi = mid - 1;
-    }
-    const int64_t n_parts = lo - c0 + 1;
+    // the chunks the run reaches: up to the last whose first key is the run's
+    const int64_t stop = (warp_lower_bound(a.keys, (c0 + 1) * a.chunk, a.n, int64_t(key) + 1) - 1) / a.chunk;
+    const int64_t n_parts = stop - c0 + 1;
     const int64_t per = (n_parts + SUM_WARPS - 1) / SUM_WARPS;
     const int64_t p0 = min(n_parts, warp * per), p1 = min(n_parts, p0 + per);
     float acc[kVec] = {};
-    const int64_t off = slice * kSlice + lane * kVec;
+    const float* part = a.partial + c0 * 2 * pitch + slice * kSlice + lane * kVec;
+#pragma unroll 4
     for (int64_t p = p0; p < p1; ++p) {
       float v[kVec];
-      load8(a.partial + ((c0 + p) * 2 + (p == 0 ? 1 : 0)) * pitch + off, v);
+      load8(part + (p * 2 + (p == 0 ? 1 : 0)) * pitch, v);
 #pragma unroll
       for (int j = 0; j < kVec; ++j) acc[j] += v[j];
     }
@@ -514,16 +890,11 @@ __global__ void __launch_bounds__(SUM_THREADS) join_kernel(O* __restrict__ out, 
     __syncthreads();
     if (warp == 0) {
       int64_t row = key;
-      if (a.out_ids) {
-        // the run's row: runs starting before chunk c0's end, less one
-        const int64_t tile = c0 * a.chunk / HD_TILE;
-        uint32_t slot = 0;
-        for (int64_t t = lane; t < tile; t += 32) slot += a.tile_heads[t];
-        slot = __reduce_add_sync(0xffffffffu, slot) + a.chunk_base[c0];
-        // run starts inside chunk c0
+      if (a.out_ids) {  // the run is the last to start in chunk c0
         const int64_t s = c0 * a.chunk + lane;
         const bool head = lane < a.chunk && (s == 0 || a.keys[s - 1] != a.keys[s]);
-        row = int64_t(slot) + __popc(__ballot_sync(0xffffffffu, head)) - 1;
+        row = int64_t(a.tile_base[c0 * a.chunk / HD_TILE]) + a.chunk_base[c0] +
+              __popc(__ballot_sync(0xffffffffu, head)) - 1;
         if (slice == 0 && lane == 0) a.out_ids[row] = key;
       }
       // element j of this lane sits at column lane * 8 + j (vector) or lane + 32 j of the slice, in both
@@ -557,8 +928,10 @@ int chunk_for(int64_t tokens, int64_t slices) {
   return chunk;
 }
 
+constexpr int64_t kClusterSort = CL_BLOCKS * RS_THREADS * 4;  // tokens; more are sorted by tiles
+
 struct GradLayout {
-  int64_t keys[2], pos[2], hist, chunk_base, tile_heads, long_list, long_count, partial, total;
+  int64_t keys[2], pos[2], hist, chunk_base, tile_base, long_list, counters, partial, total;
   int64_t tiles, chunks, slices;
   int chunk;
 };
@@ -576,11 +949,11 @@ GradLayout grad_layout(int64_t n, int64_t dim) {
   l.chunk = chunk_for(n, l.slices);
   l.chunks = (n + l.chunk - 1) / l.chunk;
   for (int i = 0; i < 2; ++i) l.keys[i] = take(4 * n), l.pos[i] = take(4 * n);
-  l.hist = take(4 * l.tiles * RS_BINS);
+  l.hist = take(n > kClusterSort ? 4 * RS_MAX_PASSES * l.tiles * RS_BINS : 0);
   l.chunk_base = take(4 * l.chunks);
-  l.tile_heads = take(4 * ((n + HD_TILE - 1) / HD_TILE));
+  l.tile_base = take(4 * ((n + HD_TILE - 1) / HD_TILE));
   l.long_list = take(4 * l.chunks);
-  l.long_count = take(4);
+  l.counters = take(8);  // long runs, finished blocks of heads_kernel
   l.partial = take(8 * l.chunks * l.slices * kSlice);
   l.total = at;
   return l;
@@ -592,10 +965,12 @@ bool float_type(int dtype) { return dtype == MUON_BF16 || dtype == MUON_F32; }
 bool too_large(int64_t a, int64_t b) { return b > 0 && a > (int64_t(1) << 58) / b; }
 
 template <typename G, typename O>
-int run_sum(const void* grad, void* out, const SumArgs& a, cudaStream_t stream) {
+int run_sum(const void* grad, void* out, SumArgs a, cudaStream_t stream) {
   const bool vec = a.dim % kVec == 0 &&
                    ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
-  const int64_t blocks = (a.chunks * a.slices + SUM_WARPS - 1) / SUM_WARPS;
+  a.sum_blocks = (a.chunks * a.slices + SUM_WARPS - 1) / SUM_WARPS;
+  const int64_t zero_rows = a.out_ids ? a.cap : a.rows;
+  const int64_t blocks = a.sum_blocks + (zero_rows + ZERO_ROWS * SUM_WARPS - 1) / (ZERO_ROWS * SUM_WARPS);
   if (blocks > 0x7fffffffLL) return set_error(MUON_ERR_ARG, "embedding gradient too large");
   const unsigned grid = static_cast<unsigned>(blocks);
   const G* g = static_cast<const G*>(grad);
@@ -674,33 +1049,52 @@ int launch_embedding_grad(const void* grad, int grad_dtype, const void* ids, int
   auto u32 = [&](int64_t off) { return reinterpret_cast<uint32_t*>(base + off); };
   // sort
   const int bits = bits_for(rows), passes = (bits + RS_BITS - 1) / RS_BITS, per = (bits + passes - 1) / passes;
-  SortSource src{ids, ids_dtype == MUON_I64, rows, padding_idx, nullptr, nullptr};
-  const unsigned tiles = static_cast<unsigned>(l.tiles);
+  const TokenSource src{ids, ids_dtype == MUON_I64, rows, padding_idx};
+  uint32_t* counters = u32(l.counters);
+  int64_t* row_count = out_ids ? count : nullptr;
   int cur = 0;
-  for (int p = 0; p < passes; ++p) {
-    radix_count_kernel<<<tiles, RS_THREADS, 0, stream>>>(src, tokens, p * per, per, u32(l.hist), u32(l.long_count),
-                                                         p == 0 ? err : nullptr);
+  if (tokens <= kClusterSort) {
+    const int n = static_cast<int>(tokens);
+    auto cluster_sort = [&](auto kernel) {
+      kernel<<<CL_BLOCKS, RS_THREADS, 0, stream>>>(src, n, passes, per, l.chunk, u32(l.keys[0]), u32(l.pos[0]),
+                                                   u32(l.keys[1]), u32(l.pos[1]), u32(l.chunk_base), u32(l.tile_base),
+                                                   counters, row_count, err);
+      cur = (passes - 1) & 1;
+    };
+    if (n <= RS_THREADS)
+      block_sort_kernel<<<1, RS_THREADS, 0, stream>>>(src, n, passes, per, l.chunk, u32(l.keys[0]), u32(l.pos[0]),
+                                                      u32(l.chunk_base), u32(l.tile_base), counters, row_count, err);
+    else if (n <= CL_BLOCKS * RS_THREADS)
+      cluster_sort(cluster_sort_kernel<1>);
+    else if (n <= CL_BLOCKS * RS_THREADS * 2)
+      cluster_sort(cluster_sort_kernel<2>);
+    else
+      cluster_sort(cluster_sort_kernel<4>);
+    if (check_cuda(cudaGetLastError(), "token sort launch")) return MUON_ERR_CUDA;
+  } else {
+    const unsigned tiles = static_cast<unsigned>(l.tiles);
+    radix_count_kernel<<<tiles, RS_THREADS, 0, stream>>>(src, tokens, per, passes, l.tiles, u32(l.hist), counters,
+                                                         err);
     if (check_cuda(cudaGetLastError(), "radix count launch")) return MUON_ERR_CUDA;
-    radix_scan_kernel<<<1, RS_BINS, 0, stream>>>(u32(l.hist), l.tiles, per);
-    if (check_cuda(cudaGetLastError(), "radix scan launch")) return MUON_ERR_CUDA;
-    radix_scatter_kernel<<<tiles, RS_THREADS, 0, stream>>>(src, tokens, p * per, per, u32(l.hist), u32(l.keys[cur]),
-                                                           u32(l.pos[cur]));
-    if (check_cuda(cudaGetLastError(), "radix scatter launch")) return MUON_ERR_CUDA;
-    src.keys = u32(l.keys[cur]);
-    src.pos = u32(l.pos[cur]);
-    cur ^= 1;
-  }
-  if (out_ids) {
+    const uint32_t *keys = nullptr, *pos = nullptr;
+    for (int p = 0; p < passes; ++p) {
+      cur = p & 1;
+      uint32_t* hist = u32(l.hist) + p * l.tiles * RS_BINS;
+      radix_scatter_kernel<<<tiles, RS_THREADS, 0, stream>>>(src, keys, pos, tokens, p * per, per, l.tiles, hist,
+                                                             p + 1 < passes ? hist + l.tiles * RS_BINS : nullptr,
+                                                             u32(l.keys[cur]), u32(l.pos[cur]));
+      if (check_cuda(cudaGetLastError(), "radix scatter launch")) return MUON_ERR_CUDA;
+      keys = u32(l.keys[cur]);
+      pos = u32(l.pos[cur]);
+    }
     const unsigned grid = static_cast<unsigned>((tokens + HD_TILE - 1) / HD_TILE);
-    heads_kernel<<<grid, HD_THREADS, 0, stream>>>(src.keys, tokens, static_cast<uint32_t>(rows), l.chunk,
-                                                  u32(l.chunk_base), u32(l.tile_heads));
+    heads_kernel<<<grid, HD_THREADS, 0, stream>>>(keys, tokens, static_cast<uint32_t>(rows), l.chunk,
+                                                  u32(l.chunk_base), u32(l.tile_base), counters + 1, row_count);
     if (check_cuda(cudaGetLastError(), "run heads launch")) return MUON_ERR_CUDA;
-  } else if (check_cuda(cudaMemsetAsync(out, 0, out_bytes, stream), "embedding gradient zeros")) {
-    return MUON_ERR_CUDA;
   }
   SumArgs a{};
-  a.keys = src.keys;
-  a.pos = src.pos;
+  a.keys = u32(l.keys[cur]);
+  a.pos = u32(l.pos[cur]);
   a.n = tokens;
   a.rows = rows;
   a.dim = dim;
@@ -709,13 +1103,13 @@ int launch_embedding_grad(const void* grad, int grad_dtype, const void* ids, int
   a.slices = l.slices;
   a.scale = scale;
   a.chunk_base = u32(l.chunk_base);
-  a.tile_heads = u32(l.tile_heads);
+  a.tile_base = u32(l.tile_base);
   a.cap = cap;
   a.out_ids = out_ids;
   a.count = count;
   a.partial = reinterpret_cast<float*>(base + l.partial);
   a.long_list = u32(l.long_list);
-  a.long_count = u32(l.long_count);
+  a.long_count = counters;
   using bf = __nv_bfloat16;
   const bool gb = grad_dtype == MUON_BF16, ob = out_dtype == MUON_BF16;
   if (gb && ob) return run_sum<bf, bf>(grad, out, a, stream);

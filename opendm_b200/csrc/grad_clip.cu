@@ -28,13 +28,16 @@ namespace {
 
 constexpr int GC_THREADS = 256;
 constexpr int GC_VEC = 8;
+constexpr int GC_STEP = GC_THREADS * GC_VEC;  // 2048 elements: one group a thread
+// Groups a thread takes of a chunk: 8 (128 bytes of bf16 in flight a thread),
+// or 1 for lists too short to fill the GPU with such chunks.
 constexpr int GC_ITERS = 8;
-constexpr int64_t GC_CHUNK = int64_t(GC_THREADS) * GC_VEC * GC_ITERS;  // 16384
 constexpr int kMaxSegs = 1024;
-constexpr int kMaxBlocks = 148 * 8;  // partials per launch
+constexpr int kBlocksPerSm = 4;                // resident: the kernels hold at most 64 registers
+constexpr int kMaxBlocks = 148 * kBlocksPerSm;  // one wave; a partial each
 
 template <int N>
-struct ClipTable {
+struct ClipTable {  // chunk_begin, chunks: in the launch's chunk size
   const void* src[N];
   void* dst[N];
   int64_t numel[N];
@@ -58,20 +61,64 @@ __device__ __forceinline__ int find_clip_segment(const ClipTable<N>& t, int chun
   return lo;
 }
 
-__device__ __forceinline__ void load_group(const void* src, bool bf, int64_t e, float (&v)[GC_VEC]) {
-  if (bf) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(src) + e);
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+// A thread's groups of 8 elements (16 bytes of bf16, 32 of fp32) in flight
+// together: 128 bytes either way.
+template <bool kBf>
+struct Batch {
+  static constexpr int kGroups = kBf ? 8 : 4;
+  static constexpr int kWords = kBf ? 1 : 2;
+  uint4 raw[kGroups][kWords];
+
+  // groups first, first + GC_THREADS, ...
+  __device__ __forceinline__ void load(const void* src, int first) {
+    const uint4* p = static_cast<const uint4*>(src) + first * kWords;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __bfloat1622float2(h[i]);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
+    for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+      for (int q = 0; q < kWords; ++q) raw[i][q] = p[i * GC_THREADS * kWords + q];
+  }
+};
+
+template <bool kBf>
+__device__ __forceinline__ void load_group(const void* src, int g, uint4 (&raw)[Batch<kBf>::kWords]) {
+#pragma unroll
+  for (int q = 0; q < Batch<kBf>::kWords; ++q) raw[q] = static_cast<const uint4*>(src)[g * Batch<kBf>::kWords + q];
+}
+
+template <bool kBf>
+__device__ __forceinline__ void unpack(const uint4 (&raw)[Batch<kBf>::kWords], float (&v)[GC_VEC]) {
+  if constexpr (kBf) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw[0]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = __bfloat1622float2(h[k]);
+      v[2 * k] = f.x;
+      v[2 * k + 1] = f.y;
     }
   } else {
-    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(src) + e);
-    const float4 a = p[0], b = p[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      v[4 * q] = __uint_as_float(raw[q].x);
+      v[4 * q + 1] = __uint_as_float(raw[q].y);
+      v[4 * q + 2] = __uint_as_float(raw[q].z);
+      v[4 * q + 3] = __uint_as_float(raw[q].w);
+    }
+  }
+}
+
+// Group `at` of dst = round(v * coef).
+template <bool kBf>
+__device__ __forceinline__ void store_group(void* dst, int at, const float (&v)[GC_VEC], float coef) {
+  if constexpr (kBf) {
+    uint4 raw;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&raw);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) h[k] = __floats2bfloat162_rn(v[2 * k] * coef, v[2 * k + 1] * coef);
+    static_cast<uint4*>(dst)[at] = raw;
+  } else {
+    float4* p = static_cast<float4*>(dst) + at * 2;
+    p[0] = make_float4(v[0] * coef, v[1] * coef, v[2] * coef, v[3] * coef);
+    p[1] = make_float4(v[4] * coef, v[5] * coef, v[6] * coef, v[7] * coef);
   }
 }
 
@@ -85,6 +132,12 @@ __device__ __forceinline__ void store_one(void* dst, bool bf, int64_t e, float x
     reinterpret_cast<__nv_bfloat16*>(dst)[e] = __float2bfloat16_rn(x);
   else
     reinterpret_cast<float*>(dst)[e] = x;
+}
+
+// Elements e, e + GC_THREADS, ... below n (0 past it): unaligned chunks and ends of tensors.
+__device__ __forceinline__ void load_ones(const void* src, bool bf, int e, int n, float (&v)[GC_VEC]) {
+#pragma unroll
+  for (int k = 0; k < GC_VEC; ++k) v[k] = e + k * GC_THREADS < n ? load_one(src, bf, e + k * GC_THREADS) : 0.f;
 }
 
 __device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -140,41 +193,62 @@ __device__ __forceinline__ double block_join(double x, double* shared) {
   return x;
 }
 
-template <int kNorm, int N>
-__global__ void __launch_bounds__(GC_THREADS) list_norm_kernel(const __grid_constant__ ClipTable<N> t,
-                                                               double* __restrict__ partials) {
+// A whole long chunk.
+template <int kNorm, bool kBf>
+__device__ __forceinline__ double norm_chunk(const void* src, double total) {
+#pragma unroll 1
+  for (int g = threadIdx.x; g < GC_ITERS * GC_THREADS; g += Batch<kBf>::kGroups * GC_THREADS) {
+    Batch<kBf> b;
+    b.load(src, g);
+#pragma unroll
+    for (int i = 0; i < Batch<kBf>::kGroups; ++i) {
+      float v[GC_VEC];
+      unpack<kBf>(b.raw[i], v);
+      total = join<kNorm>(total, reduce_values<kNorm, GC_VEC>(v));
+    }
+  }
+  return total;
+}
+
+// The aligned groups of any chunk, one at a time.
+template <int kNorm, bool kBf>
+__device__ __forceinline__ double norm_groups(const void* src, int groups, double total) {
+#pragma unroll 1
+  for (int g = threadIdx.x; g < groups; g += GC_THREADS) {
+    uint4 raw[Batch<kBf>::kWords];
+    load_group<kBf>(src, g, raw);
+    float v[GC_VEC];
+    unpack<kBf>(raw, v);
+    total = join<kNorm>(total, reduce_values<kNorm, GC_VEC>(v));
+  }
+  return total;
+}
+
+template <int kNorm, int N, int kIters>
+__global__ void __launch_bounds__(GC_THREADS, kBlocksPerSm) list_norm_kernel(const __grid_constant__ ClipTable<N> t,
+                                                                             double* __restrict__ partials) {
+  constexpr int kChunk = kIters * GC_STEP;
   __shared__ double red[GC_THREADS / 32];
   double total = 0.0;
   for (int chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
     const int s = find_clip_segment(t, chunk);
-    const void* src = t.src[s];
-    const int64_t numel = t.numel[s];
     const bool bf = t.types[s] & 1;
-    const int64_t e0 = int64_t(chunk - t.chunk_begin[s]) * GC_CHUNK;
-    const int64_t e1 = min(e0 + GC_CHUNK, numel);
-    int64_t done = e0;
+    const int64_t e0 = int64_t(chunk - t.chunk_begin[s]) * kChunk;
+    const char* src = static_cast<const char*>(t.src[s]) + e0 * (bf ? 2 : 4);
+    const int n = static_cast<int>(min(int64_t(kChunk), t.numel[s] - e0));
+    int done = 0;
     if (aligned16(src)) {
-      done = e0 + (e1 - e0) / GC_VEC * GC_VEC;
-      float v[4][GC_VEC];
-#pragma unroll
-      for (int half = 0; half < GC_ITERS / 4; ++half) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t e = e0 + (int64_t(half * 4 + i) * GC_THREADS + threadIdx.x) * GC_VEC;
-          if (e < done) {
-            load_group(src, bf, e, v[i]);
-          } else {
-#pragma unroll
-            for (int k = 0; k < GC_VEC; ++k) v[i][k] = 0.f;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) total = join<kNorm>(total, reduce_values<kNorm, GC_VEC>(v[i]));
-      }
+      if (kIters > 1 && n == kChunk)
+        total = bf ? norm_chunk<kNorm, true>(src, total) : norm_chunk<kNorm, false>(src, total);
+      else
+        total = bf ? norm_groups<kNorm, true>(src, n / GC_VEC, total)
+                   : norm_groups<kNorm, false>(src, n / GC_VEC, total);
+      done = n / GC_VEC * GC_VEC;
     }
-    for (int64_t e = done + threadIdx.x; e < e1; e += GC_THREADS) {
-      const float v[1] = {load_one(src, bf, e)};
-      total = join<kNorm>(total, reduce_values<kNorm, 1>(v));
+    for (int e = done + threadIdx.x; e < n; e += GC_STEP) {
+      float v[GC_VEC];
+      load_ones(src, bf, e, n, v);
+      total = join<kNorm>(total, reduce_values<kNorm, GC_VEC>(v));
     }
   }
   total = block_join<kNorm>(total, red);
@@ -203,11 +277,51 @@ __global__ void __launch_bounds__(GC_THREADS) total_norm_kernel(int kind, const 
   if (threadIdx.x == 0) *total = x;
 }
 
-template <int N>
-__global__ void __launch_bounds__(GC_THREADS) list_scale_kernel(const __grid_constant__ ClipTable<N> t, int kind,
+// A whole long chunk, or any number of aligned groups one at a time.
+template <bool kBf, bool kOutBf, bool kWhole>
+__device__ __forceinline__ void scale_groups(const void* src, void* dst, int groups, float coef) {
+  if constexpr (kWhole) {
+#pragma unroll 1
+    for (int g = threadIdx.x; g < GC_ITERS * GC_THREADS; g += Batch<kBf>::kGroups * GC_THREADS) {
+      Batch<kBf> b;
+      b.load(src, g);
+#pragma unroll
+      for (int i = 0; i < Batch<kBf>::kGroups; ++i) {
+        float v[GC_VEC];
+        unpack<kBf>(b.raw[i], v);
+        store_group<kOutBf>(dst, g + i * GC_THREADS, v, coef);
+      }
+    }
+  } else {
+#pragma unroll 1
+    for (int g = threadIdx.x; g < groups; g += GC_THREADS) {
+      uint4 raw[Batch<kBf>::kWords];
+      load_group<kBf>(src, g, raw);
+      float v[GC_VEC];
+      unpack<kBf>(raw, v);
+      store_group<kOutBf>(dst, g, v, coef);
+    }
+  }
+}
+
+template <bool kWhole>
+__device__ __forceinline__ void scale_groups(const void* src, bool sbf, void* dst, bool dbf, int groups, float coef) {
+  if (sbf && dbf)
+    scale_groups<true, true, kWhole>(src, dst, groups, coef);
+  else if (sbf)
+    scale_groups<true, false, kWhole>(src, dst, groups, coef);
+  else if (dbf)
+    scale_groups<false, true, kWhole>(src, dst, groups, coef);
+  else
+    scale_groups<false, false, kWhole>(src, dst, groups, coef);
+}
+
+template <int N, int kIters>
+__global__ void __launch_bounds__(GC_THREADS, kBlocksPerSm) list_scale_kernel(const __grid_constant__ ClipTable<N> t, int kind,
                                                                 const double* __restrict__ partials, int n_partials,
                                                                 float max_norm, float* __restrict__ total_out,
                                                                 const float* __restrict__ total_in) {
+  constexpr int kChunk = kIters * GC_STEP;
   __shared__ double red[GC_THREADS / 32];
   float total;
   if (partials) {
@@ -223,54 +337,39 @@ __global__ void __launch_bounds__(GC_THREADS) list_scale_kernel(const __grid_con
     const void* src = t.src[s];
     void* dst = t.dst[s];
     if (src == dst && coef == 1.f) continue;
-    const int64_t numel = t.numel[s];
     const bool sbf = t.types[s] & 1, dbf = t.types[s] & 2;
-    const int64_t e0 = int64_t(chunk - t.chunk_begin[s]) * GC_CHUNK;
-    const int64_t e1 = min(e0 + GC_CHUNK, numel);
-    int64_t done = e0;
+    const int64_t e0 = int64_t(chunk - t.chunk_begin[s]) * kChunk;
+    const int n = static_cast<int>(min(int64_t(kChunk), t.numel[s] - e0));
+    src = static_cast<const char*>(src) + e0 * (sbf ? 2 : 4);
+    dst = static_cast<char*>(dst) + e0 * (dbf ? 2 : 4);
+    int done = 0;
     if (aligned16(src) && aligned16(dst)) {
-      done = e0 + (e1 - e0) / GC_VEC * GC_VEC;
-      float v[4][GC_VEC];
-#pragma unroll
-      for (int half = 0; half < GC_ITERS / 4; ++half) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t e = e0 + (int64_t(half * 4 + i) * GC_THREADS + threadIdx.x) * GC_VEC;
-          if (e < done) load_group(src, sbf, e, v[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t e = e0 + (int64_t(half * 4 + i) * GC_THREADS + threadIdx.x) * GC_VEC;
-          if (e >= done) continue;
-          if (dbf) {
-            uint4 raw;
-            __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&raw);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) h[k] = __floats2bfloat162_rn(v[i][2 * k] * coef, v[i][2 * k + 1] * coef);
-            *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(dst) + e) = raw;
-          } else {
-            float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(dst) + e);
-            p[0] = make_float4(v[i][0] * coef, v[i][1] * coef, v[i][2] * coef, v[i][3] * coef);
-            p[1] = make_float4(v[i][4] * coef, v[i][5] * coef, v[i][6] * coef, v[i][7] * coef);
-          }
-        }
-      }
+      if (kIters > 1 && n == kChunk)
+        scale_groups<true>(src, sbf, dst, dbf, 0, coef);
+      else
+        scale_groups<false>(src, sbf, dst, dbf, n / GC_VEC, coef);
+      done = n / GC_VEC * GC_VEC;
     }
-    for (int64_t e = done + threadIdx.x; e < e1; e += GC_THREADS)
-      store_one(dst, dbf, e, load_one(src, sbf, e) * coef);
+    for (int e = done + threadIdx.x; e < n; e += GC_STEP) {
+      float v[GC_VEC];
+      load_ones(src, sbf, e, n, v);
+#pragma unroll
+      for (int k = 0; k < GC_VEC; ++k)
+        if (e + k * GC_THREADS < n) store_one(dst, dbf, e + k * GC_THREADS, v[k] * coef);
+    }
   }
 }
 
 constexpr int64_t kMaxChunks = 0x3fffffff;  // of a whole list
 
-int64_t chunks_of(int64_t numel) { return (numel + GC_CHUNK - 1) / GC_CHUNK; }
+int64_t chunks_of(int64_t numel, int iters) { return (numel + iters * GC_STEP - 1) / (iters * GC_STEP); }
 
 int check_segs(const muon_clip_seg* segs, int64_t n, bool outputs) {
   if (n < 0 || (n > 0 && !segs)) return set_error(MUON_ERR_ARG, "null clip segment table or negative count");
   int64_t chunks = 0;
   for (int64_t i = 0; i < n; ++i) {
     const muon_clip_seg& s = segs[i];
-    if (s.numel < 0 || s.numel > GC_CHUNK * kMaxChunks || (chunks += chunks_of(s.numel)) > kMaxChunks)
+    if (s.numel < 0 || s.numel > kMaxChunks * GC_STEP || (chunks += chunks_of(s.numel, GC_ITERS)) > kMaxChunks)
       return set_error(MUON_ERR_ARG, "clip segment sizes out of range");
     const int es = s.grad_dtype == MUON_BF16 ? 2 : 4;
     if ((s.grad_dtype != MUON_BF16 && s.grad_dtype != MUON_F32) ||
@@ -289,7 +388,7 @@ int check_segs(const muon_clip_seg* segs, int64_t n, bool outputs) {
 
 // Fills `t` with segments from `i` on (empty ones skipped) and returns the next index.
 template <int N>
-int64_t fill_table(ClipTable<N>& t, const muon_clip_seg* segs, int64_t i, int64_t n) {
+int64_t fill_table(ClipTable<N>& t, const muon_clip_seg* segs, int64_t i, int64_t n, int iters) {
   t.n = 0;
   int64_t chunks = 0;
   for (; i < n && t.n < N; ++i) {
@@ -301,7 +400,7 @@ int64_t fill_table(ClipTable<N>& t, const muon_clip_seg* segs, int64_t i, int64_
     t.chunk_begin[t.n] = static_cast<int32_t>(chunks);
     t.types[t.n] = (s.grad_dtype == MUON_BF16 ? 1 : 0) | (s.out_dtype == MUON_BF16 ? 2 : 0);
     ++t.n;
-    chunks += chunks_of(s.numel);
+    chunks += chunks_of(s.numel, iters);
   }
   t.chunks = static_cast<int32_t>(chunks);
   return i;
@@ -309,12 +408,23 @@ int64_t fill_table(ClipTable<N>& t, const muon_clip_seg* segs, int64_t i, int64_
 
 int blocks_for(int chunks) { return chunks < kMaxBlocks ? chunks : kMaxBlocks; }
 
-// Runs `launch(table)` for every batch of the list.
-template <int N, typename F>
+// How a list is launched: its parameter block is copied with every launch, so
+// short lists take a short one.
+constexpr int kShortSegs = 64;
+
+// Long chunks once they give every resident block two.
+int iters_for(const muon_clip_seg* segs, int64_t n) {
+  int64_t chunks = 0;
+  for (int64_t i = 0; i < n; ++i) chunks += chunks_of(segs[i].numel, GC_ITERS);
+  return chunks >= 2 * kMaxBlocks ? GC_ITERS : 1;
+}
+
+// Runs launch(table) for every batch of the list.
+template <int N, int kIters, typename F>
 int for_batches(const muon_clip_seg* segs, int64_t n, F&& launch) {
   ClipTable<N> t;
   for (int64_t i = 0; i < n;) {
-    i = fill_table(t, segs, i, n);
+    i = fill_table(t, segs, i, n, kIters);
     if (t.n == 0) break;
     const int rc = launch(t);
     if (rc != MUON_OK) return rc;
@@ -322,41 +432,52 @@ int for_batches(const muon_clip_seg* segs, int64_t n, F&& launch) {
   return MUON_OK;
 }
 
-template <int N>
+template <int N, int kIters>
 int norm_batches(const muon_clip_seg* segs, int64_t n, int kind, double* partials, int* n_partials,
                  cudaStream_t stream) {
   *n_partials = 0;
-  return for_batches<N>(segs, n, [&](const ClipTable<N>& t) {
+  return for_batches<N, kIters>(segs, n, [&](const ClipTable<N>& t) {
     const int blocks = blocks_for(t.chunks);
     double* out = partials + *n_partials;
     if (kind == MUON_NORM_2)
-      list_norm_kernel<MUON_NORM_2, N><<<blocks, GC_THREADS, 0, stream>>>(t, out);
+      list_norm_kernel<MUON_NORM_2, N, kIters><<<blocks, GC_THREADS, 0, stream>>>(t, out);
     else if (kind == MUON_NORM_1)
-      list_norm_kernel<MUON_NORM_1, N><<<blocks, GC_THREADS, 0, stream>>>(t, out);
+      list_norm_kernel<MUON_NORM_1, N, kIters><<<blocks, GC_THREADS, 0, stream>>>(t, out);
     else
-      list_norm_kernel<MUON_NORM_INF, N><<<blocks, GC_THREADS, 0, stream>>>(t, out);
+      list_norm_kernel<MUON_NORM_INF, N, kIters><<<blocks, GC_THREADS, 0, stream>>>(t, out);
     *n_partials += blocks;
     return check_cuda(cudaGetLastError(), "list norm launch");
   });
 }
 
-template <int N>
+template <int N, int kIters>
 int scale_batches(const muon_clip_seg* segs, int64_t n, int kind, const double* partials, int n_partials,
                   float max_norm, float* total_out, const float* total_in, cudaStream_t stream) {
-  return for_batches<N>(segs, n, [&](const ClipTable<N>& t) {
-    list_scale_kernel<N><<<blocks_for(t.chunks), GC_THREADS, 0, stream>>>(t, kind, partials, n_partials, max_norm,
-                                                                         total_out, total_in);
+  return for_batches<N, kIters>(segs, n, [&](const ClipTable<N>& t) {
+    list_scale_kernel<N, kIters><<<blocks_for(t.chunks), GC_THREADS, 0, stream>>>(t, kind, partials, n_partials,
+                                                                                 max_norm, total_out, total_in);
     total_out = nullptr;  // written by the first batch
     return check_cuda(cudaGetLastError(), "list scale launch");
   });
 }
 
-// The parameter block is copied with every launch: short lists take a short one.
-constexpr int kShortSegs = 64;
-
 int norm_list(const muon_clip_seg* segs, int64_t n, int kind, double* partials, int* n_partials, cudaStream_t stream) {
-  return n <= kShortSegs ? norm_batches<kShortSegs>(segs, n, kind, partials, n_partials, stream)
-                         : norm_batches<kMaxSegs>(segs, n, kind, partials, n_partials, stream);
+  const bool lng = iters_for(segs, n) == GC_ITERS;
+  if (n <= kShortSegs)
+    return lng ? norm_batches<kShortSegs, GC_ITERS>(segs, n, kind, partials, n_partials, stream)
+               : norm_batches<kShortSegs, 1>(segs, n, kind, partials, n_partials, stream);
+  return lng ? norm_batches<kMaxSegs, GC_ITERS>(segs, n, kind, partials, n_partials, stream)
+             : norm_batches<kMaxSegs, 1>(segs, n, kind, partials, n_partials, stream);
+}
+
+int scale_list(const muon_clip_seg* segs, int64_t n, int kind, const double* partials, int n_partials, float max_norm,
+               float* total_out, const float* total_in, cudaStream_t stream) {
+  const bool lng = iters_for(segs, n) == GC_ITERS;
+  auto run = [&](auto batches) {
+    return batches(segs, n, kind, partials, n_partials, max_norm, total_out, total_in, stream);
+  };
+  if (n <= kShortSegs) return lng ? run(scale_batches<kShortSegs, GC_ITERS>) : run(scale_batches<kShortSegs, 1>);
+  return lng ? run(scale_batches<kMaxSegs, GC_ITERS>) : run(scale_batches<kMaxSegs, 1>);
 }
 
 bool all_empty(const muon_clip_seg* segs, int64_t n) {
@@ -396,18 +517,14 @@ int launch_clip_grads(const muon_clip_seg* segs, int64_t n_segs, int norm_kind, 
   double* partials = static_cast<double*>(workspace);
   int n = 0;
   if (int rc = norm_list(segs, n_segs, norm_kind, partials, &n, stream)) return rc;
-  return n_segs <= kShortSegs
-             ? scale_batches<kShortSegs>(segs, n_segs, norm_kind, partials, n, max_norm, total, nullptr, stream)
-             : scale_batches<kMaxSegs>(segs, n_segs, norm_kind, partials, n, max_norm, total, nullptr, stream);
+  return scale_list(segs, n_segs, norm_kind, partials, n, max_norm, total, nullptr, stream);
 }
 
 int launch_scale_grads(const muon_clip_seg* segs, int64_t n_segs, float max_norm, const float* total,
                        cudaStream_t stream) {
   if (!total) return set_error(MUON_ERR_ARG, "null norm");
   if (int rc = check_segs(segs, n_segs, true)) return rc;
-  return n_segs <= kShortSegs
-             ? scale_batches<kShortSegs>(segs, n_segs, 0, nullptr, 0, max_norm, nullptr, total, stream)
-             : scale_batches<kMaxSegs>(segs, n_segs, 0, nullptr, 0, max_norm, nullptr, total, stream);
+  return scale_list(segs, n_segs, 0, nullptr, 0, max_norm, nullptr, total, stream);
 }
 
 }  // namespace muon
