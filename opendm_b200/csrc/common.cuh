@@ -44,6 +44,12 @@ __device__ __forceinline__ unsigned long long global_timer_ns() {
   return t;
 }
 
+// ------------------------------------------- overlapped launches
+// Let the next launch_overlapped() kernel start while this one runs on.
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Wait until the kernels before this one have finished and their writes are visible.
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count)

@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_kernel(const W* __restrict_
 // Other rows: a warp takes up to 1024 columns of one token, eight single
 // elements a lane at a time (no division per element).
 constexpr int LK_COLS = 1024;
+constexpr int LK_LANE = 8;
 
 template <typename W, typename O>
 __global__ void __launch_bounds__(LK_THREADS) lookup_rows_kernel(const W* __restrict__ weight, int64_t rows,
@@ -137,13 +138,23 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_rows_kernel(const W* __rest
   const int n = static_cast<int>(min(int64_t(LK_COLS), dim - c0));
   const W* src = weight + (ok ? id * ld : 0) + c0;
   O* dst = out + t * dim + c0;
-  for (int base = lane; base < n; base += 32 * kVec) {
-    float v[kVec];
+  src += lane;
+  dst += lane;
+  int at = 0;
+  for (; at + 32 * LK_LANE <= n; at += 32 * LK_LANE) {  // without a test per element
+    float v[LK_LANE];
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) v[k] = ok && base + 32 * k < n ? load1(src + base + 32 * k) : 0.f;
+    for (int k = 0; k < LK_LANE; ++k) v[k] = ok ? load1(src + at + 32 * k) : 0.f;
 #pragma unroll
-    for (int k = 0; k < kVec; ++k)
-      if (base + 32 * k < n) store1(dst + base + 32 * k, v[k] * scale);
+    for (int k = 0; k < LK_LANE; ++k) store1(dst + at + 32 * k, v[k] * scale);
+  }
+  if (at < n) {
+    float v[LK_LANE];
+#pragma unroll
+    for (int k = 0; k < LK_LANE; ++k) v[k] = ok && at + lane + 32 * k < n ? load1(src + at + 32 * k) : 0.f;
+#pragma unroll
+    for (int k = 0; k < LK_LANE; ++k)
+      if (at + lane + 32 * k < n) store1(dst + at + 32 * k, v[k] * scale);
   }
 }
 
@@ -304,6 +315,7 @@ __global__ void __launch_bounds__(RS_THREADS) block_sort_kernel(TokenSource src,
   __shared__ uint16_t counts[RS_WARPS][RS_BINS];
   __shared__ uint16_t base[RS_BINS];
   __shared__ uint32_t sums[RS_WARPS];
+  allow_next();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = threadIdx.x;
   const uint32_t rows = static_cast<uint32_t>(src.rows), mask = (1u << bits) - 1u;
   uint32_t key[1] = {e < n ? token_key(src, e, err) : 0xffffffffu};  // places past n sort last: all digits highest
@@ -359,6 +371,7 @@ __global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(RS_THREADS)
   __shared__ uint32_t base[RS_BINS];
   __shared__ uint32_t sums[RS_WARPS];
   __shared__ uint32_t block_heads;
+  allow_next();
   cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
   const unsigned block = cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -457,6 +470,7 @@ __global__ void __launch_bounds__(RS_THREADS) radix_count_kernel(TokenSource src
                                                                  int64_t tiles, uint32_t* __restrict__ hist,
                                                                  uint32_t* __restrict__ zeroed, int* err) {
   __shared__ uint32_t h[RS_BINS];
+  allow_next();
   const int lane = threadIdx.x & 31;
   if (threadIdx.x < RS_BINS) {
     h[threadIdx.x] = 0;
@@ -488,7 +502,10 @@ __global__ void __launch_bounds__(RS_THREADS) radix_scatter_kernel(TokenSource s
   __shared__ uint32_t half[2][RS_BINS];
   __shared__ uint32_t base[RS_BINS];
   __shared__ uint32_t sums[RS_WARPS];
+  allow_next();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  clear_counts(counts);
+  wait_previous();
   const int64_t e0 = int64_t(blockIdx.x) * RS_TILE + warp * 32 * RS_PER + lane;
   const uint32_t mask = (1u << bits) - 1u;
   uint32_t key[RS_PER], pos[RS_PER], rank[RS_PER];
@@ -502,7 +519,6 @@ __global__ void __launch_bounds__(RS_THREADS) radix_scatter_kernel(TokenSource s
       if (keys) pos[i] = positions[e];
     }
   }
-  clear_counts(counts);
   // this tile's first position of every digit: two threads a bin, half of the tiles each
   const int bin = threadIdx.x & (RS_BINS - 1), part = threadIdx.x / RS_BINS;
   uint32_t before = 0, total = 0;
@@ -554,6 +570,8 @@ __global__ void __launch_bounds__(HD_THREADS) heads_kernel(const uint32_t* __res
   constexpr int kWarps = HD_THREADS / 32, kRounds = HD_TILE / HD_THREADS;
   __shared__ uint32_t warp_sum[kWarps];
   __shared__ uint32_t last;
+  allow_next();
+  wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t e0 = int64_t(blockIdx.x) * HD_TILE + warp * 32 * kRounds + lane;
   uint32_t heads[kRounds], key[kRounds];
@@ -610,7 +628,7 @@ __global__ void __launch_bounds__(HD_THREADS) heads_kernel(const uint32_t* __res
 constexpr int SUM_THREADS = 256;
 constexpr int SUM_WARPS = SUM_THREADS / 32;
 constexpr int SUM_STAGE_BYTES = 4096;  // rows in flight of one warp
-constexpr int ZERO_ROWS = 16;          // rows one warp of the zero part looks after
+constexpr int ZERO_BYTES = 8192;         // of rows one warp of the zero part looks after
 
 template <bool kVector, typename T>
 __device__ __forceinline__ void store_cols(T* row, int64_t col, int64_t dim, const float (&v)[kVec]) {
@@ -623,6 +641,12 @@ __device__ __forceinline__ void store_cols(T* row, int64_t col, int64_t dim, con
   }
 }
 
+struct LongRun {
+  uint32_t chunk;  // the chunk it starts in
+  uint32_t parts;  // how many chunks it reaches
+  int64_t row;     // of the result
+};
+
 struct SumArgs {
   const uint32_t* keys;
   const uint32_t* pos;
@@ -633,6 +657,7 @@ struct SumArgs {
   int64_t chunks;
   int64_t slices;
   int64_t sum_blocks;
+  int64_t zero_rows;  // rows of a warp that writes zeros
   float scale;
   const uint32_t* chunk_base;
   const uint32_t* tile_base;
@@ -640,7 +665,7 @@ struct SumArgs {
   int64_t* out_ids;  // NULL: dense form
   const int64_t* count;
   float* partial;  // [chunks][2][slices * kSlice]: a run from an earlier chunk; a long run starting here
-  uint32_t* long_list;
+  LongRun* long_list;
   uint32_t* long_count;
 };
 
@@ -679,16 +704,15 @@ __device__ __forceinline__ void zero_span(O* out, int64_t begin, int64_t end) {
 // the row form those past the count.
 template <typename O>
 __device__ __forceinline__ void zero_rows(O* out, const SumArgs& a, int64_t unit) {
-  const int64_t r0 = unit * ZERO_ROWS;
+  const int64_t r0 = unit * a.zero_rows;
   if (a.out_ids) {
-    const int64_t from = max(r0, *a.count), to = min(r0 + ZERO_ROWS, a.cap);
+    const int64_t from = max(r0, *a.count), to = min(r0 + a.zero_rows, a.cap);
     if (from >= to) return;
     zero_span(out, from * a.dim, to * a.dim);
-    const int lane = threadIdx.x & 31;
-    if (from + lane < to) a.out_ids[from + lane] = 0;
+    for (int64_t r = from + (threadIdx.x & 31); r < to; r += 32) a.out_ids[r] = 0;
     return;
   }
-  const int64_t r1 = min(r0 + ZERO_ROWS, a.rows);
+  const int64_t r1 = min(r0 + a.zero_rows, a.rows);
   if (r0 >= r1) return;
   int64_t at = warp_lower_bound(a.keys, 0, a.n, r0);
   int64_t row = r0;
@@ -713,16 +737,20 @@ __device__ __forceinline__ void copy_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
-// Blocks below sum_blocks: one chunk and 256 columns a warp. The rows of dY
+// One chunk and 256 columns a warp. The rows of dY
 // come through a ring in shared memory (4 KB a warp, filled by asynchronous
 // copies that each lane makes and reads for itself), so few registers are
-// held and seven blocks fit an SM. The other blocks write the zeros.
+// held. The blocks behind sum_blocks write the zeros, 8 KB of rows a warp: with 64 KB
+// the dense gradient of 16384 tokens (151936 x 2048 bf16) took 106-124 us, not 99, and
+// zeros laid among the other blocks 117.
 template <typename G, typename O, bool kVector>
 __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ grad, O* __restrict__ out,
                                                           const SumArgs a) {
   constexpr int kStages = SUM_STAGE_BYTES / (kSlice * int(sizeof(G)));
   constexpr int kCopies = kVec * sizeof(G) / 16;
   __shared__ __align__(16) unsigned char ring[kVector ? SUM_WARPS : 1][kVector ? SUM_STAGE_BYTES : 16];
+  allow_next();
+  wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (int64_t(blockIdx.x) >= a.sum_blocks) {
     zero_rows(out, a, (int64_t(blockIdx.x) - a.sum_blocks) * SUM_WARPS + warp);
@@ -772,7 +800,6 @@ __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ 
   }
   if (valid < len) end = valid, tail = false;
   if (begin >= end) return;
-  if (tail && slice == 0 && lane == 0) a.long_list[atomicAdd(a.long_count, 1u)] = uint32_t(c);
   // where a run ends
   const uint32_t after_a = __shfl_down_sync(0xffffffffu, key_a, 1), after_b = __shfl_down_sync(0xffffffffu, key_b, 1);
   const uint32_t ends_a =
@@ -857,6 +884,14 @@ __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ 
       finish(r);
     }
   }
+  if (tail && slice == 0) {  // list the run for the join: it reaches the last chunk whose first key is its own
+    const int64_t stop = (warp_lower_bound(a.keys, s1, a.n, int64_t(last) + 1) - 1) / a.chunk;
+    if (lane == 0) {
+      a.long_list[atomicAdd(a.long_count, 1u)] = {uint32_t(c), uint32_t(stop - c + 1),
+                                                  a.out_ids ? int64_t(slot) : int64_t(last)};
+      if (a.out_ids) a.out_ids[slot] = last;
+    }
+  }
 }
 
 // -------------------------------------------------------------------- join
@@ -865,20 +900,17 @@ __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ 
 template <typename O, bool kVector>
 __global__ void __launch_bounds__(SUM_THREADS) join_kernel(O* __restrict__ out, const SumArgs a) {
   __shared__ float red[SUM_WARPS][kSlice];
+  wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t pitch = a.slices * kSlice;
   const int64_t jobs = int64_t(*a.long_count) * a.slices;
   for (int64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
-    const int64_t c0 = a.long_list[job / a.slices];
-    const int64_t slice = job % a.slices;
-    const uint32_t key = a.keys[(c0 + 1) * a.chunk];
-    // the chunks the run reaches: up to the last whose first key is the run's
-    const int64_t stop = (warp_lower_bound(a.keys, (c0 + 1) * a.chunk, a.n, int64_t(key) + 1) - 1) / a.chunk;
-    const int64_t n_parts = stop - c0 + 1;
+    const LongRun run = a.long_list[job / a.slices];
+    const int64_t slice = job % a.slices, n_parts = run.parts;
     const int64_t per = (n_parts + SUM_WARPS - 1) / SUM_WARPS;
     const int64_t p0 = min(n_parts, warp * per), p1 = min(n_parts, p0 + per);
     float acc[kVec] = {};
-    const float* part = a.partial + c0 * 2 * pitch + slice * kSlice + lane * kVec;
+    const float* part = a.partial + int64_t(run.chunk) * 2 * pitch + slice * kSlice + lane * kVec;
 #pragma unroll 4
     for (int64_t p = p0; p < p1; ++p) {
       float v[kVec];
@@ -889,14 +921,6 @@ __global__ void __launch_bounds__(SUM_THREADS) join_kernel(O* __restrict__ out, 
     store8(&red[warp][lane * kVec], acc);
     __syncthreads();
     if (warp == 0) {
-      int64_t row = key;
-      if (a.out_ids) {  // the run is the last to start in chunk c0
-        const int64_t s = c0 * a.chunk + lane;
-        const bool head = lane < a.chunk && (s == 0 || a.keys[s - 1] != a.keys[s]);
-        row = int64_t(a.tile_base[c0 * a.chunk / HD_TILE]) + a.chunk_base[c0] +
-              __popc(__ballot_sync(0xffffffffu, head)) - 1;
-        if (slice == 0 && lane == 0) a.out_ids[row] = key;
-      }
       // element j of this lane sits at column lane * 8 + j (vector) or lane + 32 j of the slice, in both
       // layouts at red[..][lane * 8 + j]
       float w[kVec];
@@ -906,7 +930,7 @@ __global__ void __launch_bounds__(SUM_THREADS) join_kernel(O* __restrict__ out, 
         for (int q = 0; q < SUM_WARPS; ++q) sum += red[q][lane * kVec + j];
         w[j] = sum * a.scale;
       }
-      store_cols<kVector>(out + row * a.dim, slice * kSlice + (kVector ? lane * kVec : lane), a.dim, w);
+      store_cols<kVector>(out + run.row * a.dim, slice * kSlice + (kVector ? lane * kVec : lane), a.dim, w);
     }
     __syncthreads();
   }
@@ -920,11 +944,11 @@ int bits_for(int64_t rows) {  // keys 0 .. rows
   return bits;
 }
 
-// Chunk length: long chunks save partial rows and searches, short ones give
-// more warps.
+// Chunk length: long chunks save partial rows, short ones give more warps.
+// 16384 tokens x 8 slices (bf16): 26.3 us with 32, 26-28 with 16, 33 with 8.
 int chunk_for(int64_t tokens, int64_t slices) {
   int chunk = kMaxChunk;
-  while (chunk > 8 && tokens / chunk * slices < 148 * 32) chunk /= 2;
+  while (chunk > 8 && tokens / chunk * slices < 148 * 16) chunk /= 2;
   return chunk;
 }
 
@@ -952,7 +976,7 @@ GradLayout grad_layout(int64_t n, int64_t dim) {
   l.hist = take(n > kClusterSort ? 4 * RS_MAX_PASSES * l.tiles * RS_BINS : 0);
   l.chunk_base = take(4 * l.chunks);
   l.tile_base = take(4 * ((n + HD_TILE - 1) / HD_TILE));
-  l.long_list = take(4 * l.chunks);
+  l.long_list = take(sizeof(LongRun) * l.chunks);
   l.counters = take(8);  // long runs, finished blocks of heads_kernel
   l.partial = take(8 * l.chunks * l.slices * kSlice);
   l.total = at;
@@ -969,23 +993,19 @@ int run_sum(const void* grad, void* out, SumArgs a, cudaStream_t stream) {
   const bool vec = a.dim % kVec == 0 &&
                    ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
   a.sum_blocks = (a.chunks * a.slices + SUM_WARPS - 1) / SUM_WARPS;
-  const int64_t zero_rows = a.out_ids ? a.cap : a.rows;
-  const int64_t blocks = a.sum_blocks + (zero_rows + ZERO_ROWS * SUM_WARPS - 1) / (ZERO_ROWS * SUM_WARPS);
+  const int64_t row_bytes = a.dim * int64_t(sizeof(O)), rows = a.out_ids ? a.cap : a.rows;
+  a.zero_rows = row_bytes >= ZERO_BYTES ? 1 : ZERO_BYTES / row_bytes;
+  const int64_t blocks = a.sum_blocks + (rows + a.zero_rows * SUM_WARPS - 1) / (a.zero_rows * SUM_WARPS);
   if (blocks > 0x7fffffffLL) return set_error(MUON_ERR_ARG, "embedding gradient too large");
   const unsigned grid = static_cast<unsigned>(blocks);
   const G* g = static_cast<const G*>(grad);
   O* o = static_cast<O*>(out);
-  if (vec)
-    sum_kernel<G, O, true><<<grid, SUM_THREADS, 0, stream>>>(g, o, a);
-  else
-    sum_kernel<G, O, false><<<grid, SUM_THREADS, 0, stream>>>(g, o, a);
-  if (check_cuda(cudaGetLastError(), "embedding gradient sum launch")) return MUON_ERR_CUDA;
+  if (int rc = launch_overlapped("embedding gradient sum launch", vec ? sum_kernel<G, O, true> : sum_kernel<G, O, false>,
+                                 grid, SUM_THREADS, stream, g, o, a))
+    return rc;
   const unsigned join_grid = static_cast<unsigned>(a.chunks * a.slices < 592 ? a.chunks * a.slices : 592);
-  if (vec)
-    join_kernel<O, true><<<join_grid, SUM_THREADS, 0, stream>>>(o, a);
-  else
-    join_kernel<O, false><<<join_grid, SUM_THREADS, 0, stream>>>(o, a);
-  return check_cuda(cudaGetLastError(), "embedding gradient join launch");
+  return launch_overlapped("embedding gradient join launch", vec ? join_kernel<O, true> : join_kernel<O, false>,
+                           join_grid, SUM_THREADS, stream, o, a);
 }
 
 }  // namespace
@@ -1080,17 +1100,19 @@ int launch_embedding_grad(const void* grad, int grad_dtype, const void* ids, int
     for (int p = 0; p < passes; ++p) {
       cur = p & 1;
       uint32_t* hist = u32(l.hist) + p * l.tiles * RS_BINS;
-      radix_scatter_kernel<<<tiles, RS_THREADS, 0, stream>>>(src, keys, pos, tokens, p * per, per, l.tiles, hist,
-                                                             p + 1 < passes ? hist + l.tiles * RS_BINS : nullptr,
-                                                             u32(l.keys[cur]), u32(l.pos[cur]));
-      if (check_cuda(cudaGetLastError(), "radix scatter launch")) return MUON_ERR_CUDA;
+      if (int rc = launch_overlapped("radix scatter launch", radix_scatter_kernel, tiles, RS_THREADS, stream, src, keys,
+                                     pos, tokens, p * per, per, l.tiles, hist,
+                                     p + 1 < passes ? hist + l.tiles * RS_BINS : nullptr, u32(l.keys[cur]),
+                                     u32(l.pos[cur])))
+        return rc;
       keys = u32(l.keys[cur]);
       pos = u32(l.pos[cur]);
     }
     const unsigned grid = static_cast<unsigned>((tokens + HD_TILE - 1) / HD_TILE);
-    heads_kernel<<<grid, HD_THREADS, 0, stream>>>(keys, tokens, static_cast<uint32_t>(rows), l.chunk,
-                                                  u32(l.chunk_base), u32(l.tile_base), counters + 1, row_count);
-    if (check_cuda(cudaGetLastError(), "run heads launch")) return MUON_ERR_CUDA;
+    if (int rc = launch_overlapped("run heads launch", heads_kernel, grid, HD_THREADS, stream, keys, tokens,
+                                   static_cast<uint32_t>(rows), l.chunk, u32(l.chunk_base), u32(l.tile_base),
+                                   counters + 1, row_count))
+      return rc;
   }
   SumArgs a{};
   a.keys = u32(l.keys[cur]);
@@ -1108,7 +1130,7 @@ int launch_embedding_grad(const void* grad, int grad_dtype, const void* ids, int
   a.out_ids = out_ids;
   a.count = count;
   a.partial = reinterpret_cast<float*>(base + l.partial);
-  a.long_list = u32(l.long_list);
+  a.long_list = reinterpret_cast<LongRun*>(base + l.long_list);
   a.long_count = counters;
   using bf = __nv_bfloat16;
   const bool gb = grad_dtype == MUON_BF16, ob = out_dtype == MUON_BF16;

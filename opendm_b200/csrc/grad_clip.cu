@@ -17,7 +17,9 @@
 // double from the registers: squares over- or underflow fp32 long before the
 // norm does.
 
-#include <cmath>
+#include <algorithm>
+#include <new>
+#include <vector>
 
 #include "common.cuh"
 #include "internal.h"
@@ -229,6 +231,7 @@ __global__ void __launch_bounds__(GC_THREADS, kBlocksPerSm) list_norm_kernel(con
                                                                              double* __restrict__ partials) {
   constexpr int kChunk = kIters * GC_STEP;
   __shared__ double red[GC_THREADS / 32];
+  allow_next();
   double total = 0.0;
   for (int chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
     const int s = find_clip_segment(t, chunk);
@@ -323,6 +326,7 @@ __global__ void __launch_bounds__(GC_THREADS, kBlocksPerSm) list_scale_kernel(co
                                                                 const float* __restrict__ total_in) {
   constexpr int kChunk = kIters * GC_STEP;
   __shared__ double red[GC_THREADS / 32];
+  wait_previous();
   float total;
   if (partials) {
     total = join_partials(kind, partials, n_partials, red);
@@ -384,6 +388,35 @@ int check_segs(const muon_clip_seg* segs, int64_t n, bool outputs) {
       return set_error(MUON_ERR_ARG, "clipping in place needs one dtype");
   }
   return MUON_OK;
+}
+
+// Outputs must not share memory with one another or with another segment's
+// gradient: blocks read and write them in no fixed order.
+int check_overlap(const muon_clip_seg* segs, int64_t n) try {
+  struct Span {
+    uintptr_t begin, end;
+    int64_t seg;
+  };
+  std::vector<Span> outs;
+  outs.reserve(n);
+  for (int64_t i = 0; i < n; ++i) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(segs[i].out);
+    if (segs[i].numel > 0) outs.push_back({p, p + segs[i].numel * (segs[i].out_dtype == MUON_BF16 ? 2 : 4), i});
+  }
+  std::sort(outs.begin(), outs.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  for (size_t i = 1; i < outs.size(); ++i)
+    if (outs[i].begin < outs[i - 1].end) return set_error(MUON_ERR_ARG, "clipped gradients overlap in memory");
+  for (int64_t i = 0; i < n; ++i) {
+    if (segs[i].numel == 0 || segs[i].grad == segs[i].out) continue;
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(segs[i].grad);
+    const uintptr_t end = begin + segs[i].numel * (segs[i].grad_dtype == MUON_BF16 ? 2 : 4);
+    auto after = std::lower_bound(outs.begin(), outs.end(), end, [](const Span& s, uintptr_t e) { return s.begin < e; });
+    if (after != outs.begin() && (after - 1)->end > begin)
+      return set_error(MUON_ERR_ARG, "gradients overlap the memory they are clipped into");
+  }
+  return MUON_OK;
+} catch (const std::bad_alloc&) {
+  return set_error(MUON_ERR_ARG, "out of host memory");
 }
 
 // Fills `t` with segments from `i` on (empty ones skipped) and returns the next index.
@@ -454,10 +487,10 @@ template <int N, int kIters>
 int scale_batches(const muon_clip_seg* segs, int64_t n, int kind, const double* partials, int n_partials,
                   float max_norm, float* total_out, const float* total_in, cudaStream_t stream) {
   return for_batches<N, kIters>(segs, n, [&](const ClipTable<N>& t) {
-    list_scale_kernel<N, kIters><<<blocks_for(t.chunks), GC_THREADS, 0, stream>>>(t, kind, partials, n_partials,
-                                                                                 max_norm, total_out, total_in);
+    const int rc = launch_overlapped("list scale launch", list_scale_kernel<N, kIters>, blocks_for(t.chunks),
+                                     GC_THREADS, stream, t, kind, partials, n_partials, max_norm, total_out, total_in);
     total_out = nullptr;  // written by the first batch
-    return check_cuda(cudaGetLastError(), "list scale launch");
+    return rc;
   });
 }
 
@@ -510,6 +543,7 @@ int launch_total_norm(const muon_clip_seg* segs, int64_t n_segs, int norm_kind, 
 int launch_clip_grads(const muon_clip_seg* segs, int64_t n_segs, int norm_kind, float max_norm, void* workspace,
                       float* total, cudaStream_t stream) {
   if (int rc = check_segs(segs, n_segs, true)) return rc;
+  if (int rc = check_overlap(segs, n_segs)) return rc;
   if (all_empty(segs, n_segs)) return launch_total_norm(segs, n_segs, norm_kind, workspace, total, stream);
   if (norm_kind < MUON_NORM_2 || norm_kind > MUON_NORM_INF) return set_error(MUON_ERR_ARG, "unknown norm kind");
   if (!total || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u))
@@ -524,6 +558,7 @@ int launch_scale_grads(const muon_clip_seg* segs, int64_t n_segs, float max_norm
                        cudaStream_t stream) {
   if (!total) return set_error(MUON_ERR_ARG, "null norm");
   if (int rc = check_segs(segs, n_segs, true)) return rc;
+  if (int rc = check_overlap(segs, n_segs)) return rc;
   return scale_list(segs, n_segs, 0, nullptr, 0, max_norm, nullptr, total, stream);
 }
 

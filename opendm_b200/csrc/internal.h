@@ -51,6 +51,24 @@ int launch_momentum_f16(const muon_momentum_f16_seg* segs_dev, int n_segs, int64
                         float momentum, int nesterov, float eps, float* partials_dev, float* pscale_dev,
                         float* scales_dev, int* redo_dev, const float* grad_scale, cudaStream_t stream);
 
+// Launches `kernel` so that it may start while the kernel before it on the
+// stream (one of this library that calls allow_next()) drains; it has to call
+// wait_previous() before it touches memory.
+template <typename... Params, typename... Args>
+int launch_overlapped(const char* what, void (*kernel)(Params...), unsigned grid, unsigned block, cudaStream_t stream,
+                      Args... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, Params(args)...), what);
+}
+
 int launch_adamw_rows(const muon_adamw_rows_seg* seg, double beta1, double beta2, float eps, float wd_factor,
                       const float* grad_scale, cudaStream_t stream);
 

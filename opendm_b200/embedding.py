@@ -59,17 +59,24 @@ class _ErrorWord:
 
     def __init__(self, device: torch.device):
         self.word = torch.zeros(1, dtype=torch.int32, device=device)
+        self.pointer = self.word.data_ptr()
         self.host = torch.zeros(1, dtype=torch.int32).pin_memory()
         self.event = None
 
 
 _WORDS: dict[int, _ErrorWord] = {}
 
+# The current stream's handle: torch.cuda.current_stream(index).cuda_stream without its
+# Stream object where this torch has the call (0.1 us instead of 1.2).
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-def _device_index(t: torch.Tensor) -> int:
-    if t.device.type != "cuda":
+
+def device_index(t: torch.Tensor) -> int:
+    index = t.get_device()
+    if index < 0 or not t.is_cuda:
         raise RuntimeError("opendm_b200 runs on CUDA (sm_100) tensors only; got a tensor on " + str(t.device))
-    return t.device.index
+    return index
 
 
 def _error_word(index: int) -> _ErrorWord:
@@ -99,8 +106,7 @@ def check_errors(device: torch.device | int | None = None) -> None:
         with torch.cuda.device(index):
             torch.cuda.synchronize()
             code = c_int(0)
-            N.check(N.lib().muon_read_error(word.word.data_ptr(), byref(code),
-                                            torch.cuda.current_stream().cuda_stream), "embedding")
+            N.check(N.lib().muon_read_error(word.pointer, byref(code), raw_stream(index)), "embedding")
 
 
 def record_error_check(device: torch.device) -> None:
@@ -132,83 +138,80 @@ def _code(table: dict, dtype: torch.dtype, what: str) -> int:
     return code
 
 
-def _on_device(index: int, call):
+def on_device(index: int, call, *args):
     """Run ``call`` with the device current (the usual case costs one query)."""
     if torch.cuda.current_device() == index:
-        return call()
+        return call(*args)
     with torch.cuda.device(index):
-        return call()
+        return call(*args)
 
 
 def _lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float, out_dtype: torch.dtype) -> torch.Tensor:
     if weight.ndim != 2:
         raise ValueError("embedding weight must be 2-D")
-    index = _device_index(weight)
-    if ids.device != weight.device:
+    index = device_index(weight)
+    if ids.get_device() != index:
         raise RuntimeError(f"ids are on {ids.device}, the weight on {weight.device}")
     w_code, o_code = _code(_FLOAT_CODE, weight.dtype, "weight"), _code(_FLOAT_CODE, out_dtype, "output")
     i_code = _code(_INDEX_CODE, ids.dtype, "id")
     rows, dim = weight.shape
-    ld = weight.stride(0)
-    if rows <= 1:
-        ld = dim
-    if (weight.stride(1) != 1 and dim > 1) or ld < dim:
+    if not weight.is_contiguous():
+        if dim > 1 and (weight.stride(1) != 1 or (rows > 1 and weight.stride(0) < dim)):
+            weight = weight.contiguous()
+    ld = weight.stride(0) if rows > 1 else dim
+    if ld < dim:  # rows that share memory: an expanded weight
         weight = weight.contiguous()
         ld = dim
-    ids = ids.contiguous()
+    return on_device(index, _launch_lookup, index, ids.contiguous(), i_code, weight, w_code, rows, dim, ld, scale,
+                     out_dtype, o_code)
 
-    def call():
-        word = _error_word(index)
-        out = torch.empty((*ids.shape, dim), dtype=out_dtype, device=weight.device)
-        N.check(N.lib().muon_embedding(weight.data_ptr(), w_code, rows, dim, ld, ids.data_ptr(), i_code, ids.numel(),
-                                       scale, out.data_ptr(), o_code, word.word.data_ptr(),
-                                       torch.cuda.current_stream().cuda_stream), "muon_embedding")
-        return out
 
-    return _on_device(index, call)
+def _launch_lookup(index, ids, i_code, weight, w_code, rows, dim, ld, scale, out_dtype, o_code):
+    out = weight.new_empty((*ids.shape, dim), dtype=out_dtype)
+    N.check(N.lib().muon_embedding(weight.data_ptr(), w_code, rows, dim, ld, ids.data_ptr(), i_code, ids.numel(),
+                                   scale, out.data_ptr(), o_code, _error_word(index).pointer, raw_stream(index)),
+            "muon_embedding")
+    return out
 
 
 def _gradient(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: float, padding_idx: int | None,
               dtype: torch.dtype | None, as_rows: bool):
-    index = _device_index(grad)
-    if ids.device != grad.device:
+    index = device_index(grad)
+    if ids.get_device() != index:
         raise RuntimeError(f"ids are on {ids.device}, the gradient on {grad.device}")
-    if grad.ndim != ids.ndim + 1 or grad.shape[:-1] != ids.shape:
+    if grad.shape[:-1] != ids.shape or grad.ndim == 0:
         raise ValueError(f"gradient of shape {tuple(grad.shape)} does not match ids of shape {tuple(ids.shape)}")
     dtype = dtype or grad.dtype
     g_code, o_code = _code(_FLOAT_CODE, grad.dtype, "gradient"), _code(_FLOAT_CODE, dtype, "result")
     i_code = _code(_INDEX_CODE, ids.dtype, "id")
-    num_rows, dim, tokens = int(num_rows), grad.shape[-1], ids.numel()
+    num_rows = int(num_rows)
     pad = -1 if padding_idx is None else int(padding_idx)
     if num_rows < 0 or (padding_idx is not None and not 0 <= pad < num_rows):
         raise ValueError(f"padding_idx {padding_idx} is not one of {num_rows} rows")
-    grad, ids = grad.contiguous(), ids.contiguous()
+    return on_device(index, _launch_gradient, index, grad.contiguous(), g_code, ids.contiguous(), i_code, num_rows,
+                     pad, scale, dtype, o_code, as_rows)
 
-    def call():
-        lib = N.lib()
-        word = _error_word(index)
-        need = lib.muon_embedding_grad_workspace_bytes(tokens, num_rows, dim)
-        if need < 0:
-            raise RuntimeError(f"embedding gradient of {tokens} tokens, {num_rows} x {dim} is out of range")
-        dev = grad.device
-        work = torch.empty(need, dtype=torch.uint8, device=dev)
-        if as_rows:
-            cap = min(tokens, num_rows)
-            out = torch.empty((cap, dim), dtype=dtype, device=dev)
-            index_out = torch.empty(cap + 1, dtype=torch.int64, device=dev)
-            out_ids, count = index_out[:cap], index_out[cap:]
-            ids_ptr = index_out.data_ptr()  # (an empty view's pointer would be null: the dense form)
-            count_ptr = ids_ptr + 8 * cap
-        else:
-            out = torch.empty((num_rows, dim), dtype=dtype, device=dev)
-            ids_ptr = count_ptr = None
-        N.check(lib.muon_embedding_grad(grad.data_ptr(), g_code, ids.data_ptr(), i_code, tokens, num_rows, dim, pad,
-                                        scale, out.data_ptr(), o_code, ids_ptr, count_ptr, work.data_ptr(), need,
-                                        word.word.data_ptr(), torch.cuda.current_stream().cuda_stream),
-                "muon_embedding_grad")
-        return RowGrad(num_rows, out_ids, out, count) if as_rows else out
 
-    return _on_device(index, call)
+def _launch_gradient(index, grad, g_code, ids, i_code, num_rows, pad, scale, dtype, o_code, as_rows):
+    lib = N.lib()
+    dim, tokens = grad.shape[-1], ids.numel()
+    need = lib.muon_embedding_grad_workspace_bytes(tokens, num_rows, dim)
+    if need < 0:
+        raise RuntimeError(f"embedding gradient of {tokens} tokens, {num_rows} x {dim} is out of range")
+    work = grad.new_empty(need, dtype=torch.uint8)
+    if as_rows:
+        cap = min(tokens, num_rows)
+        out = grad.new_empty((cap, dim), dtype=dtype)
+        index_out = grad.new_empty(cap + 1, dtype=torch.int64)
+        ids_ptr = index_out.data_ptr()  # (an empty view's pointer would be null: the dense form)
+        count_ptr = ids_ptr + 8 * cap
+    else:
+        out = grad.new_empty((num_rows, dim), dtype=dtype)
+        ids_ptr = count_ptr = None
+    N.check(lib.muon_embedding_grad(grad.data_ptr(), g_code, ids.data_ptr(), i_code, tokens, num_rows, dim, pad, scale,
+                                    out.data_ptr(), o_code, ids_ptr, count_ptr, work.data_ptr(), need,
+                                    _error_word(index).pointer, raw_stream(index)), "muon_embedding_grad")
+    return RowGrad(num_rows, index_out[:cap], out, index_out[cap:]) if as_rows else out
 
 
 def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, *, scale: float = 1.0,
@@ -256,7 +259,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, pa
         raise ValueError(f"padding_idx {padding_idx} is not one of {weight.shape[0]} rows")
     if torch.is_grad_enabled() and weight.requires_grad:
         return _EmbeddingFn.apply(weight, ids, scale, padding_idx, bool(sparse), out_dtype)
-    return _lookup(ids, weight.detach(), scale, out_dtype)
+    return _lookup(ids, weight, scale, out_dtype)
 
 
 class ScaledEmbedding(torch.nn.Embedding):

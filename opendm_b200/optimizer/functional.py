@@ -20,14 +20,19 @@ from __future__ import annotations
 import math
 from array import array
 from collections.abc import Iterable
+from operator import attrgetter, or_
 
 import torch
 
 from .. import _native as N
-from ..embedding import RowGrad, _device_index, _on_device, embedding_row_grad
+from ..embedding import RowGrad, device_index, embedding_row_grad, on_device, raw_stream
 from ..engine import AdamItem
 
 _CODE = {torch.bfloat16: N.MUON_BF16, torch.float32: N.MUON_F32}
+# The lists are long and each call is short: what is asked of every tensor goes through map.
+_POINTER, _NUMEL, _DEVICE = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
+_CONTIGUOUS, _SIZE = torch.Tensor.is_contiguous, torch.Tensor.size
+_LAYOUT, _DTYPE = attrgetter("layout"), attrgetter("dtype")
 _NORMS = {2.0: N.MUON_NORM_2, 1.0: N.MUON_NORM_1, math.inf: N.MUON_NORM_INF}
 
 
@@ -52,43 +57,34 @@ def _dense_storage(t: torch.Tensor) -> bool:
 
 def _check_grads(grads: list[torch.Tensor], what: str) -> int:
     """Device index of the list; raises for layouts, dtypes and devices the kernels do not take."""
-    index = _device_index(grads[0])
-    device = grads[0].device
-    for g in grads:
-        if g.layout is not torch.strided:
-            raise RuntimeError(f"{what} must be dense tensors, got layout {g.layout}")
-        if g.device != device:
-            raise RuntimeError(f"{what} must be on one device; got {device} and {g.device}")
-        if g.dtype not in _CODE:
-            raise RuntimeError(f"unsupported dtype {g.dtype}: the kernels take bfloat16 or float32")
+    index = device_index(grads[0])
+    if set(map(_LAYOUT, grads)) != {torch.strided}:
+        raise RuntimeError(f"{what} must be dense tensors")
+    if set(map(_DEVICE, grads)) != {index}:
+        raise RuntimeError(f"{what} must be on one device")
     return index
 
 
-def _table(src: list[torch.Tensor], dst: list[torch.Tensor]) -> array:
-    """The list as muon_clip_seg structures: pointers, size and the two 32-bit dtypes of each."""
-    flat = array("q")
-    for s, d in zip(src, dst):
-        flat.extend((s.data_ptr(), d.data_ptr(), s.numel(), _CODE[s.dtype] | _CODE[d.dtype] << 32))
-    return flat
+def _codes(grads: list[torch.Tensor]) -> list[int]:
+    dtypes = list(map(_DTYPE, grads))
+    for dtype in set(dtypes):
+        if dtype not in _CODE:
+            raise RuntimeError(f"unsupported dtype {dtype}: the kernels take bfloat16 or float32")
+    return list(map(_CODE.__getitem__, dtypes))
 
 
-def _refuse_overlap(src: list[torch.Tensor], dst: list[torch.Tensor]) -> None:
-    """Every output must own its memory: blocks write them in no fixed order."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in dst if t.numel())
-    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-        raise RuntimeError("gradients to be clipped overlap in memory")
-    if src is dst:
-        return
-    starts = [s[0] for s in spans]
-    from bisect import bisect_left
-
-    for s, d in zip(src, dst):
-        if not s.numel() or s.data_ptr() == d.data_ptr():
-            continue
-        lo, hi = s.data_ptr(), s.data_ptr() + s.numel() * s.element_size()
-        at = bisect_left(starts, hi) - 1
-        if at >= 0 and spans[at][1] > lo:
-            raise RuntimeError("gradients overlap the tensors they are clipped into")
+def _table(src: list[torch.Tensor], dst: list[torch.Tensor] | None) -> array:
+    """The list as muon_clip_seg structures: two pointers, the size and the two 32-bit dtypes of each."""
+    flat = [0] * (4 * len(src))
+    pointers, codes = list(map(_POINTER, src)), _codes(src)
+    flat[0::4] = pointers
+    flat[2::4] = map(_NUMEL, src)
+    flat[3::4] = codes
+    if dst is not None:
+        flat[1::4] = pointers if dst is src else map(_POINTER, dst)
+        out_codes = codes if dst is src else _codes(dst)
+        flat[3::4] = map(or_, codes, [c << 32 for c in out_codes])
+    return array("q", flat)
 
 
 def _unique(tensors: Iterable[torch.Tensor]) -> list[torch.Tensor]:
@@ -96,8 +92,8 @@ def _unique(tensors: Iterable[torch.Tensor]) -> list[torch.Tensor]:
     return [t for t in tensors if not (id(t) in seen or seen.add(id(t)))]
 
 
-def _workspace(n: int, device: torch.device) -> torch.Tensor:
-    return torch.empty(int(N.lib().muon_clip_workspace_bytes(n)), dtype=torch.uint8, device=device)
+def _workspace(grads: list[torch.Tensor]) -> torch.Tensor:
+    return grads[0].new_empty(N.lib().muon_clip_workspace_bytes(len(grads)), dtype=torch.uint8)
 
 
 def _raise_nonfinite(total: torch.Tensor, norm_type: float) -> None:
@@ -120,13 +116,13 @@ def get_total_norm(tensors: torch.Tensor | Iterable[torch.Tensor], norm_type: fl
     tensors = [t if _dense_storage(t) else t.contiguous() for t in tensors]
 
     def call():
-        total = torch.empty((), dtype=torch.float32, device=tensors[0].device)
-        table, work = _table(tensors, tensors), _workspace(len(tensors), total.device)
+        total = tensors[0].new_empty((), dtype=torch.float32)
+        table, work = _table(tensors, None), _workspace(tensors)
         N.check(N.lib().muon_total_norm(table.buffer_info()[0], len(tensors), kind, work.data_ptr(), total.data_ptr(),
-                                        torch.cuda.current_stream().cuda_stream), "muon_total_norm")
+                                        raw_stream(index)), "muon_total_norm")
         return total
 
-    total = _on_device(index, call)
+    total = on_device(index, call)
     if error_if_nonfinite:
         _raise_nonfinite(total, norm_type)
     return total
@@ -136,26 +132,23 @@ def _apply(grads: list[torch.Tensor], outs: list[torch.Tensor], max_norm: float,
            total: torch.Tensor | None) -> torch.Tensor:
     """Norm (unless given) and scaling of dense-storage tensors."""
     index = _check_grads(grads, "gradients")
-    if outs is not grads:
-        _check_grads(outs, "outputs")
-        if outs[0].device != grads[0].device:
-            raise RuntimeError("gradients and outputs must be on one device")
-    _refuse_overlap(grads, outs)
+    if outs is not grads and _check_grads(outs, "outputs") != index:
+        raise RuntimeError("gradients and outputs must be on one device")
 
     def call():
-        lib, stream = N.lib(), torch.cuda.current_stream().cuda_stream
+        lib, stream = N.lib(), raw_stream(index)
         table = _table(grads, outs)
         if total is not None:
             N.check(lib.muon_scale_grads(table.buffer_info()[0], len(grads), max_norm, total.data_ptr(), stream),
                     "muon_scale_grads")
             return total
-        norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-        work = _workspace(len(grads), norm.device)
+        norm = grads[0].new_empty((), dtype=torch.float32)
+        work = _workspace(grads)
         N.check(lib.muon_clip_grads(table.buffer_info()[0], len(grads), _norm_kind(norm_type), max_norm,
                                     work.data_ptr(), norm.data_ptr(), stream), "muon_clip_grads")
         return norm
 
-    return _on_device(index, call)
+    return on_device(index, call)
 
 
 def _max_norm(max_norm: float) -> float:
@@ -169,7 +162,7 @@ def _clip(grads: list[torch.Tensor], outs: list[torch.Tensor] | None, max_norm: 
           total: torch.Tensor | None) -> torch.Tensor:
     if outs is None:
         outs = grads
-    if all(g.is_contiguous() for g in grads) and (outs is grads or all(o.is_contiguous() for o in outs)):
+    if all(map(_CONTIGUOUS, grads)) and (outs is grads or all(map(_CONTIGUOUS, outs))):
         return _apply(grads, outs, max_norm, norm_type, total)
     # Other strides: elementwise work needs only that both sides agree on the
     # order of elements, else a contiguous copy is scaled and copied back.
@@ -207,7 +200,7 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *, norm_type: flo
         grads = _unique(grads)
     else:
         out = list(out)
-        if len(out) != len(grads) or any(o.shape != g.shape for o, g in zip(out, grads)):
+        if len(out) != len(grads) or list(map(_SIZE, out)) != list(map(_SIZE, grads)):
             raise ValueError("out must match the gradients in number and shapes")
     if not grads:
         return torch.tensor(0.0)
@@ -297,7 +290,7 @@ def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor],
         if any(t.dtype != torch.float32 or t.shape != p.shape or not t.is_contiguous() for t in (m, v)):
             raise RuntimeError("AdamW moments must be contiguous float32 tensors of their parameter's shape")
     items = [AdamItem(*it) for it in zip(params, grads, exp_avgs, exp_avg_sqs, map(float, steps))]
-    index = _device_index(params[0])
+    index = device_index(params[0])
     engine = _engine_for(params[0].device, "fp16")
-    _on_device(index, lambda: engine.adamw(items, lr=float(lr), beta1=float(beta1), beta2=float(beta2),
+    on_device(index, lambda: engine.adamw(items, lr=float(lr), beta1=float(beta1), beta2=float(beta2),
                                            eps=float(eps), weight_decay=float(weight_decay)))
