@@ -9,7 +9,7 @@
 // Gradient. The tokens are sorted by id (stable, so a row's tokens keep their
 // order), then summed:
 //   1. sort. Ids left out (padding, out of range) get the key `rows`, which
-//      sorts last and is dropped. Up to 1024 tokens in one block, up to
+//      sorts last and is dropped. Up to 2048 tokens in one block, up to
 //      32768 in a cluster of eight, more by tiles over the GPU.
 //   2. sum. The sorted tokens are cut into chunks of C positions; a warp takes
 //      one chunk and 256 columns and adds the rows of dY in sorted order in
@@ -22,6 +22,8 @@
 // atomics, two calls give the same bits.
 
 #include <cooperative_groups.h>
+
+#include <algorithm>
 
 #include "common.cuh"
 #include "internal.h"
@@ -41,36 +43,89 @@ __device__ __forceinline__ int64_t load_id(const void* ids, bool wide, int64_t t
 
 __device__ __forceinline__ void record_error(int* err, int code) { atomicCAS(err, 0, code); }
 
-// 8 consecutive elements as fp32.
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[kVec]) {
-  const uint4 raw = *reinterpret_cast<const uint4*>(p);
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+// kE consecutive elements (aligned to all of them, up to 16 bytes) as fp32.
+template <int kE, typename T>
+__device__ __forceinline__ void load_group(const T* p, float (&v)[kE]) {
+  constexpr int kBytes = kE * sizeof(T);
+  if constexpr (kBytes > 16) {
+    float lo[kE / 2], hi[kE / 2];
+    load_group<kE / 2>(p, lo);
+    load_group<kE / 2>(p + kE / 2, hi);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __bfloat1622float2(h[i]);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+    for (int i = 0; i < kE / 2; ++i) v[i] = lo[i], v[kE / 2 + i] = hi[i];
+  } else if constexpr (kE == 1) {
+    if constexpr (sizeof(T) == 2)
+      v[0] = __bfloat162float(*p);
+    else
+      v[0] = *p;
+  } else {
+    uint32_t w[kBytes / 4];
+    if constexpr (kBytes == 16) {
+      const uint4 x = *reinterpret_cast<const uint4*>(p);
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else if constexpr (kBytes == 8) {
+      const uint2 x = *reinterpret_cast<const uint2*>(p);
+      w[0] = x.x, w[1] = x.y;
+    } else {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+#pragma unroll
+    for (int i = 0; i < kBytes / 4; ++i) {
+      if constexpr (sizeof(T) == 2) {  // bf16 is the upper half of an fp32
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        v[i] = __uint_as_float(w[i]);
+      }
+    }
   }
 }
-__device__ __forceinline__ void load8(const float* p, float (&v)[kVec]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[kVec]) {
-  uint4 raw;
-  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&raw);
+
+template <int kE, typename T>
+__device__ __forceinline__ void store_group(T* p, const float (&v)[kE]) {
+  constexpr int kBytes = kE * sizeof(T);
+  if constexpr (kBytes > 16) {
+    float lo[kE / 2], hi[kE / 2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-  *reinterpret_cast<uint4*>(p) = raw;
+    for (int i = 0; i < kE / 2; ++i) lo[i] = v[i], hi[i] = v[kE / 2 + i];
+    store_group<kE / 2>(p, lo);
+    store_group<kE / 2>(p + kE / 2, hi);
+  } else if constexpr (kE == 1) {
+    if constexpr (sizeof(T) == 2)
+      *p = __float2bfloat16_rn(v[0]);
+    else
+      *p = v[0];
+  } else {
+    uint32_t w[kBytes / 4];
+#pragma unroll
+    for (int i = 0; i < kBytes / 4; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        w[i] = __float_as_uint(v[i]);
+      }
+    }
+    if constexpr (kBytes == 16)
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (kBytes == 8)
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else
+      *reinterpret_cast<uint32_t*>(p) = w[0];
+  }
 }
-__device__ __forceinline__ void store8(float* p, const float (&v)[kVec]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+
+// Widest group (8, 4, 2 or 1 elements) that rows of `dim` elements `pitch`
+// apart can be cut into, both tensors aligned to it (to 16 bytes at most).
+int group_width(int64_t dim, int64_t pitch, const void* a, int a_size, const void* b, int b_size) {
+  for (int e = 8; e > 1; e /= 2) {
+    const uintptr_t a_bytes = e * a_size < 16 ? e * a_size : 16, b_bytes = e * b_size < 16 ? e * b_size : 16;
+    if (dim % e == 0 && pitch % e == 0 && reinterpret_cast<uintptr_t>(a) % a_bytes == 0 &&
+        reinterpret_cast<uintptr_t>(b) % b_bytes == 0)
+      return e;
+  }
+  return 1;
 }
-__device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ float load1(const float* p) { return *p; }
-__device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 
 // ------------------------------------------------------------------ lookup
 constexpr int LK_THREADS = 256;
@@ -110,23 +165,25 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_kernel(const W* __restrict_
     const uint32_t o = i * LK_THREADS + threadIdx.x;
     if (o >= left) continue;
     float v[kVec];
-    load8(reinterpret_cast<const W*>(raw[i]), v);
+    load_group<kVec>(reinterpret_cast<const W*>(raw[i]), v);
 #pragma unroll
     for (int k = 0; k < kVec; ++k) v[k] *= scale;
-    store8(out + (base + o) * kVec, v);
+    store_group<kVec>(out + (base + o) * kVec, v);
   }
 }
 
-// Other rows: a warp takes up to 1024 columns of one token, eight single
-// elements a lane at a time (no division per element).
+// Other rows: a warp takes up to 1024 columns of one token, eight elements a
+// lane at a time in groups of kE (4, 2 or 1): no division per element. The
+// fp32 32003 x 1001 table with 40961 tokens takes 30 us: its 164 MB of fp32
+// rows and 82 MB of results all cross L2, in part sectors.
 constexpr int LK_COLS = 1024;
-constexpr int LK_LANE = 8;
 
-template <typename W, typename O>
+template <int kE, typename W, typename O>
 __global__ void __launch_bounds__(LK_THREADS) lookup_rows_kernel(const W* __restrict__ weight, int64_t rows,
                                                                  int64_t ld, const void* __restrict__ ids, bool wide,
                                                                  int64_t tokens, int64_t dim, int64_t parts,
                                                                  float scale, O* __restrict__ out, int* err) {
+  constexpr int kGroups = kVec / kE, kStep = 32 * kE;
   const int lane = threadIdx.x & 31;
   const int64_t unit = int64_t(blockIdx.x) * (LK_THREADS / 32) + (threadIdx.x >> 5);
   const int64_t t = unit / parts, part = unit - t * parts;
@@ -135,47 +192,50 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_rows_kernel(const W* __rest
   const bool ok = id >= 0 && id < rows;
   if (!ok && part == 0 && lane == 0) record_error(err, MUON_DEV_BAD_INDEX);
   const int64_t c0 = part * LK_COLS;
-  const int n = static_cast<int>(min(int64_t(LK_COLS), dim - c0));
-  const W* src = weight + (ok ? id * ld : 0) + c0;
-  O* dst = out + t * dim + c0;
-  src += lane;
-  dst += lane;
-  int at = 0;
-  for (; at + 32 * LK_LANE <= n; at += 32 * LK_LANE) {  // without a test per element
-    float v[LK_LANE];
+  const int n = static_cast<int>(min(int64_t(LK_COLS), dim - c0)) - lane * kE;  // columns from this lane's first on
+  const W* src = weight + (ok ? id * ld : 0) + c0 + lane * kE;
+  O* dst = out + t * dim + c0 + lane * kE;
+  for (int at = 0; at < n; at += kGroups * kStep) {
+    float v[kGroups][kE];
 #pragma unroll
-    for (int k = 0; k < LK_LANE; ++k) v[k] = ok ? load1(src + at + 32 * k) : 0.f;
+    for (int k = 0; k < kGroups; ++k) {
 #pragma unroll
-    for (int k = 0; k < LK_LANE; ++k) store1(dst + at + 32 * k, v[k] * scale);
-  }
-  if (at < n) {
-    float v[LK_LANE];
+      for (int i = 0; i < kE; ++i) v[k][i] = 0.f;
+      if (ok && at + k * kStep < n) load_group<kE>(src + at + k * kStep, v[k]);
+    }
 #pragma unroll
-    for (int k = 0; k < LK_LANE; ++k) v[k] = ok && at + lane + 32 * k < n ? load1(src + at + 32 * k) : 0.f;
+    for (int k = 0; k < kGroups; ++k) {
 #pragma unroll
-    for (int k = 0; k < LK_LANE; ++k)
-      if (at + lane + 32 * k < n) store1(dst + at + 32 * k, v[k] * scale);
+      for (int i = 0; i < kE; ++i) v[k][i] *= scale;
+      if (at + k * kStep < n) store_group<kE>(dst + at + k * kStep, v[k]);
+    }
   }
 }
 
 template <typename W, typename O>
 int run_lookup(const void* weight, int64_t rows, int64_t dim, int64_t ld, const void* ids, bool wide, int64_t tokens,
                float scale, void* out, int* err, cudaStream_t stream) {
-  const bool vec = dim % kVec == 0 && ld % kVec == 0 &&
-                   ((reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+  const int width = group_width(dim, ld, weight, sizeof(W), out, sizeof(O));
+  const bool flat = width == kVec;
   const int64_t groups = dim / kVec, parts = (dim + LK_COLS - 1) / LK_COLS;
-  const int64_t units = vec ? tokens * groups : tokens * parts, per = vec ? LK_THREADS * LK_PER : LK_THREADS / 32;
+  const int64_t units = flat ? tokens * groups : tokens * parts, per = flat ? LK_THREADS * LK_PER : LK_THREADS / 32;
   const int64_t blocks = (units + per - 1) / per;
   if (blocks > 0x7fffffffLL) return set_error(MUON_ERR_ARG, "embedding output too large");
   const unsigned grid = static_cast<unsigned>(blocks);
   const W* w = static_cast<const W*>(weight);
   O* o = static_cast<O*>(out);
-  if (vec)
+  auto by_rows = [&](auto kernel) {
+    kernel<<<grid, LK_THREADS, 0, stream>>>(w, rows, ld, ids, wide, tokens, dim, parts, scale, o, err);
+  };
+  if (flat)
     lookup_kernel<W, O><<<grid, LK_THREADS, 0, stream>>>(w, rows, ld, ids, wide, tokens,
                                                          static_cast<uint32_t>(groups), scale, o, err);
+  else if (width == 4)
+    by_rows(lookup_rows_kernel<4, W, O>);
+  else if (width == 2)
+    by_rows(lookup_rows_kernel<2, W, O>);
   else
-    lookup_rows_kernel<W, O><<<grid, LK_THREADS, 0, stream>>>(w, rows, ld, ids, wide, tokens, dim, parts, scale, o,
-                                                              err);
+    by_rows(lookup_rows_kernel<1, W, O>);
   return check_cuda(cudaGetLastError(), "embedding launch");
 }
 
@@ -187,7 +247,7 @@ int run_lookup(const void* weight, int64_t rows, int64_t dim, int64_t ld, const 
 // is kept.
 constexpr int RS_BITS = 9;
 constexpr int RS_BINS = 1 << RS_BITS;
-constexpr int RS_THREADS = 1024;
+constexpr int RS_THREADS = RS_BINS;  // a thread a bin
 constexpr int RS_WARPS = RS_THREADS / 32;
 constexpr int RS_MAX_PASSES = 4;
 
@@ -224,7 +284,7 @@ __device__ __forceinline__ uint32_t block_exclusive(uint32_t x, uint32_t* sums, 
   const uint32_t inc = warp_inclusive(x);
   if (lane == 31) sums[warp] = inc;
   __syncthreads();
-  const uint32_t mine = sums[lane];
+  const uint32_t mine = lane < RS_WARPS ? sums[lane] : 0;
   const uint32_t all = warp_inclusive(mine);
   const uint32_t before = __shfl_sync(0xffffffffu, all - mine, warp);
   if (total) *total = __shfl_sync(0xffffffffu, all, 31);
@@ -261,19 +321,16 @@ __device__ __forceinline__ void warp_ranks(uint16_t* counts, uint32_t (&rank)[kP
   }
 }
 
-// counts[warp][bin] -> how many keys of that bin the warps before hold; returns the bin's total (threads below
-// RS_BINS; 0 otherwise).
+// counts[warp][bin] -> how many keys of that bin the warps before hold; returns the total of the thread's bin.
 __device__ __forceinline__ uint32_t scan_warps(uint16_t (*counts)[RS_BINS]) {
   uint32_t run = 0;
-  if (threadIdx.x < RS_BINS) {
-    uint16_t c[RS_WARPS];
+  uint16_t c[RS_WARPS];
 #pragma unroll
-    for (int w = 0; w < RS_WARPS; ++w) c[w] = counts[w][threadIdx.x];
+  for (int w = 0; w < RS_WARPS; ++w) c[w] = counts[w][threadIdx.x];
 #pragma unroll
-    for (int w = 0; w < RS_WARPS; ++w) {
-      counts[w][threadIdx.x] = static_cast<uint16_t>(run);
-      run += c[w];
-    }
+  for (int w = 0; w < RS_WARPS; ++w) {
+    counts[w][threadIdx.x] = static_cast<uint16_t>(run);
+    run += c[w];
   }
   return run;
 }
@@ -301,8 +358,9 @@ __device__ __forceinline__ uint32_t run_heads(const uint32_t (&key)[kPer], uint3
   return mine;
 }
 
-// Sort of up to RS_THREADS tokens in one block, with the run starts counted
-// on the way out.
+// Sort of up to RS_THREADS x kPer tokens in one block, with the run starts
+// counted on the way out.
+template <int kPer>
 __global__ void __launch_bounds__(RS_THREADS) block_sort_kernel(TokenSource src, int n, int passes, int bits,
                                                                 int chunk, uint32_t* __restrict__ out_keys,
                                                                 uint32_t* __restrict__ out_pos,
@@ -310,79 +368,20 @@ __global__ void __launch_bounds__(RS_THREADS) block_sort_kernel(TokenSource src,
                                                                 uint32_t* __restrict__ tile_base,
                                                                 uint32_t* __restrict__ long_count,
                                                                 int64_t* __restrict__ row_count, int* err) {
-  __shared__ uint32_t skey[RS_THREADS];
-  __shared__ uint16_t spos[RS_THREADS];
+  __shared__ uint32_t skey[RS_THREADS * kPer];
+  __shared__ uint16_t spos[RS_THREADS * kPer];
   __shared__ uint16_t counts[RS_WARPS][RS_BINS];
   __shared__ uint16_t base[RS_BINS];
   __shared__ uint32_t sums[RS_WARPS];
   allow_next();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = threadIdx.x;
-  const uint32_t rows = static_cast<uint32_t>(src.rows), mask = (1u << bits) - 1u;
-  uint32_t key[1] = {e < n ? token_key(src, e, err) : 0xffffffffu};  // places past n sort last: all digits highest
-  uint32_t pos = e;
-  for (int p = 0; p < passes; ++p) {
-    const int shift = p * bits;
-    clear_counts(counts);
-    __syncthreads();
-    uint32_t rank[1];
-    const uint32_t d = (key[0] >> shift) & mask;
-    warp_ranks<1>(counts[warp], rank, [&](int) { return d; });
-    __syncthreads();
-    const uint32_t first = block_exclusive(scan_warps(counts), sums);
-    if (threadIdx.x < RS_BINS) base[threadIdx.x] = static_cast<uint16_t>(first);
-    __syncthreads();
-    const uint32_t to = base[d] + counts[warp][d] + rank[0];
-    skey[to] = key[0];
-    spos[to] = static_cast<uint16_t>(pos);
-    __syncthreads();
-    key[0] = skey[e];
-    pos = spos[e];
-  }
-  uint32_t heads[1], total;
-  const uint32_t mine = run_heads<1>(key, rows, heads, [&](int) { return e > 0 ? skey[e - 1] : 0xffffffffu; });
-  if (e < n) {
-    out_keys[e] = key[0];
-    out_pos[e] = pos;
-  }
-  uint32_t before = block_exclusive(lane == 0 ? mine : 0, sums, &total);
-  before = __shfl_sync(0xffffffffu, before, 0);  // run starts before this warp's first position
-  if (e < n && e % chunk == 0) chunk_base[e / chunk] = before + __popc(heads[0] & ((1u << lane) - 1u));
-  if (threadIdx.x == 0) {
-    tile_base[0] = 0;
-    *long_count = 0;
-    if (row_count) *row_count = total;
-  }
-}
-
-// The same by a cluster of eight blocks for up to 8 x RS_THREADS x kPer
-// tokens: the digit totals cross the blocks through distributed shared
-// memory, the scattered keys through L2 (one block alone needs 44 us for
-// 16384 tokens, bound by its instruction issue).
-constexpr int CL_BLOCKS = 8;
-
-template <int kPer>
-__global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(RS_THREADS)
-    cluster_sort_kernel(TokenSource src, int n, int passes, int bits, int chunk, uint32_t* keys0, uint32_t* pos0,
-                        uint32_t* keys1, uint32_t* pos1, uint32_t* __restrict__ chunk_base,
-                        uint32_t* __restrict__ tile_base, uint32_t* __restrict__ long_count,
-                        int64_t* __restrict__ row_count, int* err) {
-  __shared__ uint16_t counts[RS_WARPS][RS_BINS];
-  __shared__ uint32_t totals[RS_BINS];
-  __shared__ uint32_t base[RS_BINS];
-  __shared__ uint32_t sums[RS_WARPS];
-  __shared__ uint32_t block_heads;
-  allow_next();
-  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
-  const unsigned block = cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int e0 = int(block) * RS_THREADS * kPer + warp * 32 * kPer + lane;
+  const int e0 = warp * 32 * kPer + lane;
   const uint32_t rows = static_cast<uint32_t>(src.rows), mask = (1u << bits) - 1u;
-  uint32_t key[kPer], pos[kPer];  // element e0 + 32 i
+  uint32_t key[kPer], pos[kPer];  // element e0 + 32 i; places past n sort last: all digits highest
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int e = e0 + 32 * i;
-    key[i] = e < n ? token_key(src, e, err) : 0xffffffffu;
-    pos[i] = e;
+    pos[i] = e0 + 32 * i;
+    key[i] = e0 + 32 * i < n ? token_key(src, e0 + 32 * i, err) : 0xffffffffu;
   }
   for (int p = 0; p < passes; ++p) {
     const int shift = p * bits;
@@ -391,70 +390,137 @@ __global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(RS_THREADS)
     uint32_t rank[kPer];
     warp_ranks<kPer>(counts[warp], rank, [&](int i) { return (key[i] >> shift) & mask; });
     __syncthreads();
-    const uint32_t mine = scan_warps(counts);
-    if (threadIdx.x < RS_BINS) totals[threadIdx.x] = mine;
-    cluster.sync();
-    uint32_t all = 0, before = 0;
-    if (threadIdx.x < RS_BINS) {
-#pragma unroll
-      for (unsigned q = 0; q < CL_BLOCKS; ++q) {
-        const uint32_t c = *cluster.map_shared_rank(&totals[threadIdx.x], q);
-        all += c;
-        if (q < block) before += c;
-      }
-    }
-    const uint32_t first = block_exclusive(all, sums);
-    if (threadIdx.x < RS_BINS) base[threadIdx.x] = first + before;
+    const uint32_t first = block_exclusive(scan_warps(counts), sums);
+    base[threadIdx.x] = static_cast<uint16_t>(first);
     __syncthreads();
-    uint32_t* out_keys = p & 1 ? keys1 : keys0;
-    uint32_t* out_pos = p & 1 ? pos1 : pos0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const uint32_t d = (key[i] >> shift) & mask;
       const uint32_t to = base[d] + counts[warp][d] + rank[i];
-      if (to < uint32_t(n)) {  // the places past n stay behind
-        out_keys[to] = key[i];
-        out_pos[to] = pos[i];
-      }
+      skey[to] = key[i];
+      spos[to] = static_cast<uint16_t>(pos[i]);
     }
-    cluster.sync();
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {  // written by other SMs: past this one's L1
-      const int e = e0 + 32 * i;
-      key[i] = e < n ? __ldcg(out_keys + e) : 0xffffffffu;
-      if (p + 1 < passes) pos[i] = e < n ? __ldcg(out_pos + e) : 0;
+    for (int i = 0; i < kPer; ++i) {
+      key[i] = skey[e0 + 32 * i];
+      pos[i] = spos[e0 + 32 * i];
     }
   }
-  const uint32_t* sorted = (passes - 1) & 1 ? keys1 : keys0;
-  uint32_t heads[kPer], total = 0, before_block = 0;
+  uint32_t heads[kPer], total;
   const uint32_t mine = run_heads<kPer>(key, rows, heads, [&](int i) {
     const int e = e0 + 32 * i;
-    const uint32_t up = __shfl_up_sync(0xffffffffu, key[i], 1);
-    return lane > 0 ? up : (e > 0 && e < n ? __ldcg(sorted + e - 1) : 0xffffffffu);
+    return e > 0 ? skey[e - 1] : 0xffffffffu;
   });
   uint32_t before = block_exclusive(lane == 0 ? mine : 0, sums, &total);
-  if (threadIdx.x == 0) block_heads = total;
-  cluster.sync();
-  total = 0;
-#pragma unroll
-  for (unsigned q = 0; q < CL_BLOCKS; ++q) {
-    const uint32_t h = *cluster.map_shared_rank(&block_heads, q);
-    total += h;
-    if (q < block) before_block += h;
-  }
-  before = __shfl_sync(0xffffffffu, before, 0) + before_block;
+  before = __shfl_sync(0xffffffffu, before, 0);  // run starts before this warp's first position
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int e = e0 + 32 * i;
-    if (e < n && e % chunk == 0) chunk_base[e / chunk] = before + __popc(heads[i] & ((1u << lane) - 1u));
+    if (e < n) {
+      out_keys[e] = key[i];
+      out_pos[e] = pos[i];
+      if (e % chunk == 0) chunk_base[e / chunk] = before + __popc(heads[i] & ((1u << lane) - 1u));
+    }
     before += __popc(heads[i]);
   }
-  if (block == 0) {
-    if (int(threadIdx.x) * HD_TILE < n) tile_base[threadIdx.x] = 0;
-    if (threadIdx.x == 0) {
-      *long_count = 0;
-      if (row_count) *row_count = total;
+  if (threadIdx.x == 0) {
+    tile_base[0] = 0;
+    *long_count = 0;
+    if (row_count) *row_count = total;
+  }
+}
+
+// The same by a cluster of eight blocks for up to 8 x RS_THREADS x kPer
+// tokens (one block alone needs 44 us for 16384, bound by its instruction
+// issue): digit totals and the scattered keys cross the blocks through
+// distributed shared memory. tile_base gets each block's own run starts.
+constexpr int CL_BLOCKS = 8;
+
+template <int kPer>
+struct ClusterSortShared {
+  uint2 recv[RS_THREADS * kPer];  // (key, position) that this block holds after a pass
+  uint16_t counts[RS_WARPS][RS_BINS];
+  uint32_t totals[RS_BINS];
+  uint32_t base[RS_BINS];
+  uint32_t sums[RS_WARPS];
+};
+
+template <int kPer>
+__global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(RS_THREADS)
+    cluster_sort_kernel(TokenSource src, int n, int passes, int bits, int chunk, uint32_t* __restrict__ out_keys,
+                        uint32_t* __restrict__ out_pos, uint32_t* __restrict__ chunk_base,
+                        uint32_t* __restrict__ tile_base, uint32_t* __restrict__ long_count, int* err) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  ClusterSortShared<kPer>& sh = *reinterpret_cast<ClusterSortShared<kPer>*>(raw);
+  constexpr int kHeld = RS_THREADS * kPer;
+  allow_next();
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const unsigned block = cluster.block_rank();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int h0 = warp * 32 * kPer + lane, e0 = int(block) * kHeld + h0;
+  const uint32_t rows = static_cast<uint32_t>(src.rows), mask = (1u << bits) - 1u;
+  uint32_t key[kPer], pos[kPer];  // element e0 + 32 i; places past n sort last: all digits highest
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = e0 + 32 * i;
+    key[i] = e < n ? token_key(src, e, err) : 0xffffffffu;
+    pos[i] = e;
+  }
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * bits;
+    clear_counts(sh.counts);
+    __syncthreads();
+    uint32_t rank[kPer];
+    warp_ranks<kPer>(sh.counts[warp], rank, [&](int i) { return (key[i] >> shift) & mask; });
+    __syncthreads();
+    sh.totals[threadIdx.x] = scan_warps(sh.counts);
+    cluster.sync();  // totals written, and recv of the pass before read
+    uint32_t all = 0, before = 0;
+#pragma unroll
+    for (unsigned q = 0; q < CL_BLOCKS; ++q) {
+      const uint32_t c = *cluster.map_shared_rank(&sh.totals[threadIdx.x], q);
+      all += c;
+      if (q < block) before += c;
     }
+    const uint32_t first = block_exclusive(all, sh.sums);
+    sh.base[threadIdx.x] = first + before;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t d = (key[i] >> shift) & mask;
+      const uint32_t to = sh.base[d] + sh.counts[warp][d] + rank[i];
+      *cluster.map_shared_rank(&sh.recv[to % kHeld], to / kHeld) = make_uint2(key[i], pos[i]);
+    }
+    cluster.sync();  // recv written, and totals read
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint2 x = sh.recv[h0 + 32 * i];
+      key[i] = x.x;
+      pos[i] = x.y;
+    }
+  }
+  uint32_t heads[kPer], total;
+  const uint32_t mine = run_heads<kPer>(key, rows, heads, [&](int i) {
+    const int h = h0 + 32 * i;
+    if (h > 0) return sh.recv[h - 1].x;
+    return block > 0 ? cluster.map_shared_rank(&sh.recv[kHeld - 1], block - 1)->x : 0xffffffffu;
+  });
+  uint32_t before = block_exclusive(lane == 0 ? mine : 0, sh.sums, &total);
+  before = __shfl_sync(0xffffffffu, before, 0);  // run starts in this block before this warp's first position
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = e0 + 32 * i;
+    if (e < n) {
+      out_keys[e] = key[i];
+      out_pos[e] = pos[i];
+      if (e % chunk == 0) chunk_base[e / chunk] = before + __popc(heads[i] & ((1u << lane) - 1u));
+    }
+    before += __popc(heads[i]);
+  }
+  if (threadIdx.x == 0) {
+    tile_base[block] = total;
+    if (block == 0) *long_count = 0;
   }
   cluster.sync();  // no block leaves while another reads its shared memory
 }
@@ -463,7 +529,7 @@ __global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(RS_THREADS)
 // scatter a pass. A scatter block adds the tiles' counts itself (its first
 // positions are the sums over the smaller digits and the tiles before it)
 // and counts the next pass's digits by destination tile as it writes.
-constexpr int RS_PER = 4;
+constexpr int RS_PER = 8;
 constexpr int RS_TILE = RS_THREADS * RS_PER;
 
 __global__ void __launch_bounds__(RS_THREADS) radix_count_kernel(TokenSource src, int64_t n, int bits, int passes,
@@ -472,10 +538,8 @@ __global__ void __launch_bounds__(RS_THREADS) radix_count_kernel(TokenSource src
   __shared__ uint32_t h[RS_BINS];
   allow_next();
   const int lane = threadIdx.x & 31;
-  if (threadIdx.x < RS_BINS) {
-    h[threadIdx.x] = 0;
-    for (int p = 1; p < passes; ++p) hist[(p * tiles + blockIdx.x) * RS_BINS + threadIdx.x] = 0;
-  }
+  h[threadIdx.x] = 0;
+  for (int p = 1; p < passes; ++p) hist[(p * tiles + blockIdx.x) * RS_BINS + threadIdx.x] = 0;
   if (blockIdx.x == 0 && threadIdx.x < 2) zeroed[threadIdx.x] = 0;
   __syncthreads();
   const int64_t base = int64_t(blockIdx.x) * RS_TILE;
@@ -488,7 +552,7 @@ __global__ void __launch_bounds__(RS_THREADS) radix_count_kernel(TokenSource src
       atomicAdd(&h[d], static_cast<uint32_t>(__popc(peers)));
   }
   __syncthreads();
-  if (threadIdx.x < RS_BINS) hist[int64_t(blockIdx.x) * RS_BINS + threadIdx.x] = h[threadIdx.x];
+  hist[int64_t(blockIdx.x) * RS_BINS + threadIdx.x] = h[threadIdx.x];
 }
 
 __global__ void __launch_bounds__(RS_THREADS) radix_scatter_kernel(TokenSource src, const uint32_t* __restrict__ keys,
@@ -499,7 +563,6 @@ __global__ void __launch_bounds__(RS_THREADS) radix_scatter_kernel(TokenSource s
                                                                    uint32_t* __restrict__ out_keys,
                                                                    uint32_t* __restrict__ out_pos) {
   __shared__ uint16_t counts[RS_WARPS][RS_BINS];
-  __shared__ uint32_t half[2][RS_BINS];
   __shared__ uint32_t base[RS_BINS];
   __shared__ uint32_t sums[RS_WARPS];
   allow_next();
@@ -519,22 +582,18 @@ __global__ void __launch_bounds__(RS_THREADS) radix_scatter_kernel(TokenSource s
       if (keys) pos[i] = positions[e];
     }
   }
-  // this tile's first position of every digit: two threads a bin, half of the tiles each
-  const int bin = threadIdx.x & (RS_BINS - 1), part = threadIdx.x / RS_BINS;
+  // this tile's first position of every digit, a thread a digit
   uint32_t before = 0, total = 0;
-  const int64_t mid = (tiles + 1) / 2;
-#pragma unroll 8
-  for (int64_t t = part ? mid : 0; t < (part ? tiles : mid); ++t) {
-    const uint32_t c = hist[t * RS_BINS + bin];
+#pragma unroll 16
+  for (int64_t t = 0; t < tiles; ++t) {
+    const uint32_t c = hist[t * RS_BINS + threadIdx.x];
     total += c;
     if (t < int64_t(blockIdx.x)) before += c;
   }
-  if (part) half[0][bin] = before, half[1][bin] = total;
   __syncthreads();
-  if (!part) before += half[0][bin], total += half[1][bin];
   warp_ranks<RS_PER>(counts[warp], rank, [&](int i) { return (key[i] >> shift) & mask; });
-  const uint32_t first = block_exclusive(part ? 0 : total, sums);
-  if (!part) base[bin] = first + before;
+  const uint32_t first = block_exclusive(total, sums);
+  base[threadIdx.x] = first + before;
   scan_warps(counts);
   __syncthreads();
 #pragma unroll
@@ -628,16 +687,18 @@ __global__ void __launch_bounds__(HD_THREADS) heads_kernel(const uint32_t* __res
 constexpr int SUM_THREADS = 256;
 constexpr int SUM_WARPS = SUM_THREADS / 32;
 constexpr int SUM_STAGE_BYTES = 4096;  // rows in flight of one warp
-constexpr int ZERO_BYTES = 8192;         // of rows one warp of the zero part looks after
+constexpr int64_t ZERO_BYTES = 8192;         // of rows one warp of the zero part looks after
 
-template <bool kVector, typename T>
-__device__ __forceinline__ void store_cols(T* row, int64_t col, int64_t dim, const float (&v)[kVec]) {
-  if constexpr (kVector) {
-    if (col < dim) store8(row + col, v);
-  } else {
+// A lane's 8 of a slice's 256 columns: groups of kE, 32 kE columns apart.
+template <int kE, typename T>
+__device__ __forceinline__ void store_cols(T* row, int64_t slice, int64_t dim, const float (&v)[kVec]) {
+  const int64_t col = slice * kSlice + (threadIdx.x & 31) * kE;
 #pragma unroll
-    for (int k = 0; k < kVec; ++k)
-      if (col + 32 * k < dim) store1(row + col + 32 * k, v[k]);
+  for (int k = 0; k < kVec / kE; ++k) {
+    float g[kE];
+#pragma unroll
+    for (int i = 0; i < kE; ++i) g[i] = v[k * kE + i];
+    if (col + k * 32 * kE < dim) store_group<kE>(row + col + k * 32 * kE, g);
   }
 }
 
@@ -661,13 +722,22 @@ struct SumArgs {
   float scale;
   const uint32_t* chunk_base;
   const uint32_t* tile_base;
+  int64_t tile;    // positions that share one entry of tile_base
+  int raw_tiles;   // entries of tile_base that hold counts of their own, to be added up (0: sums already)
   int64_t cap;
   int64_t* out_ids;  // NULL: dense form
-  const int64_t* count;
+  int64_t* count;
   float* partial;  // [chunks][2][slices * kSlice]: a run from an earlier chunk; a long run starting here
   LongRun* long_list;
   uint32_t* long_count;
 };
+
+// Run starts before tile `t` (t = raw_tiles: all of them), by a whole warp.
+__device__ __forceinline__ uint32_t heads_before(const SumArgs& a, int t) {
+  if (a.raw_tiles == 0) return a.tile_base[t];
+  const int lane = threadIdx.x & 31;
+  return __reduce_add_sync(0xffffffffu, lane < t ? a.tile_base[lane] : 0u);
+}
 
 // First index in keys[lo, hi) whose key is >= `key`, by a whole warp: 32
 // probes a step, four dependent loads for a million tokens.
@@ -691,45 +761,61 @@ template <typename O>
 __device__ __forceinline__ void zero_span(O* out, int64_t begin, int64_t end) {
   constexpr int kPer = 16 / sizeof(O);
   const int lane = threadIdx.x & 31;
+  const float zero[1] = {0.f};
   const int64_t skew = (reinterpret_cast<uintptr_t>(out) / sizeof(O)) % kPer;  // elements past a 16-byte boundary
   const int64_t body = min(end, (begin + skew + kPer - 1) / kPer * kPer - skew);
-  for (int64_t e = begin + lane; e < body; e += 32) store1(out + e, 0.f);
+  for (int64_t e = begin + lane; e < body; e += 32) store_group<1>(out + e, zero);
   const int64_t vectors = (end - body) / kPer;
   uint4* v = reinterpret_cast<uint4*>(out + body);
   for (int64_t i = lane; i < vectors; i += 32) v[i] = make_uint4(0, 0, 0, 0);
-  for (int64_t e = body + vectors * kPer + lane; e < end; e += 32) store1(out + e, 0.f);
+  for (int64_t e = body + vectors * kPer + lane; e < end; e += 32) store_group<1>(out + e, zero);
 }
 
 // Rows no token has: in the dense form the gaps between the sorted keys, in
 // the row form those past the count.
 template <typename O>
 __device__ __forceinline__ void zero_rows(O* out, const SumArgs& a, int64_t unit) {
+  const int lane = threadIdx.x & 31;
   const int64_t r0 = unit * a.zero_rows;
   if (a.out_ids) {
-    const int64_t from = max(r0, *a.count), to = min(r0 + a.zero_rows, a.cap);
+    const int64_t count = a.raw_tiles ? int64_t(heads_before(a, a.raw_tiles)) : *a.count;
+    if (a.raw_tiles && unit == 0 && lane == 0) *a.count = count;
+    const int64_t from = max(r0, count), to = min(r0 + a.zero_rows, a.cap);
     if (from >= to) return;
     zero_span(out, from * a.dim, to * a.dim);
-    for (int64_t r = from + (threadIdx.x & 31); r < to; r += 32) a.out_ids[r] = 0;
+    if (from + lane < to) a.out_ids[from + lane] = 0;
     return;
   }
-  const int64_t r1 = min(r0 + a.zero_rows, a.rows);
-  if (r0 >= r1) return;
+  const int n = static_cast<int>(min(a.zero_rows, a.rows - r0));  // at most 32
+  if (n <= 0) return;
+  // which of the rows have tokens, a bit each: 32 sorted keys at a time, long runs skipped by a search
+  uint32_t taken = 0;
   int64_t at = warp_lower_bound(a.keys, 0, a.n, r0);
-  int64_t row = r0;
-  while (true) {
-    const int64_t key = at < a.n ? min(int64_t(a.keys[at]), r1) : r1;
-    if (key > row) zero_span(out, row * a.dim, key * a.dim);
-    if (key == r1) break;
-    row = key + 1;
-    if (at + 1 < a.n && int64_t(a.keys[at + 1]) != key)
-      ++at;
-    else
-      at = warp_lower_bound(a.keys, at, a.n, row);
+  while (at < a.n) {
+    const uint32_t key = at + lane < a.n ? a.keys[at + lane] : 0xffffffffu;
+    const bool mine = int64_t(key) < r0 + n;
+    taken |= __reduce_or_sync(0xffffffffu, mine ? 1u << (key - uint32_t(r0)) : 0u);
+    if (!__all_sync(0xffffffffu, mine)) break;
+    const uint32_t first = __shfl_sync(0xffffffffu, key, 0), last = __shfl_sync(0xffffffffu, key, 31);
+    at = first == last ? warp_lower_bound(a.keys, at + 32, a.n, int64_t(last) + 1) : at + 32;
+  }
+  uint32_t empty = ~taken & (n == 32 ? 0xffffffffu : (1u << n) - 1u);
+  while (empty) {  // spans of rows without tokens
+    const int from = __ffs(empty) - 1;
+    const uint32_t above = ~(empty >> from);
+    const int span = above ? __ffs(above) - 1 : 32;
+    zero_span(out, (r0 + from) * a.dim, (r0 + from + span) * a.dim);
+    if (from + span >= 32) break;
+    empty &= ~0u << (from + span);
   }
 }
 
-__device__ __forceinline__ void copy_async16(uint32_t shared, const void* global) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared), "l"(global) : "memory");
+template <int kBytes>
+__device__ __forceinline__ void copy_async(uint32_t shared, const void* global) {
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared), "l"(global) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(shared), "l"(global), "n"(kBytes) : "memory");
 }
 __device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending>
@@ -737,18 +823,22 @@ __device__ __forceinline__ void copy_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
-// One chunk and 256 columns a warp. The rows of dY
-// come through a ring in shared memory (4 KB a warp, filled by asynchronous
-// copies that each lane makes and reads for itself), so few registers are
-// held. The blocks behind sum_blocks write the zeros, 8 KB of rows a warp: with 64 KB
-// the dense gradient of 16384 tokens (151936 x 2048 bf16) took 106-124 us, not 99, and
-// zeros laid among the other blocks 117.
-template <typename G, typename O, bool kVector>
+// One chunk and 256 columns a warp, eight columns a lane in groups of kE. The
+// rows of dY come through a ring in shared memory (4 KB a warp, filled by
+// asynchronous copies that each lane makes and reads for itself), so few
+// registers are held; single bf16 elements, too small for such copies, are
+// loaded four rows ahead instead. The blocks behind sum_blocks write the
+// zeros, 8 KB of rows a warp: with 64 KB the dense gradient of 16384 tokens
+// (151936 x 2048 bf16) took 106-124 us, not 99, and zeros laid among the other
+// blocks 117.
+template <int kE, typename G, typename O>
 __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ grad, O* __restrict__ out,
                                                           const SumArgs a) {
+  constexpr bool kRing = kE * sizeof(G) >= 4;
   constexpr int kStages = SUM_STAGE_BYTES / (kSlice * int(sizeof(G)));
-  constexpr int kCopies = kVec * sizeof(G) / 16;
-  __shared__ __align__(16) unsigned char ring[kVector ? SUM_WARPS : 1][kVector ? SUM_STAGE_BYTES : 16];
+  constexpr int kGroups = kVec / kE, kGroupBytes = kE * sizeof(G);
+  static_assert(kGroupBytes <= 16, "one asynchronous copy a group");
+  __shared__ __align__(16) unsigned char ring[kRing ? SUM_WARPS : 1][kRing ? SUM_STAGE_BYTES : 16];
   allow_next();
   wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -773,7 +863,7 @@ __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ 
   const uint32_t pos_b = lane < next ? a.pos[s1 + lane] : 0;
   const uint32_t before = s0 > 0 ? a.keys[s0 - 1] : none;
   const uint32_t before_last = s0 > a.chunk ? a.keys[s0 - a.chunk - 1] : none;
-  uint32_t slot = a.chunk_base[c] + a.tile_base[s0 / HD_TILE];
+  uint32_t slot = a.chunk_base[c] + heads_before(a, static_cast<int>(s0 / a.tile));
   const uint32_t first = __shfl_sync(0xffffffffu, key_a, 0);
   const uint32_t last = __shfl_sync(0xffffffffu, key_a, len - 1);
   const uint32_t next_first = __shfl_sync(0xffffffffu, key_b, 0);
@@ -805,7 +895,7 @@ __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ 
   const uint32_t ends_a =
       __ballot_sync(0xffffffffu, lane < len && key_a != (lane == len - 1 ? next_first : after_a));
   const uint32_t ends_b = __ballot_sync(0xffffffffu, lane < next && (lane == next - 1 || key_b != after_b));
-  const int64_t col = slice * kSlice + (kVector ? lane * kVec : lane);
+  const int64_t col = slice * kSlice + lane * kE;
   const int64_t pitch = a.slices * kSlice;
   float* part = a.partial + c * 2 * pitch + slice * kSlice + lane * kVec;
 
@@ -818,33 +908,31 @@ __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ 
     const bool run_ends = r < len ? (ends_a >> r) & 1u : (ends_b >> (r - len)) & 1u;
     if (!run_ends && r + 1 < end) return;
     if (r < lead) {
-      store8(part, acc);
+      store_group<kVec>(part, acc);
     } else if (tail && r == end - 1) {
-      store8(part + pitch, acc);
+      store_group<kVec>(part + pitch, acc);
     } else {
 #pragma unroll
       for (int j = 0; j < kVec; ++j) acc[j] *= a.scale;
       const uint32_t ka = __shfl_sync(0xffffffffu, key_a, r & 31);
       const uint32_t key = r < len ? ka : last;
       const int64_t row = a.out_ids ? int64_t(slot) : int64_t(key);
-      store_cols<kVector>(out + row * a.dim, col, a.dim, acc);
+      store_cols<kE>(out + row * a.dim, slice, a.dim, acc);
       if (a.out_ids && slice == 0 && lane == 0) a.out_ids[slot] = key;
       ++slot;
     }
 #pragma unroll
     for (int j = 0; j < kVec; ++j) acc[j] = 0.f;
   };
-  if constexpr (kVector) {
-    const bool on = col < a.dim;
-    const uint32_t mine = smem_u32(ring[warp]) + lane * 16;
-    const uint4* mine_read = reinterpret_cast<const uint4*>(ring[warp]) + lane;
+  if constexpr (kRing) {
+    const unsigned char* mine = ring[warp] + lane * kGroupBytes;
+    const uint32_t mine_to = smem_u32(mine);
     auto fetch = [&](int r) {
-      const G* row = row_of(r);
-      if (on) {
+      const G* row = row_of(r) + col;
 #pragma unroll
-        for (int q = 0; q < kCopies; ++q)
-          copy_async16(mine + ((r % kStages) * kCopies + q) * 512, row + col + q * (16 / int(sizeof(G))));
-      }
+      for (int k = 0; k < kGroups; ++k)
+        if (col + k * 32 * kE < a.dim)
+          copy_async<kGroupBytes>(mine_to + ((r % kStages) * kGroups + k) * 32 * kGroupBytes, row + k * 32 * kE);
     };
     for (int r = begin; r < begin + kStages; ++r) {
       if (r < end) fetch(r);
@@ -852,36 +940,39 @@ __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ 
     }
     for (int r = begin; r < end; ++r) {
       copy_async_wait<kStages - 1>();
-      if constexpr (sizeof(G) == 2) {
-        const uint4 x = mine_read[(r % kStages) * 32];
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&x);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = __bfloat1622float2(h[j]);
-          acc[2 * j] += f.x;
-          acc[2 * j + 1] += f.y;
-        }
-      } else {
+      for (int k = 0; k < kGroups; ++k) {
+        float v[kE];
+        load_group<kE>(reinterpret_cast<const G*>(mine + ((r % kStages) * kGroups + k) * 32 * kGroupBytes), v);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const uint4 x = mine_read[((r % kStages) * 2 + q) * 32];
-          acc[4 * q] += __uint_as_float(x.x);
-          acc[4 * q + 1] += __uint_as_float(x.y);
-          acc[4 * q + 2] += __uint_as_float(x.z);
-          acc[4 * q + 3] += __uint_as_float(x.w);
-        }
+        for (int i = 0; i < kE; ++i) acc[k * kE + i] += v[i];
       }
       if (r + kStages < end) fetch(r + kStages);
       copy_async_commit();
       finish(r);
     }
   } else {
-    for (int r = begin; r < end; ++r) {
-      const G* row = row_of(r);
+    constexpr int kAhead = 4;
+    for (int r0 = begin; r0 < end; r0 += kAhead) {
+      float v[kAhead][kVec];
 #pragma unroll
-      for (int k = 0; k < kVec; ++k)
-        if (col + 32 * k < a.dim) acc[k] += load1(row + col + 32 * k);
-      finish(r);
+      for (int q = 0; q < kAhead; ++q) {
+        if (r0 + q >= end) continue;
+        const G* row = row_of(r0 + q) + col;
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) {
+          float x[1] = {0.f};
+          if (col + 32 * k < a.dim) load_group<1>(row + 32 * k, x);
+          v[q][k] = x[0];
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        if (r0 + q >= end) continue;
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) acc[k] += v[q][k];
+        finish(r0 + q);
+      }
     }
   }
   if (tail && slice == 0) {  // list the run for the join: it reaches the last chunk whose first key is its own
@@ -897,7 +988,7 @@ __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ 
 // -------------------------------------------------------------------- join
 // One block per (long run, slice): the run's partial rows, split evenly over
 // the warps in chunk order, then the warps' sums in order.
-template <typename O, bool kVector>
+template <int kE, typename O>
 __global__ void __launch_bounds__(SUM_THREADS) join_kernel(O* __restrict__ out, const SumArgs a) {
   __shared__ float red[SUM_WARPS][kSlice];
   wait_previous();
@@ -914,15 +1005,13 @@ __global__ void __launch_bounds__(SUM_THREADS) join_kernel(O* __restrict__ out, 
 #pragma unroll 4
     for (int64_t p = p0; p < p1; ++p) {
       float v[kVec];
-      load8(part + (p * 2 + (p == 0 ? 1 : 0)) * pitch, v);
+      load_group<kVec>(part + (p * 2 + (p == 0 ? 1 : 0)) * pitch, v);
 #pragma unroll
       for (int j = 0; j < kVec; ++j) acc[j] += v[j];
     }
-    store8(&red[warp][lane * kVec], acc);
+    store_group<kVec>(&red[warp][lane * kVec], acc);
     __syncthreads();
     if (warp == 0) {
-      // element j of this lane sits at column lane * 8 + j (vector) or lane + 32 j of the slice, in both
-      // layouts at red[..][lane * 8 + j]
       float w[kVec];
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
@@ -930,7 +1019,7 @@ __global__ void __launch_bounds__(SUM_THREADS) join_kernel(O* __restrict__ out, 
         for (int q = 0; q < SUM_WARPS; ++q) sum += red[q][lane * kVec + j];
         w[j] = sum * a.scale;
       }
-      store_cols<kVector>(out + run.row * a.dim, slice * kSlice + (kVector ? lane * kVec : lane), a.dim, w);
+      store_cols<kE>(out + run.row * a.dim, slice, a.dim, w);
     }
     __syncthreads();
   }
@@ -952,7 +1041,7 @@ int chunk_for(int64_t tokens, int64_t slices) {
   return chunk;
 }
 
-constexpr int64_t kClusterSort = CL_BLOCKS * RS_THREADS * 4;  // tokens; more are sorted by tiles
+constexpr int64_t kClusterSort = CL_BLOCKS * RS_THREADS * 8;  // tokens; more are sorted by tiles
 
 struct GradLayout {
   int64_t keys[2], pos[2], hist, chunk_base, tile_base, long_list, counters, partial, total;
@@ -975,7 +1064,7 @@ GradLayout grad_layout(int64_t n, int64_t dim) {
   for (int i = 0; i < 2; ++i) l.keys[i] = take(4 * n), l.pos[i] = take(4 * n);
   l.hist = take(n > kClusterSort ? 4 * RS_MAX_PASSES * l.tiles * RS_BINS : 0);
   l.chunk_base = take(4 * l.chunks);
-  l.tile_base = take(4 * ((n + HD_TILE - 1) / HD_TILE));
+  l.tile_base = take(4 * ((n + HD_TILE - 1) / HD_TILE + CL_BLOCKS));
   l.long_list = take(sizeof(LongRun) * l.chunks);
   l.counters = take(8);  // long runs, finished blocks of heads_kernel
   l.partial = take(8 * l.chunks * l.slices * kSlice);
@@ -988,24 +1077,34 @@ bool float_type(int dtype) { return dtype == MUON_BF16 || dtype == MUON_F32; }
 // elements x 4 bytes must fit an int64 with room to spare
 bool too_large(int64_t a, int64_t b) { return b > 0 && a > (int64_t(1) << 58) / b; }
 
+template <int kE, typename G, typename O>
+int run_sum(const void* grad, void* out, const SumArgs& a, unsigned grid, cudaStream_t stream) {
+  const G* g = static_cast<const G*>(grad);
+  O* o = static_cast<O*>(out);
+  if (int rc = launch_overlapped("embedding gradient sum launch", sum_kernel<kE, G, O>, grid, SUM_THREADS, stream, g, o, a))
+    return rc;
+  const unsigned join_grid = static_cast<unsigned>(a.chunks * a.slices < 592 ? a.chunks * a.slices : 592);
+  return launch_overlapped("embedding gradient join launch", join_kernel<kE, O>, join_grid, SUM_THREADS, stream, o, a);
+}
+
 template <typename G, typename O>
 int run_sum(const void* grad, void* out, SumArgs a, cudaStream_t stream) {
-  const bool vec = a.dim % kVec == 0 &&
-                   ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
   a.sum_blocks = (a.chunks * a.slices + SUM_WARPS - 1) / SUM_WARPS;
   const int64_t row_bytes = a.dim * int64_t(sizeof(O)), rows = a.out_ids ? a.cap : a.rows;
-  a.zero_rows = row_bytes >= ZERO_BYTES ? 1 : ZERO_BYTES / row_bytes;
+  a.zero_rows = std::clamp(ZERO_BYTES / row_bytes, int64_t(1), int64_t(32));  // a lane or a bit each
   const int64_t blocks = a.sum_blocks + (rows + a.zero_rows * SUM_WARPS - 1) / (a.zero_rows * SUM_WARPS);
   if (blocks > 0x7fffffffLL) return set_error(MUON_ERR_ARG, "embedding gradient too large");
   const unsigned grid = static_cast<unsigned>(blocks);
-  const G* g = static_cast<const G*>(grad);
-  O* o = static_cast<O*>(out);
-  if (int rc = launch_overlapped("embedding gradient sum launch", vec ? sum_kernel<G, O, true> : sum_kernel<G, O, false>,
-                                 grid, SUM_THREADS, stream, g, o, a))
-    return rc;
-  const unsigned join_grid = static_cast<unsigned>(a.chunks * a.slices < 592 ? a.chunks * a.slices : 592);
-  return launch_overlapped("embedding gradient join launch", vec ? join_kernel<O, true> : join_kernel<O, false>,
-                           join_grid, SUM_THREADS, stream, o, a);
+  switch (group_width(a.dim, a.dim, grad, sizeof(G), out, sizeof(O))) {
+    case 8:
+      if constexpr (sizeof(G) == 2) return run_sum<8, G, O>(grad, out, a, grid, stream);  // else as four
+    case 4:
+      return run_sum<4, G, O>(grad, out, a, grid, stream);
+    case 2:
+      return run_sum<2, G, O>(grad, out, a, grid, stream);
+    default:
+      return run_sum<1, G, O>(grad, out, a, grid, stream);
+  }
 }
 
 }  // namespace
@@ -1072,24 +1171,38 @@ int launch_embedding_grad(const void* grad, int grad_dtype, const void* ids, int
   const TokenSource src{ids, ids_dtype == MUON_I64, rows, padding_idx};
   uint32_t* counters = u32(l.counters);
   int64_t* row_count = out_ids ? count : nullptr;
+  SumArgs a{};
+  a.tile = HD_TILE;
   int cur = 0;
   if (tokens <= kClusterSort) {
     const int n = static_cast<int>(tokens);
-    auto cluster_sort = [&](auto kernel) {
-      kernel<<<CL_BLOCKS, RS_THREADS, 0, stream>>>(src, n, passes, per, l.chunk, u32(l.keys[0]), u32(l.pos[0]),
-                                                   u32(l.keys[1]), u32(l.pos[1]), u32(l.chunk_base), u32(l.tile_base),
-                                                   counters, row_count, err);
-      cur = (passes - 1) & 1;
+    auto cluster_sort = [&](auto kernel, int per_thread, size_t smem) {
+      if (smem > 48 * 1024 &&
+          check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)),
+                     "cluster sort attribute"))
+        return int(MUON_ERR_CUDA);
+      kernel<<<CL_BLOCKS, RS_THREADS, smem, stream>>>(src, n, passes, per, l.chunk, u32(l.keys[0]), u32(l.pos[0]),
+                                                      u32(l.chunk_base), u32(l.tile_base), counters, err);
+      a.tile = RS_THREADS * per_thread;
+      a.raw_tiles = CL_BLOCKS;
+      return int(MUON_OK);
+    };
+    int rc = MUON_OK;
+    auto block_sort = [&](auto kernel) {
+      kernel<<<1, RS_THREADS, 0, stream>>>(src, n, passes, per, l.chunk, u32(l.keys[0]), u32(l.pos[0]),
+                                           u32(l.chunk_base), u32(l.tile_base), counters, row_count, err);
     };
     if (n <= RS_THREADS)
-      block_sort_kernel<<<1, RS_THREADS, 0, stream>>>(src, n, passes, per, l.chunk, u32(l.keys[0]), u32(l.pos[0]),
-                                                      u32(l.chunk_base), u32(l.tile_base), counters, row_count, err);
-    else if (n <= CL_BLOCKS * RS_THREADS)
-      cluster_sort(cluster_sort_kernel<1>);
+      block_sort(block_sort_kernel<1>);
+    else if (n <= RS_THREADS * 4)
+      block_sort(block_sort_kernel<4>);
     else if (n <= CL_BLOCKS * RS_THREADS * 2)
-      cluster_sort(cluster_sort_kernel<2>);
+      rc = cluster_sort(cluster_sort_kernel<2>, 2, sizeof(ClusterSortShared<2>));
+    else if (n <= CL_BLOCKS * RS_THREADS * 4)
+      rc = cluster_sort(cluster_sort_kernel<4>, 4, sizeof(ClusterSortShared<4>));
     else
-      cluster_sort(cluster_sort_kernel<4>);
+      rc = cluster_sort(cluster_sort_kernel<8>, 8, sizeof(ClusterSortShared<8>));
+    if (rc != MUON_OK) return rc;
     if (check_cuda(cudaGetLastError(), "token sort launch")) return MUON_ERR_CUDA;
   } else {
     const unsigned tiles = static_cast<unsigned>(l.tiles);
@@ -1114,7 +1227,6 @@ int launch_embedding_grad(const void* grad, int grad_dtype, const void* ids, int
                                    counters + 1, row_count))
       return rc;
   }
-  SumArgs a{};
   a.keys = u32(l.keys[cur]);
   a.pos = u32(l.pos[cur]);
   a.n = tokens;

@@ -202,16 +202,16 @@ def _launch_gradient(index, grad, g_code, ids, i_code, num_rows, pad, scale, dty
     if as_rows:
         cap = min(tokens, num_rows)
         out = grad.new_empty((cap, dim), dtype=dtype)
-        index_out = grad.new_empty(cap + 1, dtype=torch.int64)
-        ids_ptr = index_out.data_ptr()  # (an empty view's pointer would be null: the dense form)
-        count_ptr = ids_ptr + 8 * cap
+        out_ids, count = grad.new_empty(cap, dtype=torch.int64), grad.new_empty(1, dtype=torch.int64)
+        count_ptr = count.data_ptr()
+        ids_ptr = out_ids.data_ptr() or count_ptr  # of no ids: a null pointer would ask for the dense form
     else:
         out = grad.new_empty((num_rows, dim), dtype=dtype)
         ids_ptr = count_ptr = None
     N.check(lib.muon_embedding_grad(grad.data_ptr(), g_code, ids.data_ptr(), i_code, tokens, num_rows, dim, pad, scale,
                                     out.data_ptr(), o_code, ids_ptr, count_ptr, work.data_ptr(), need,
                                     _error_word(index).pointer, raw_stream(index)), "muon_embedding_grad")
-    return RowGrad(num_rows, index_out[:cap], out, index_out[cap:]) if as_rows else out
+    return RowGrad(num_rows, out_ids, out, count) if as_rows else out
 
 
 def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, *, scale: float = 1.0,

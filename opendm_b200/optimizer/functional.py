@@ -32,7 +32,7 @@ _CODE = {torch.bfloat16: N.MUON_BF16, torch.float32: N.MUON_F32}
 # The lists are long and each call is short: what is asked of every tensor goes through map.
 _POINTER, _NUMEL, _DEVICE = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
 _CONTIGUOUS, _SIZE = torch.Tensor.is_contiguous, torch.Tensor.size
-_LAYOUT, _DTYPE = attrgetter("layout"), attrgetter("dtype")
+_DTYPE = attrgetter("dtype")
 _NORMS = {2.0: N.MUON_NORM_2, 1.0: N.MUON_NORM_1, math.inf: N.MUON_NORM_INF}
 
 
@@ -45,6 +45,8 @@ def _norm_kind(norm_type: float) -> int:
 
 def _dense_storage(t: torch.Tensor) -> bool:
     """True when the tensor's elements fill one block of memory, in any order."""
+    if t.layout is not torch.strided:
+        raise RuntimeError(f"gradients must be dense tensors, got layout {t.layout}")
     if t.is_contiguous():
         return True
     expect = 1
@@ -56,21 +58,18 @@ def _dense_storage(t: torch.Tensor) -> bool:
 
 
 def _check_grads(grads: list[torch.Tensor], what: str) -> int:
-    """Device index of the list; raises for layouts, dtypes and devices the kernels do not take."""
+    """Device index of the list; raises where a tensor is on another."""
     index = device_index(grads[0])
-    if set(map(_LAYOUT, grads)) != {torch.strided}:
-        raise RuntimeError(f"{what} must be dense tensors")
     if set(map(_DEVICE, grads)) != {index}:
         raise RuntimeError(f"{what} must be on one device")
     return index
 
 
 def _codes(grads: list[torch.Tensor]) -> list[int]:
-    dtypes = list(map(_DTYPE, grads))
-    for dtype in set(dtypes):
-        if dtype not in _CODE:
-            raise RuntimeError(f"unsupported dtype {dtype}: the kernels take bfloat16 or float32")
-    return list(map(_CODE.__getitem__, dtypes))
+    codes = list(map(_CODE.get, map(_DTYPE, grads)))
+    if None in codes:
+        raise RuntimeError(f"unsupported dtype {grads[codes.index(None)].dtype}: the kernels take bfloat16 or float32")
+    return codes
 
 
 def _table(src: list[torch.Tensor], dst: list[torch.Tensor] | None) -> array:
@@ -103,7 +102,6 @@ def _raise_nonfinite(total: torch.Tensor, norm_type: float) -> None:
                            "gradients by the non-finite norm anyway, set `error_if_nonfinite=False`")
 
 
-@torch.no_grad()
 def get_total_norm(tensors: torch.Tensor | Iterable[torch.Tensor], norm_type: float = 2.0,
                    error_if_nonfinite: bool = False, foreach: bool | None = None) -> torch.Tensor:
     """Norm of all elements of ``tensors`` together, a 0-d fp32 tensor.
@@ -113,7 +111,8 @@ def get_total_norm(tensors: torch.Tensor | Iterable[torch.Tensor], norm_type: fl
     if not tensors:
         return torch.tensor(0.0)
     index = _check_grads(tensors, "tensors")
-    tensors = [t if _dense_storage(t) else t.contiguous() for t in tensors]
+    if not all(map(_CONTIGUOUS, tensors)):
+        tensors = [t if _dense_storage(t) else t.contiguous() for t in tensors]
 
     def call():
         total = tensors[0].new_empty((), dtype=torch.float32)
@@ -168,9 +167,10 @@ def _clip(grads: list[torch.Tensor], outs: list[torch.Tensor] | None, max_norm: 
     # order of elements, else a contiguous copy is scaled and copied back.
     src, dst, back = [], [], []
     for g, o in zip(grads, outs):
+        dense, _ = _dense_storage(g), _dense_storage(o)
         if any(n > 1 and s == 0 for s, n in zip(o.stride(), o.shape)):
             raise RuntimeError("an expanded tensor cannot be clipped in place: several elements share memory")
-        if g.stride() == o.stride() and _dense_storage(g):
+        if g.stride() == o.stride() and dense:
             src.append(g)
             dst.append(o)
             continue
@@ -181,12 +181,12 @@ def _clip(grads: list[torch.Tensor], outs: list[torch.Tensor] | None, max_norm: 
             dst.append(torch.empty(o.shape, dtype=o.dtype, device=o.device))
             back.append((o, dst[-1]))
     norm = _apply(src, dst, max_norm, norm_type, total)
-    for o, d in back:
-        o.copy_(d)
+    with torch.no_grad():
+        for o, d in back:
+            o.copy_(d)
     return norm
 
 
-@torch.no_grad()
 def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *, norm_type: float = 2.0,
                out: Iterable[torch.Tensor] | None = None) -> torch.Tensor:
     """Scale ``grads`` by min(max_norm / (total + 1e-6), 1), in place or into
@@ -268,7 +268,6 @@ def clip_grads_with_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max
     _clip([g if g.layout is torch.strided else g._values() for g in grads], None, max_norm, None, total_norm)
 
 
-@torch.no_grad()
 def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor], exp_avg_sqs: list[torch.Tensor],
           steps: list[float], *, lr: float, beta1: float, beta2: float, eps: float, weight_decay: float) -> None:
     """One AdamW update of each parameter, in place with its fp32 moments

@@ -51,7 +51,8 @@ def _close(got, ref, bound):
 @pytest.mark.parametrize("wdt,odt", [(torch.bfloat16, torch.bfloat16), (torch.float32, torch.bfloat16),
                                      (torch.bfloat16, torch.float32), (torch.float32, torch.float32)])
 @pytest.mark.parametrize("n,rows,dim", [(1, 1, 1), (1, 100, 2048), (7, 5, 8), (33, 1000, 257), (1000, 77, 24),
-                                        (513, 50, 1001), (3, 40, 70000)])
+                                        (513, 50, 1001), (3, 40, 70000),
+                                        (300, 60, 36), (300, 60, 250), (90, 60, 2052)])
 def test_lookup_matches_formula(wdt, odt, n, rows, dim):
     from opendm_b200.embedding import check_errors, embedding
 
@@ -148,7 +149,8 @@ def _check_gradient(grad, ids, rows, *, scale=1.0, padding_idx=None, dtype=None)
 
 GRAD_SIZES = [(1, 1, 1), (1, 100, 8), (2, 1, 16), (31, 7, 8), (32, 1, 8), (33, 1, 24), (64, 1, 257), (65, 2, 8),
               (500, 3, 40), (512, 32003, 1024), (2048, 1, 64), (2049, 5, 8), (5000, 151936, 256), (8191, 100, 33),
-              (8193, 100, 32), (20000, 50000, 72), (70000, 262144, 8), (40000, 9, 520)]
+              (8193, 100, 32), (3000, 700, 36), (3001, 700, 250), (1500, 90, 1002), (40000, 60000, 4), (33000, 300, 2),
+              (20000, 50000, 72), (70000, 262144, 8), (40000, 9, 520)]
 
 
 @pytest.mark.parametrize("gdt,odt", [(torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32)])
