@@ -569,6 +569,15 @@ __global__ void __launch_bounds__(RS_THREADS) radix_scatter_kernel(TokenSource s
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   clear_counts(counts);
   wait_previous();
+  // this tile's first position of every digit, a thread a digit (before the keys are asked for: behind them the
+  // sort of 400000 tokens took 59 us, not 44)
+  uint32_t before = 0, total = 0;
+#pragma unroll 16
+  for (int64_t t = 0; t < tiles; ++t) {
+    const uint32_t c = hist[t * RS_BINS + threadIdx.x];
+    total += c;
+    if (t < int64_t(blockIdx.x)) before += c;
+  }
   const int64_t e0 = int64_t(blockIdx.x) * RS_TILE + warp * 32 * RS_PER + lane;
   const uint32_t mask = (1u << bits) - 1u;
   uint32_t key[RS_PER], pos[RS_PER], rank[RS_PER];
@@ -581,14 +590,6 @@ __global__ void __launch_bounds__(RS_THREADS) radix_scatter_kernel(TokenSource s
       key[i] = keys ? keys[e] : token_key(src, e, nullptr);
       if (keys) pos[i] = positions[e];
     }
-  }
-  // this tile's first position of every digit, a thread a digit
-  uint32_t before = 0, total = 0;
-#pragma unroll 16
-  for (int64_t t = 0; t < tiles; ++t) {
-    const uint32_t c = hist[t * RS_BINS + threadIdx.x];
-    total += c;
-    if (t < int64_t(blockIdx.x)) before += c;
   }
   __syncthreads();
   warp_ranks<RS_PER>(counts[warp], rank, [&](int i) { return (key[i] >> shift) & mask; });
@@ -1002,7 +1003,7 @@ __global__ void __launch_bounds__(SUM_THREADS) join_kernel(O* __restrict__ out, 
     const int64_t p0 = min(n_parts, warp * per), p1 = min(n_parts, p0 + per);
     float acc[kVec] = {};
     const float* part = a.partial + int64_t(run.chunk) * 2 * pitch + slice * kSlice + lane * kVec;
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t p = p0; p < p1; ++p) {
       float v[kVec];
       load_group<kVec>(part + (p * 2 + (p == 0 ? 1 : 0)) * pitch, v);
@@ -1033,11 +1034,14 @@ int bits_for(int64_t rows) {  // keys 0 .. rows
   return bits;
 }
 
-// Chunk length: long chunks save partial rows, short ones give more warps.
-// 16384 tokens x 8 slices (bf16): 26.3 us with 32, 26-28 with 16, 33 with 8.
-int chunk_for(int64_t tokens, int64_t slices) {
+// Chunk length: long chunks leave fewer partial rows to join, short ones give
+// more warps (counted in whole slices: a warp of a narrow row does little).
+// 16384 tokens x 2048 (bf16): 26.3 us with 32, 26-28 with 16, 33 with 8; 131072
+// x 64: 36 us with 32, 34 with 16, 42 with 8 (long runs then have 950 parts).
+int chunk_for(int64_t tokens, int64_t dim) {
+  const int least = tokens > 8192 ? 16 : 8;
   int chunk = kMaxChunk;
-  while (chunk > 8 && tokens / chunk * slices < 148 * 16) chunk /= 2;
+  while (chunk > least && tokens / chunk * dim < 148 * 16 * kSlice) chunk /= 2;
   return chunk;
 }
 
@@ -1059,7 +1063,7 @@ GradLayout grad_layout(int64_t n, int64_t dim) {
   };
   l.tiles = (n + RS_TILE - 1) / RS_TILE;
   l.slices = (dim + kSlice - 1) / kSlice;
-  l.chunk = chunk_for(n, l.slices);
+  l.chunk = chunk_for(n, dim);
   l.chunks = (n + l.chunk - 1) / l.chunk;
   for (int i = 0; i < 2; ++i) l.keys[i] = take(4 * n), l.pos[i] = take(4 * n);
   l.hist = take(n > kClusterSort ? 4 * RS_MAX_PASSES * l.tiles * RS_BINS : 0);
