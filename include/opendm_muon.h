@@ -478,6 +478,7 @@ int muon_embedding(const void* weight, int weight_dtype, int64_t rows, int64_t d
  *     the distinct ids, ascending, and their rows, *count of them; the rows
  *     past *count are written as zeros with id 0, so that (out_ids, out) is a
  *     valid coordinate list whatever *count is.
+ * With no tokens, rows or columns the ids are not read (and *count is 0).
  * workspace: muon_embedding_grad_workspace_bytes() bytes, 256-byte aligned
  * (-1 for sizes the call refuses: tokens or rows >= 2^31 - 1). One workspace
  * serves one call at a time. */

@@ -147,30 +147,27 @@ def on_device(index: int, call, *args):
 
 
 def _lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float, out_dtype: torch.dtype) -> torch.Tensor:
+    index = device_index(weight)
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _lookup(ids, weight, scale, out_dtype)
     if weight.ndim != 2:
         raise ValueError("embedding weight must be 2-D")
-    index = device_index(weight)
     if ids.get_device() != index:
         raise RuntimeError(f"ids are on {ids.device}, the weight on {weight.device}")
-    w_code, o_code = _code(_FLOAT_CODE, weight.dtype, "weight"), _code(_FLOAT_CODE, out_dtype, "output")
-    i_code = _code(_INDEX_CODE, ids.dtype, "id")
+    w_code, o_code = _FLOAT_CODE.get(weight.dtype), _FLOAT_CODE.get(out_dtype)
+    i_code = _INDEX_CODE.get(ids.dtype)
+    if w_code is None or o_code is None or i_code is None:
+        _code(_FLOAT_CODE, weight.dtype, "weight"), _code(_FLOAT_CODE, out_dtype, "output")
+        _code(_INDEX_CODE, ids.dtype, "id")
     rows, dim = weight.shape
-    if not weight.is_contiguous():
-        if dim > 1 and (weight.stride(1) != 1 or (rows > 1 and weight.stride(0) < dim)):
-            weight = weight.contiguous()
-    ld = weight.stride(0) if rows > 1 else dim
-    if ld < dim:  # rows that share memory: an expanded weight
-        weight = weight.contiguous()
-        ld = dim
-    return on_device(index, _launch_lookup, index, ids.contiguous(), i_code, weight, w_code, rows, dim, ld, scale,
-                     out_dtype, o_code)
-
-
-def _launch_lookup(index, ids, i_code, weight, w_code, rows, dim, ld, scale, out_dtype, o_code):
+    if not weight.is_contiguous() and (dim > 1 and weight.stride(1) != 1 or rows > 1 and weight.stride(0) < dim):
+        weight = weight.contiguous()  # columns apart, or rows that share memory
+    ids = ids.contiguous()
     out = weight.new_empty((*ids.shape, dim), dtype=out_dtype)
-    N.check(N.lib().muon_embedding(weight.data_ptr(), w_code, rows, dim, ld, ids.data_ptr(), i_code, ids.numel(),
-                                   scale, out.data_ptr(), o_code, _error_word(index).pointer, raw_stream(index)),
-            "muon_embedding")
+    N.check(N.lib().muon_embedding(weight.data_ptr(), w_code, rows, dim, weight.stride(0) if rows > 1 else dim,
+                                   ids.data_ptr(), i_code, ids.numel(), scale, out.data_ptr(), o_code,
+                                   _error_word(index).pointer, raw_stream(index)), "muon_embedding")
     return out
 
 

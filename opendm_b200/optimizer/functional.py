@@ -281,6 +281,10 @@ def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor],
         raise ValueError("adamw lists must have one entry per parameter")
     if not params:
         return
+    if len(set(map(_POINTER, params))) != len(params):
+        raise ValueError("adamw parameters must be distinct")
+    if min(steps) < 1:
+        raise ValueError("adamw steps count from 1")
     for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
         if isinstance(g, RowGrad):
             continue  # checked by the engine

@@ -249,6 +249,54 @@ def test_gradient_keeps_nonfinite_values_in_their_rows():
     assert torch.equal(got[fine], want[fine])  # small whole numbers: exact
 
 
+def test_padding_gradients_are_never_read():
+    """NaN and infinities in the rows of dropped tokens stay out of every sum."""
+    dev = _dev()
+    for n, rows in ((300, 40), (5000, 40), (40000, 3)):
+        ids = torch.randint(rows, (n,), device=dev, generator=_gen(n))
+        grad = torch.randn(n, 40, device=dev, generator=_gen(n + 1))
+        grad[ids == 2] = torch.tensor([math.nan, math.inf, -math.inf, 1e38], device=dev).repeat(10)
+        _check_gradient(torch.where((ids == 2)[:, None], 0.0, grad), ids, rows, padding_idx=2)
+        from opendm_b200.embedding import embedding_grad
+
+        got = embedding_grad(grad, ids, rows, padding_idx=2)
+        want = embedding_grad(torch.where((ids == 2)[:, None], 0.0, grad), ids, rows, padding_idx=2)
+        assert torch.equal(got, want) and got.isfinite().all()
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements in the weight, the output, the gradient and the dense result."""
+    from opendm_b200.embedding import RowGrad, check_errors, embedding, embedding_grad
+    from opendm_b200.optimizer import adamw
+
+    dev, big, dim = _dev(), 1_100_000, 2048
+    w = torch.zeros(big, dim, device=dev, dtype=torch.bfloat16)
+    w[-1], w[-2] = 3.0, 5.0
+    got = embedding(torch.tensor([big - 1, 0, big - 2], device=dev), w)
+    assert bool((got[0] == 3).all()) and not got[1].any() and bool((got[2] == 5).all())
+    ids = torch.arange(big, device=dev) % 50
+    out = embedding(ids, (torch.arange(50, device=dev)[:, None] + torch.zeros(dim, device=dev)).bfloat16())
+    assert torch.equal(out[:, 0].float(), ids.float()) and torch.equal(out[:, -1].float(), ids.float())
+    out.fill_(1.0)
+    sums = embedding_grad(out, ids, 50, dtype=torch.float32)
+    assert bool((sums == big / 50).all())  # whole numbers below 2^24: exact
+    del out
+    g = torch.ones(3, dim, device=dev, dtype=torch.bfloat16)
+    dense = embedding_grad(g, torch.tensor([big - 1, 7, big - 1], device=dev), big)
+    assert bool((dense[-1] == 2).all()) and bool((dense[7] == 1).all())
+    assert not dense[:7].any() and not dense[8:-1].any()
+    del dense
+    # AdamW of the same size: the last row and one without a gradient, against a small parameter's
+    m, v = torch.zeros(big, dim, device=dev), torch.full((big, dim), 1e-4, device=dev)
+    kw = dict(lr=0.02, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0)
+    small = [t[-3:].clone() for t in (w, m, v)]
+    adamw([w], [RowGrad(big, torch.tensor([big - 1], device=dev), g[:1])], [m], [v], [2], **kw)
+    adamw([small[0]], [RowGrad(3, torch.tensor([2], device=dev), g[:1])], [small[1]], [small[2]], [2], **kw)
+    for a, b in zip((w, m, v), small):
+        assert torch.equal(a[-3:], b)
+    check_errors()
+
+
 # ---------------------------------------------------------------- autograd
 @pytest.mark.parametrize("sparse", [False, True])
 def test_autograd_matches_formula_and_differences(sparse):
@@ -431,6 +479,10 @@ def test_adamw_rows_mixed_lists_clip_and_refusals():
                 {"grad": RowGrad(300, rg.ids.cpu(), rg.values, rg.count)}, {"grad": rg.to_sparse()}):
         with pytest.raises(RuntimeError):
             call(**bad)
+    with pytest.raises(ValueError, match="distinct"):
+        adamw([q, q], [rg, rg], [m, m], [v, v], [1, 1], **kw)
+    with pytest.raises(ValueError, match="count from 1"):
+        adamw([q], [rg], [m], [v], [0], **kw)
 
 
 def test_adamw_rows_ignores_ids_outside_the_parameter():
