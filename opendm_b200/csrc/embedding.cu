@@ -688,7 +688,7 @@ __global__ void __launch_bounds__(HD_THREADS) heads_kernel(const uint32_t* __res
 constexpr int SUM_THREADS = 256;
 constexpr int SUM_WARPS = SUM_THREADS / 32;
 constexpr int SUM_STAGE_BYTES = 4096;  // rows in flight of one warp
-constexpr int64_t ZERO_BYTES = 8192;         // of rows one warp of the zero part looks after
+constexpr int64_t ZERO_BYTES = 8192;   // of rows one warp of the zero part looks after
 
 // A lane's 8 of a slice's 256 columns: groups of kE, 32 kE columns apart.
 template <int kE, typename T>
@@ -828,18 +828,23 @@ __device__ __forceinline__ void copy_async_wait() {
 // rows of dY come through a ring in shared memory (4 KB a warp, filled by
 // asynchronous copies that each lane makes and reads for itself), so few
 // registers are held; single bf16 elements, too small for such copies, are
-// loaded four rows ahead instead. The blocks behind sum_blocks write the
-// zeros, 8 KB of rows a warp: with 64 KB the dense gradient of 16384 tokens
-// (151936 x 2048 bf16) took 106-124 us, not 99, and zeros laid among the other
+// loaded four rows ahead instead (in at most 40 registers: 50000 x 1001 144 us,
+// 166 with 75). 131072 x 2560 bf16 into rows: 188 us, 6.5 TB/s of DRAM traffic.
+// A small batch is bound by the issue slots and its one wave of blocks: 16384 x
+// 2048 24 us; 16 columns a lane cost it 3 us more. The blocks behind sum_blocks
+// write the zeros, 8 KB of rows a warp: with 64 KB the dense gradient of 16384
+// tokens (151936 x 2048) took 106-124 us, not 99, and zeros laid among the other
 // blocks 117.
 template <int kE, typename G, typename O>
-__global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ grad, O* __restrict__ out,
-                                                          const SumArgs a) {
+__global__ void __launch_bounds__(SUM_THREADS, kE * sizeof(G) >= 4 ? 1 : 6)
+    sum_kernel(const G* __restrict__ grad, O* __restrict__ out, const SumArgs a) {
   constexpr bool kRing = kE * sizeof(G) >= 4;
   constexpr int kStages = SUM_STAGE_BYTES / (kSlice * int(sizeof(G)));
   constexpr int kGroups = kVec / kE, kGroupBytes = kE * sizeof(G);
   static_assert(kGroupBytes <= 16, "one asynchronous copy a group");
   __shared__ __align__(16) unsigned char ring[kRing ? SUM_WARPS : 1][kRing ? SUM_STAGE_BYTES : 16];
+  __shared__ int64_t held_row[SUM_WARPS][2 * kMaxChunk];  // first element of the rows of this chunk and the next
+  __shared__ uint32_t held_key[SUM_WARPS][2 * kMaxChunk];
   allow_next();
   wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -891,23 +896,22 @@ __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ 
   }
   if (valid < len) end = valid, tail = false;
   if (begin >= end) return;
-  // where a run ends
+  // where a sum is to be written: at the end of a run, and of this warp's part of one
   const uint32_t after_a = __shfl_down_sync(0xffffffffu, key_a, 1), after_b = __shfl_down_sync(0xffffffffu, key_b, 1);
   const uint32_t ends_a =
       __ballot_sync(0xffffffffu, lane < len && key_a != (lane == len - 1 ? next_first : after_a));
   const uint32_t ends_b = __ballot_sync(0xffffffffu, lane < next && (lane == next - 1 || key_b != after_b));
+  uint64_t ends = (ends_a | uint64_t(ends_b) << len | uint64_t(1) << (end - 1)) >> begin;
+  if (lane < len) held_row[warp][lane] = pos_a * a.dim, held_key[warp][lane] = key_a;
+  if (lane < next) held_row[warp][len + lane] = pos_b * a.dim, held_key[warp][len + lane] = key_b;
+  __syncwarp();
   const int64_t col = slice * kSlice + lane * kE;
   const int64_t pitch = a.slices * kSlice;
-  float* part = a.partial + c * 2 * pitch + slice * kSlice + lane * kVec;
+  const G* first_col = grad + col;
 
   float acc[kVec] = {};
-  auto row_of = [&](int r) {
-    const uint32_t pa = __shfl_sync(0xffffffffu, pos_a, r & 31), pb = __shfl_sync(0xffffffffu, pos_b, (r - len) & 31);
-    return grad + int64_t(r < len ? pa : pb) * a.dim;
-  };
-  auto finish = [&](int r) {  // row r is added: write the sum if its run or this warp's part of it ends here
-    const bool run_ends = r < len ? (ends_a >> r) & 1u : (ends_b >> (r - len)) & 1u;
-    if (!run_ends && r + 1 < end) return;
+  auto write = [&](int r) {  // the sum that ends with row r
+    float* part = a.partial + c * 2 * pitch + slice * kSlice + lane * kVec;
     if (r < lead) {
       store_group<kVec>(part, acc);
     } else if (tail && r == end - 1) {
@@ -915,8 +919,7 @@ __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ 
     } else {
 #pragma unroll
       for (int j = 0; j < kVec; ++j) acc[j] *= a.scale;
-      const uint32_t ka = __shfl_sync(0xffffffffu, key_a, r & 31);
-      const uint32_t key = r < len ? ka : last;
+      const uint32_t key = held_key[warp][r];
       const int64_t row = a.out_ids ? int64_t(slot) : int64_t(key);
       store_cols<kE>(out + row * a.dim, slice, a.dim, acc);
       if (a.out_ids && slice == 0 && lane == 0) a.out_ids[slot] = key;
@@ -926,31 +929,36 @@ __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ 
     for (int j = 0; j < kVec; ++j) acc[j] = 0.f;
   };
   if constexpr (kRing) {
+    constexpr int kStageBytes = kSlice * int(sizeof(G));
     const unsigned char* mine = ring[warp] + lane * kGroupBytes;
     const uint32_t mine_to = smem_u32(mine);
-    auto fetch = [&](int r) {
-      const G* row = row_of(r) + col;
+    auto fetch = [&](int r, int stage) {
+      const G* row = first_col + held_row[warp][r];
 #pragma unroll
       for (int k = 0; k < kGroups; ++k)
         if (col + k * 32 * kE < a.dim)
-          copy_async<kGroupBytes>(mine_to + ((r % kStages) * kGroups + k) * 32 * kGroupBytes, row + k * 32 * kE);
+          copy_async<kGroupBytes>(mine_to + stage + k * 32 * kGroupBytes, row + k * 32 * kE);
     };
-    for (int r = begin; r < begin + kStages; ++r) {
-      if (r < end) fetch(r);
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) {
+      if (begin + i < end) fetch(begin + i, i * kStageBytes);
       copy_async_commit();
     }
+    int stage = 0;
     for (int r = begin; r < end; ++r) {
       copy_async_wait<kStages - 1>();
 #pragma unroll
       for (int k = 0; k < kGroups; ++k) {
         float v[kE];
-        load_group<kE>(reinterpret_cast<const G*>(mine + ((r % kStages) * kGroups + k) * 32 * kGroupBytes), v);
+        load_group<kE>(reinterpret_cast<const G*>(mine + stage + k * 32 * kGroupBytes), v);
 #pragma unroll
         for (int i = 0; i < kE; ++i) acc[k * kE + i] += v[i];
       }
-      if (r + kStages < end) fetch(r + kStages);
+      if (r + kStages < end) fetch(r + kStages, stage);
       copy_async_commit();
-      finish(r);
+      stage = (stage + kStageBytes) % SUM_STAGE_BYTES;
+      if (ends & 1u) write(r);
+      ends >>= 1;
     }
   } else {
     constexpr int kAhead = 4;
@@ -959,7 +967,7 @@ __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ 
 #pragma unroll
       for (int q = 0; q < kAhead; ++q) {
         if (r0 + q >= end) continue;
-        const G* row = row_of(r0 + q) + col;
+        const G* row = first_col + held_row[warp][r0 + q];
 #pragma unroll
         for (int k = 0; k < kVec; ++k) {
           float x[1] = {0.f};
@@ -972,7 +980,8 @@ __global__ void __launch_bounds__(SUM_THREADS) sum_kernel(const G* __restrict__ 
         if (r0 + q >= end) continue;
 #pragma unroll
         for (int k = 0; k < kVec; ++k) acc[k] += v[q][k];
-        finish(r0 + q);
+        if (ends & 1u) write(r0 + q);
+        ends >>= 1;
       }
     }
   }
@@ -1087,7 +1096,7 @@ int run_sum(const void* grad, void* out, const SumArgs& a, unsigned grid, cudaSt
   O* o = static_cast<O*>(out);
   if (int rc = launch_overlapped("embedding gradient sum launch", sum_kernel<kE, G, O>, grid, SUM_THREADS, stream, g, o, a))
     return rc;
-  const unsigned join_grid = static_cast<unsigned>(a.chunks * a.slices < 592 ? a.chunks * a.slices : 592);
+  const unsigned join_grid = static_cast<unsigned>(std::min<int64_t>(a.chunks * a.slices, 148 * 8));
   return launch_overlapped("embedding gradient join launch", join_kernel<kE, O>, join_grid, SUM_THREADS, stream, o, a);
 }
 
