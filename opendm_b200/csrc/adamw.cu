@@ -10,6 +10,9 @@
 //   p = p + (-step_size) * (m / (fl(sqrt(v) / bc2_sqrt) + eps))
 // The rounding sequence follows torch's CPU kernels for these ops.
 
+#include <cmath>
+#include <type_traits>
+
 #include "common.cuh"
 #include "internal.h"
 
@@ -34,13 +37,14 @@ __device__ __forceinline__ int find_adam_segment(const muon_adamw_seg* segs, int
   return lo;
 }
 
+__device__ __forceinline__ float decayed(float p, float wd_factor, bool bf16_param) {
+  return bf16_param ? bf16_round(p * wd_factor) : p * wd_factor;
+}
+
 __device__ __forceinline__ float adam_elem(float p, float g, float& m, float& v, float beta1w, float beta2,
                                            float one_minus_beta2, float eps, float wd_factor, float neg_step,
                                            float bc2_sqrt, bool bf16_param) {
-  if (wd_factor != 1.f) {
-    p = p * wd_factor;
-    if (bf16_param) p = bf16_round(p);
-  }
+  if (wd_factor != 1.f) p = decayed(p, wd_factor, bf16_param);
   m = fmaf(beta1w, g - m, m);
   v = __fadd_rn(__fmul_rn(v, beta2), __fmul_rn(__fmul_rn(one_minus_beta2, g), g));
   const float denom = __fadd_rn(__fdiv_rn(sqrtf(v), bc2_sqrt), eps);
@@ -207,7 +211,15 @@ struct AdamwRowsArgs {
   int64_t rows, dim, cap, numel;
   float beta1w, beta2, one_minus_beta2, eps, wd_factor, neg_step, bc2_sqrt;
   const float* grad_scale;
+  bool quiet;
 };
+
+// Rows that no step has touched, or none for many steps, keep zero or denormal
+// first moments, whose division is a slow one. With |m| <= 2^-90 after the
+// step, eps >= 2^-30 and a step size of at most 2^6 the update is at most
+// 2^-54: for |p| >= 2^-20 under a quarter of p's last place, so p stays as it
+// is (and for m = 0 any p does); only the moments decay, and zeros stay put.
+constexpr float kQuietMoment = 0x1p-90f, kQuietParam = 0x1p-20f;
 
 constexpr int ROWS_ITERS = 4;
 constexpr int ROWS_BLOCKS = 8;  // 64 warps an SM: the element's two divisions and root fill the issue slots
@@ -217,10 +229,12 @@ constexpr int ROWS_CHUNK = ADAM_THREADS * ADAM_VEC * ROWS_ITERS;  // 4096 elemen
 // may span rows. kGradVector: they never do, and rows of values are aligned too.
 // 151936 x 2048 bf16, 16384 tokens: 999 us (6.26 TB/s of 6.55 measured); with
 // 8192 elements a block 991, with 2048 1079, with six blocks an SM 1034. An fp32
-// 32003 x 257: 54 us with 2048 or 4096, 57 with 8192.
+// 32003 x 257: 54 us with 2048 or 4096, 57 with 8192. With zero moments in the
+// 97% of its rows no token names (the start of a run) the first takes 680 us,
+// the dense kernel, whose divisions are then slow ones, 1407.
 template <typename P, typename G, bool kVector, bool kGradVector>
-__global__ void __launch_bounds__(ADAM_THREADS, ROWS_BLOCKS) adamw_rows_kernel(P* __restrict__ param, const G* __restrict__ values,
-                                                                  const AdamwRowsArgs a) {
+__global__ void __launch_bounds__(ADAM_THREADS, ROWS_BLOCKS)
+    adamw_rows_kernel(P* __restrict__ param, const G* __restrict__ values, const AdamwRowsArgs a) {
   // slot of each of the block's rows (at most ROWS_CHUNK + 1, when dim is 1), or -1
   extern __shared__ int32_t slots[];
   const int64_t e0 = int64_t(blockIdx.x) * ROWS_CHUNK;
@@ -228,6 +242,9 @@ __global__ void __launch_bounds__(ADAM_THREADS, ROWS_BLOCKS) adamw_rows_kernel(P
   const int64_t row0 = e0 / a.dim, row1 = (e0 + len - 1) / a.dim + 1;
   const uint32_t col0 = static_cast<uint32_t>(e0 - row0 * a.dim), dim = static_cast<uint32_t>(a.dim);
   const int body = kVector ? len / ADAM_VEC * ADAM_VEC : 0;
+  // whether the block looks quiet, by one first moment a thread: the loop below that tests every group for it
+  // would cost the others registers
+  const float probe = kVector && int(threadIdx.x) * ADAM_VEC < body ? a.exp_avg[e0 + threadIdx.x * ADAM_VEC] : 0.f;
   const int n_rows = static_cast<int>(row1 - row0);
   for (int r = threadIdx.x; r < n_rows; r += ADAM_THREADS) slots[r] = -1;
   __syncthreads();
@@ -241,28 +258,55 @@ __global__ void __launch_bounds__(ADAM_THREADS, ROWS_BLOCKS) adamw_rows_kernel(P
       if (!__all_sync(0xffffffffu, mine)) break;
     }
   }
-  __syncthreads();
   const bool pbf = sizeof(P) == 2, gbf = sizeof(G) == 2;
   const float coef = a.grad_scale ? *a.grad_scale : 1.f;
+  auto clipped = [&](float g) { return a.grad_scale ? clip_grad_adam(g, coef, gbf) : g; };
+  const float unlisted = clipped(0.f);  // 0, or NaN with a NaN or infinite coefficient, as in the dense form
+  const bool mostly_quiet = __syncthreads_and(a.quiet && unlisted == 0.f && fabsf(probe) <= kQuietMoment);
   auto element = [&](int o) {  // gradient of element o of the block
     const uint32_t at = col0 + o, r = at / dim;
     const int32_t slot = slots[r];
-    return slot < 0 ? 0.f : load1(values + int64_t(slot) * a.dim + (at - r * dim));
+    return slot < 0 ? unlisted : clipped(load1(values + int64_t(slot) * a.dim + (at - r * dim)));
   };
   auto update = [&](float& p, float g, float& m, float& v) {
-    if (a.grad_scale) g = clip_grad_adam(g, coef, gbf);
     p = adam_elem(p, g, m, v, a.beta1w, a.beta2, a.one_minus_beta2, a.eps, a.wd_factor, a.neg_step, a.bc2_sqrt, pbf);
   };
-  if constexpr (kVector) {
+  auto sweep = [&](auto look_for_quiet) {
+    constexpr bool kQuiet = decltype(look_for_quiet)::value;
     for (int o = threadIdx.x * ADAM_VEC; o < body; o += ADAM_THREADS * ADAM_VEC) {
       float p[4], m[4], v[4];
       load4(param + e0 + o, p);
       load4(a.exp_avg + e0 + o, m);
       load4(a.exp_avg_sq + e0 + o, v);
-      float g[4] = {};
+      float g[4] = {unlisted, unlisted, unlisted, unlisted};
       const uint32_t at = col0 + o, r = at / dim, col = at - r * dim;
       if (kGradVector || col + 3 < dim) {
         const int32_t slot = slots[r];
+        if constexpr (kQuiet) {
+          if (slot < 0) {
+            bool quiet = true;
+            uint32_t changed = 0;
+            float np[4], nm[4], nv[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              np[i] = a.wd_factor != 1.f ? decayed(p[i], a.wd_factor, pbf) : p[i];
+              nm[i] = fmaf(a.beta1w, 0.f - m[i], m[i]);
+              nv[i] = __fmul_rn(v[i], a.beta2);
+              quiet = quiet && fabsf(nm[i]) <= kQuietMoment && v[i] >= 0.f &&
+                      (nm[i] == 0.f || fabsf(np[i]) >= kQuietParam);
+              changed |= (__float_as_uint(nm[i]) ^ __float_as_uint(m[i])) |
+                         (__float_as_uint(nv[i]) ^ __float_as_uint(v[i]));
+            }
+            if (quiet) {
+              if (changed) {
+                store4(a.exp_avg + e0 + o, nm);
+                store4(a.exp_avg_sq + e0 + o, nv);
+              }
+              if (a.wd_factor != 1.f) store4(param + e0 + o, np);
+              continue;
+            }
+          }
+        }
         if (slot >= 0) {
           const G* row = values + int64_t(slot) * a.dim + col;
           if constexpr (kGradVector) {
@@ -271,6 +315,8 @@ __global__ void __launch_bounds__(ADAM_THREADS, ROWS_BLOCKS) adamw_rows_kernel(P
 #pragma unroll
             for (int i = 0; i < 4; ++i) g[i] = load1(row + i);
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) g[i] = clipped(g[i]);
         }
       } else {
 #pragma unroll
@@ -282,6 +328,12 @@ __global__ void __launch_bounds__(ADAM_THREADS, ROWS_BLOCKS) adamw_rows_kernel(P
       store4(a.exp_avg_sq + e0 + o, v);
       store4(param + e0 + o, p);
     }
+  };
+  if constexpr (kVector) {
+    if (mostly_quiet)
+      sweep(std::true_type{});
+    else
+      sweep(std::false_type{});
   }
   for (int o = body + threadIdx.x; o < len; o += ADAM_THREADS) {
     const int64_t e = e0 + o;
@@ -342,6 +394,7 @@ int launch_adamw_rows(const muon_adamw_rows_seg* seg, double beta1, double beta2
   a.neg_step = -sg.step_size;
   a.bc2_sqrt = sg.bc2_sqrt;
   a.grad_scale = grad_scale;
+  a.quiet = eps >= 0x1p-30f && sg.bc2_sqrt > 0.f && std::fabs(sg.step_size) <= 0x1p6f;
   using bf = __nv_bfloat16;
   const bool pb = sg.param_dtype == MUON_BF16, gb = sg.grad_dtype == MUON_BF16;
   if (pb && gb) return run_adamw_rows<bf, bf>(sg, a, stream);

@@ -1094,7 +1094,8 @@ template <int kE, typename G, typename O>
 int run_sum(const void* grad, void* out, const SumArgs& a, unsigned grid, cudaStream_t stream) {
   const G* g = static_cast<const G*>(grad);
   O* o = static_cast<O*>(out);
-  if (int rc = launch_overlapped("embedding gradient sum launch", sum_kernel<kE, G, O>, grid, SUM_THREADS, stream, g, o, a))
+  if (int rc = launch_overlapped("embedding gradient sum launch", sum_kernel<kE, G, O>, grid, SUM_THREADS, stream, g, o,
+                                 a))
     return rc;
   const unsigned join_grid = static_cast<unsigned>(std::min<int64_t>(a.chunks * a.slices, 148 * 8));
   return launch_overlapped("embedding gradient join launch", join_kernel<kE, O>, join_grid, SUM_THREADS, stream, o, a);
@@ -1125,10 +1126,12 @@ int run_sum(const void* grad, void* out, SumArgs a, cudaStream_t stream) {
 int launch_embedding(const void* weight, int weight_dtype, int64_t rows, int64_t dim, int64_t ld, const void* ids,
                      int ids_dtype, int64_t tokens, float scale, void* out, int out_dtype, int* err,
                      cudaStream_t stream) {
-  if (rows < 0 || dim < 0 || tokens < 0 || ld < dim) return set_error(MUON_ERR_ARG, "negative embedding size or ld < dim");
+  if (rows < 0 || dim < 0 || tokens < 0 || ld < dim)
+    return set_error(MUON_ERR_ARG, "negative embedding size or ld < dim");
   if (!float_type(weight_dtype) || !float_type(out_dtype))
     return set_error(MUON_ERR_ARG, "embedding dtypes must be MUON_BF16 or MUON_F32");
-  if (ids_dtype != MUON_I32 && ids_dtype != MUON_I64) return set_error(MUON_ERR_ARG, "ids must be MUON_I32 or MUON_I64");
+  if (ids_dtype != MUON_I32 && ids_dtype != MUON_I64)
+    return set_error(MUON_ERR_ARG, "ids must be MUON_I32 or MUON_I64");
   if (too_large(rows, ld) || too_large(tokens, dim) || dim >= kMaxIndex)
     return set_error(MUON_ERR_ARG, "embedding too large");
   if (tokens == 0 || dim == 0) return MUON_OK;
@@ -1156,18 +1159,21 @@ int launch_embedding_grad(const void* grad, int grad_dtype, const void* ids, int
   if (need < 0) return set_error(MUON_ERR_ARG, "embedding gradient sizes out of range");
   if (!float_type(grad_dtype) || !float_type(out_dtype))
     return set_error(MUON_ERR_ARG, "embedding gradient dtypes must be MUON_BF16 or MUON_F32");
-  if (ids_dtype != MUON_I32 && ids_dtype != MUON_I64) return set_error(MUON_ERR_ARG, "ids must be MUON_I32 or MUON_I64");
+  if (ids_dtype != MUON_I32 && ids_dtype != MUON_I64)
+    return set_error(MUON_ERR_ARG, "ids must be MUON_I32 or MUON_I64");
   if (padding_idx != -1 && (padding_idx < 0 || padding_idx >= rows))
     return set_error(MUON_ERR_ARG, "padding_idx must be -1 or a row");
   if (out_ids && !count) return set_error(MUON_ERR_ARG, "the row form needs a count");
   const int64_t cap = tokens < rows ? tokens : rows;
   const int64_t out_rows = out_ids ? cap : rows;
   if (out_rows * dim > 0 && !out) return set_error(MUON_ERR_ARG, "null embedding gradient output");
-  if (tokens > 0 && (!ids || !err || (dim > 0 && !grad))) return set_error(MUON_ERR_ARG, "null embedding gradient pointer");
+  if (tokens > 0 && (!ids || !err || (dim > 0 && !grad)))
+    return set_error(MUON_ERR_ARG, "null embedding gradient pointer");
   const int64_t out_bytes = rows * dim * (out_dtype == MUON_BF16 ? 2 : 4);
   if (tokens == 0 || rows == 0 || dim == 0) {
     if (out_ids) {
-      if (check_cuda(cudaMemsetAsync(count, 0, sizeof(int64_t), stream), "embedding gradient count")) return MUON_ERR_CUDA;
+      if (check_cuda(cudaMemsetAsync(count, 0, sizeof(int64_t), stream), "embedding gradient count"))
+        return MUON_ERR_CUDA;
       if (cap > 0)
         return check_cuda(cudaMemsetAsync(out_ids, 0, sizeof(int64_t) * cap, stream), "embedding gradient ids");
       return MUON_OK;

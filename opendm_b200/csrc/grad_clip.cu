@@ -230,8 +230,8 @@ __device__ __forceinline__ double norm_groups(const void* src, int groups, doubl
 }
 
 template <int kNorm, int N, int kIters>
-__global__ void __launch_bounds__(GC_THREADS, kBlocksPerSm) list_norm_kernel(const __grid_constant__ ClipTable<N> t,
-                                                                             double* __restrict__ partials) {
+__global__ void __launch_bounds__(GC_THREADS, kBlocksPerSm)
+    list_norm_kernel(const __grid_constant__ ClipTable<N> t, double* __restrict__ partials) {
   constexpr int kChunk = kIters * GC_STEP;
   __shared__ double red[GC_THREADS / 32];
   allow_next();
@@ -323,10 +323,10 @@ __device__ __forceinline__ void scale_groups(const void* src, bool sbf, void* ds
 }
 
 template <int N, int kIters>
-__global__ void __launch_bounds__(GC_THREADS, kBlocksPerSm) list_scale_kernel(const __grid_constant__ ClipTable<N> t, int kind,
-                                                                const double* __restrict__ partials, int n_partials,
-                                                                float max_norm, float* __restrict__ total_out,
-                                                                const float* __restrict__ total_in) {
+__global__ void __launch_bounds__(GC_THREADS, kBlocksPerSm)
+    list_scale_kernel(const __grid_constant__ ClipTable<N> t, int kind, const double* __restrict__ partials,
+                      int n_partials, float max_norm, float* __restrict__ total_out,
+                      const float* __restrict__ total_in) {
   constexpr int kChunk = kIters * GC_STEP;
   __shared__ double red[GC_THREADS / 32];
   wait_previous();
@@ -413,7 +413,8 @@ int check_overlap(const muon_clip_seg* segs, int64_t n) try {
     if (segs[i].numel == 0 || segs[i].grad == segs[i].out) continue;
     const uintptr_t begin = reinterpret_cast<uintptr_t>(segs[i].grad);
     const uintptr_t end = begin + segs[i].numel * (segs[i].grad_dtype == MUON_BF16 ? 2 : 4);
-    auto after = std::lower_bound(outs.begin(), outs.end(), end, [](const Span& s, uintptr_t e) { return s.begin < e; });
+    auto after =
+        std::lower_bound(outs.begin(), outs.end(), end, [](const Span& s, uintptr_t e) { return s.begin < e; });
     if (after != outs.begin() && (after - 1)->end > begin)
       return set_error(MUON_ERR_ARG, "gradients overlap the memory they are clipped into");
   }

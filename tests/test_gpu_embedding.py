@@ -405,6 +405,40 @@ def test_other_stream_and_graph_replay():
     check_errors()
 
 
+def test_backward_captured_into_a_graph():
+    """Forward and backward of the embedding, captured once and replayed with other tokens and weights."""
+    from opendm_b200.embedding import check_errors, embedding
+
+    dev = _dev()
+    ids = _zipf(600, 300, 22)
+    coef = torch.randn(600, 24, device=dev, generator=_gen(23))
+    weight = torch.nn.Parameter(torch.randn(300, 24, device=dev, generator=_gen(24)))
+
+    def step():
+        (embedding(ids, weight, scale=3.0, padding_idx=5) * coef).sum().backward()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # warm up on the stream kind that captures; its autograd graph ends with it
+        step()
+        weight.grad = None
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for seed in (25, 26):
+        ids.copy_(_zipf(600, 300, seed))
+        coef.copy_(torch.randn(600, 24, device=dev, generator=_gen(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        use = ids != 5
+        ref = torch.zeros(300, 24, dtype=torch.float64, device=dev).index_add_(0, ids[use], coef[use].double()) * 3
+        mag = torch.zeros_like(ref).index_add_(0, ids[use], coef[use].double().abs()) * 3
+        _close(weight.grad, ref, mag * 602 * E32)
+    check_errors()
+
+
 # -------------------------------------------------------------- AdamW rows
 def _moments(shape, seed):
     dev = _dev()
@@ -436,6 +470,50 @@ def test_adamw_rows_equals_dense(rows, dim, n, pdt, gdt):
         adamw([got[0]], [rg], [got[1]], [got[2]], [7], **kw)
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("eps", [1e-8, 0.0])
+@pytest.mark.parametrize("decay", [0.0, 0.1])
+@pytest.mark.parametrize("coef", [None, 0.5, math.inf])
+@pytest.mark.parametrize("dim,dtype", [(64, torch.float32), (33, torch.float32), (64, torch.bfloat16)])
+def test_adamw_rows_with_untouched_rows(eps, decay, coef, dim, dtype):
+    """Rows whose moments are (signed) zeros, denormal or tiny, alone and beside others, bit for bit as in the
+    dense form."""
+    from opendm_b200.embedding import embedding_grad, embedding_row_grad
+    from opendm_b200.optimizer import adamw
+    from opendm_b200.optimizer.muon_adamw import _engine_for
+
+    dev = _dev()
+    p = torch.randn(3000, dim, device=dev, generator=_gen(75))
+    p[::5] = torch.tensor([0.0, -0.0, 1e-42, math.inf], device=dev).repeat(dim)[:dim]
+    m, v = _moments((3000, dim), 76)
+    m[100:2900], v[100:2900] = 0.0, 0.0
+    m[200:300], m[400:500, ::3], v[600:700, ::7] = -0.0, 1e-40, 1e-42
+    m[800:900], m[1000:1100], m[1200:1300], v[1000:1100] = 2.0 ** -90, -(2.0 ** -89), 2.0 ** -95, 1e-4
+    m[1400:1500, 1::2], v[1400:1500], v[1600:1610] = 1e-44, 1e-44, math.inf
+    v[1620:1630] = math.nan
+    p[1200:1300:2] = 2.0 ** -20
+    p[1201:1300:2] = 2.0 ** -21
+    p[1640:1650] = math.nan
+    p = p.to(dtype)
+    ids = torch.randint(3000, (400,), device=dev, generator=_gen(78))
+    g = torch.randn(400, dim, device=dev, generator=_gen(79)).to(dtype)
+    kw = dict(lr=0.02, beta1=0.9, beta2=0.95, eps=eps, weight_decay=decay)
+    engine = _engine_for(dev, "fp16")
+    engine.grad_scale = None if coef is None else torch.full((1,), coef, device=dev)
+    try:
+        results = []
+        for grad in (embedding_row_grad(g, ids, 3000), embedding_grad(g, ids, 3000)):
+            t = [x.clone() for x in (p, m, v)]
+            adamw([t[0]], [grad], [t[1]], [t[2]], [4], **kw)
+            results.append(t)
+    finally:
+        engine.grad_scale = None
+    for a, b in zip(*results):
+        nan = b.isnan()
+        assert torch.equal(a.isnan(), nan)
+        bits = torch.int32 if a.dtype == torch.float32 else torch.int16
+        assert torch.equal(a.view(bits)[~nan], b.view(bits)[~nan])  # signs of zeros too
 
 
 def test_adamw_rows_mixed_lists_clip_and_refusals():
