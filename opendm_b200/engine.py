@@ -35,7 +35,7 @@ import torch
 
 from . import _native as N
 from . import trace
-from .embedding import RowGrad
+from .embedding import RowGrad, raw_stream
 
 _DTYPE_CODE = {torch.bfloat16: N.MUON_BF16, torch.float32: N.MUON_F32}
 PRECISIONS = {"tf32": N.MUON_TF32, "fp16": N.MUON_F16, "bf16": N.MUON_BF16, "parity": N.MUON_F16X3}
@@ -212,6 +212,7 @@ class CudaMuonEngine:
         self.lib = N.lib()
         idx = self.device.index if self.device.index is not None else torch.cuda.current_device()
         N.check(self.lib.muon_device_check(idx), "muon_device_check")
+        self.index = idx
         self._plans: dict = {}  # matrix-set key -> _PlanState, least recently used first
         self._tables = _TableCache(self.device)
         self._adam_tables = _TableCache(self.device, capacity=8)  # per-step scalars rewritten in place
@@ -746,10 +747,11 @@ class CudaMuonEngine:
               weight_decay: float) -> None:
         """Fused AdamW over all items (reference muon_adamw.py:333-343); an
         item whose gradient is a RowGrad gets a launch of its own."""
-        for it in items:
-            if isinstance(it.grad, RowGrad):
+        rows = [it for it in items if isinstance(it.grad, RowGrad)]
+        if rows:
+            for it in rows:
                 self._adamw_rows(it, lr=lr, beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay)
-        items = [it for it in items if not isinstance(it.grad, RowGrad)]
+            items = [it for it in items if not isinstance(it.grad, RowGrad)]
         if not items:
             return
         segs = []
@@ -805,37 +807,34 @@ class CudaMuonEngine:
     def _adamw_rows(self, it: AdamItem, *, lr: float, beta1: float, beta2: float, eps: float,
                     weight_decay: float) -> None:
         """AdamW of one parameter whose gradient is zero outside some rows."""
-        g = it.grad
-        tensors = (it.param, it.exp_avg, it.exp_avg_sq, g.ids, g.values)
-        for t in tensors + ((g.count,) if g.count is not None else ()):
-            if t.device != self.device:
-                raise RuntimeError("AdamW tensors must be on the engine's device")
-        if not all(t.is_contiguous() for t in tensors):
+        g, p, m, v = it.grad, it.param, it.exp_avg, it.exp_avg_sq
+        ids, values, count = g.ids, g.values, g.count
+        tensors = (p, m, v, ids, values) if count is None else (p, m, v, ids, values, count)
+        if set(map(torch.Tensor.get_device, tensors)) != {self.index}:
+            raise RuntimeError("AdamW tensors must be on the engine's device")
+        if not all(map(torch.Tensor.is_contiguous, tensors)):
             raise RuntimeError("AdamW parameters, moments and row gradients must be contiguous")
-        shape = it.param.shape
-        if it.param.ndim < 2 or g.num_rows != shape[0] or g.values.shape[1:] != shape[1:]:
-            raise RuntimeError(f"row gradient of {g.num_rows} rows of {tuple(g.values.shape[1:])} does not match a "
+        shape, given = p.shape, values.shape
+        if len(shape) < 2 or g.num_rows != shape[0] or given[1:] != shape[1:]:
+            raise RuntimeError(f"row gradient of {g.num_rows} rows of {tuple(given[1:])} does not match a "
                                f"parameter of shape {tuple(shape)}")
-        if it.exp_avg.shape != shape or it.exp_avg_sq.shape != shape:
+        if m.shape != shape or v.shape != shape:
             raise RuntimeError("AdamW moments must have their parameter's shape")
-        if it.exp_avg.dtype != torch.float32 or it.exp_avg_sq.dtype != torch.float32:
+        if m.dtype != torch.float32 or v.dtype != torch.float32:
             raise RuntimeError("AdamW moments must be float32")
-        if g.ids.dtype != torch.int64 or g.ids.ndim != 1 or g.ids.numel() != g.values.shape[0]:
+        if ids.dtype != torch.int64 or ids.shape != given[:1]:
             raise RuntimeError("a row gradient needs one int64 id per row of values")
-        if g.count is not None and (g.count.dtype != torch.int64 or g.count.numel() != 1):
+        if count is not None and (count.dtype != torch.int64 or count.numel() != 1):
             raise RuntimeError("a row gradient's count is one int64 value")
-        s = N.AdamwRowsSeg()
-        s.param, s.exp_avg, s.exp_avg_sq = it.param.data_ptr(), it.exp_avg.data_ptr(), it.exp_avg_sq.data_ptr()
-        s.ids, s.values = g.ids.data_ptr(), g.values.data_ptr()
-        s.count = g.count.data_ptr() if g.count is not None else None
-        s.rows, s.dim, s.cap = shape[0], math.prod(shape[1:]), g.ids.numel()
-        s.step_size, s.bc2_sqrt = lr / (1 - beta1 ** it.step), (1 - beta2 ** it.step) ** 0.5
-        s.param_dtype, s.grad_dtype = _dtype_code(it.param), _dtype_code(g.values)
+        s = N.AdamwRowsSeg(p.data_ptr(), m.data_ptr(), v.data_ptr(), ids.data_ptr(), values.data_ptr(),
+                           None if count is None else count.data_ptr(), shape[0], math.prod(shape[1:]), given[0],
+                           lr / (1 - beta1 ** it.step), (1 - beta2 ** it.step) ** 0.5, _dtype_code(p),
+                           _dtype_code(values))
         wd_factor = 1.0 - lr * weight_decay if weight_decay != 0 else 1.0
         ev = self._event_pair("adamw")
         gs = self.grad_scale
-        N.check(self.lib.muon_adamw_rows(byref(s), float(beta1), float(beta2), c_float(eps), c_float(wd_factor),
-                                         c_void_p(gs.data_ptr() if gs is not None else None), _stream_handle()),
+        N.check(self.lib.muon_adamw_rows(byref(s), beta1, beta2, eps, wd_factor,
+                                         None if gs is None else gs.data_ptr(), raw_stream(self.index)),
                 "muon_adamw_rows")
         self._event_end(ev)
         self.kernel_launches += 1
@@ -879,6 +878,20 @@ class CudaMuonEngine:
             self.close()
         except Exception:
             pass
+
+
+_ENGINES: dict[tuple, CudaMuonEngine] = {}
+
+
+def engine_for(device: torch.device, precision: str, ns_algo: str = "auto") -> CudaMuonEngine:
+    """The process's engine of a device and these options, made on first use."""
+    if device.type != "cuda":
+        raise RuntimeError("opendm_b200 runs on CUDA (sm_100) tensors only; got a tensor on " + str(device))
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    key = (idx, precision, ns_algo)
+    if key not in _ENGINES:
+        _ENGINES[key] = CudaMuonEngine(torch.device("cuda", idx), precision, ns_algo)
+    return _ENGINES[key]
 
 
 def effective_lr(lr: float, lr_scale: float, moonlight: float, shape: tuple[int, int],

@@ -11,8 +11,8 @@ roundings.) ``adamw`` is the optimizer's fused AdamW over lists, for dense
 gradients and for row gradients (``opendm_b200.embedding.RowGrad``).
 
 All run sm_100a kernels on the current stream of the tensors' device; CPU
-tensors raise. No call reads anything back unless asked to
-(``error_if_nonfinite``), so all of them can be captured into a CUDA graph.
+tensors raise. Nothing is read back unless asked for (``error_if_nonfinite``),
+and the norm and clipping calls can be captured into a CUDA graph.
 """
 
 from __future__ import annotations
@@ -26,7 +26,7 @@ import torch
 
 from .. import _native as N
 from ..embedding import RowGrad, device_index, embedding_row_grad, on_device, raw_stream
-from ..engine import AdamItem
+from ..engine import AdamItem, engine_for
 
 _CODE = {torch.bfloat16: N.MUON_BF16, torch.float32: N.MUON_F32}
 # The lists are long and each call is short: what is asked of every tensor goes through map.
@@ -275,8 +275,6 @@ def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor],
     tensors, or RowGrads for parameters whose gradient is zero outside some
     rows: the same results at the cost of those rows. ``steps``: the step
     count of each, this step included."""
-    from .muon_adamw import _engine_for
-
     if not len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(steps):
         raise ValueError("adamw lists must have one entry per parameter")
     if not params:
@@ -292,8 +290,7 @@ def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor],
             raise RuntimeError("adamw takes a dense gradient of its parameter's shape, or a RowGrad")
         if any(t.dtype != torch.float32 or t.shape != p.shape or not t.is_contiguous() for t in (m, v)):
             raise RuntimeError("AdamW moments must be contiguous float32 tensors of their parameter's shape")
-    items = [AdamItem(*it) for it in zip(params, grads, exp_avgs, exp_avg_sqs, map(float, steps))]
+    items = list(map(AdamItem, params, grads, exp_avgs, exp_avg_sqs, map(float, steps)))
     index = device_index(params[0])
-    engine = _engine_for(params[0].device, "fp16")
-    on_device(index, lambda: engine.adamw(items, lr=float(lr), beta1=float(beta1), beta2=float(beta2),
-                                           eps=float(eps), weight_decay=float(weight_decay)))
+    on_device(index, lambda: engine_for(params[0].device, "fp16").adamw(
+        items, lr=float(lr), beta1=float(beta1), beta2=float(beta2), eps=float(eps), weight_decay=float(weight_decay)))

@@ -95,7 +95,8 @@ import torch.distributed as dist
 
 from .. import embedding as emb
 from .. import trace
-from ..engine import AdamItem, CudaMuonEngine, MatrixItem, effective_lr
+from ..engine import AdamItem, MatrixItem, effective_lr
+from ..engine import engine_for as _engine_for
 from ..sharding import FlatAdamShards, FlatParamBuckets, assign_owners, assign_waves
 from .functional import clip_grad_norm_, rows_of
 
@@ -192,19 +193,6 @@ def mark_muon_parameters(model: torch.nn.Module,
     if not selected:
         raise RuntimeError("MuonAdamW selected 0 parameters.")
     return selected
-
-
-_ENGINES: dict[tuple, CudaMuonEngine] = {}
-
-
-def _engine_for(device: torch.device, precision: str, ns_algo: str = "auto") -> CudaMuonEngine:
-    if device.type != "cuda":
-        raise RuntimeError("opendm_b200 runs on CUDA (sm_100) tensors only; got a tensor on " + str(device))
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    key = (idx, precision, ns_algo)
-    if key not in _ENGINES:
-        _ENGINES[key] = CudaMuonEngine(torch.device("cuda", idx), precision, ns_algo)
-    return _ENGINES[key]
 
 
 def zeropower_via_newtonschulz5(matrix: torch.Tensor, steps: int = 5, eps: float = 1e-7, *,
