@@ -828,8 +828,9 @@ __device__ __forceinline__ void copy_async_wait() {
 // rows of dY come through a ring in shared memory (4 KB a warp, filled by
 // asynchronous copies that each lane makes and reads for itself), so few
 // registers are held; single bf16 elements, too small for such copies, are
-// loaded four rows ahead instead (in at most 40 registers: 50000 x 1001 144 us,
-// 166 with 75). 131072 x 2560 bf16 into rows: 188 us, 6.5 TB/s of DRAM traffic.
+// loaded two rows at a time instead (six blocks an SM: 50000 x 1001 137 us, with
+// four rows 144, with five blocks 151). 131072 x 2560 bf16 into rows: 184 us,
+// 6.6 TB/s of DRAM traffic.
 // A small batch is bound by the issue slots and its one wave of blocks: 16384 x
 // 2048 24 us; 16 columns a lane cost it 3 us more. The blocks behind sum_blocks
 // write the zeros, 8 KB of rows a warp: with 64 KB the dense gradient of 16384
@@ -961,7 +962,7 @@ __global__ void __launch_bounds__(SUM_THREADS, kE * sizeof(G) >= 4 ? 1 : 6)
       ends >>= 1;
     }
   } else {
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 2;
     for (int r0 = begin; r0 < end; r0 += kAhead) {
       float v[kAhead][kVec];
 #pragma unroll
