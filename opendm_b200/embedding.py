@@ -17,7 +17,7 @@ Tensors are bfloat16 or float32, ids int64 or int32.
 
 An id outside the vocabulary does not fault: its row of the lookup is zeros,
 the gradient leaves it out, and the device's error word is set, which
-``check_errors()`` (or ``MuonAdamW.check_device_errors()``, or the next
+``check_errors()`` (or ``MuonAdamW.check_device_errors()``, or a later
 ``MuonAdamW.step()`` with ``sparse_grads=True``) turns into a ``RuntimeError``.
 """
 
@@ -270,6 +270,16 @@ class ScaledEmbedding(torch.nn.Embedding):
         super().__init__(num_embeddings, embedding_dim, padding_idx, sparse=sparse, device=device, dtype=dtype)
         self.scale = float(scale)
         self.out_dtype = out_dtype
+
+    @classmethod
+    def from_pretrained(cls, embeddings: torch.Tensor, freeze: bool = True, padding_idx: int | None = None, *,
+                        scale: float = 1.0, sparse: bool = False, out_dtype: torch.dtype | None = None):
+        """``torch.nn.Embedding.from_pretrained``: a module around ``embeddings`` itself."""
+        if embeddings.ndim != 2:
+            raise ValueError("embeddings must be 2-D")
+        module = cls(*embeddings.shape, padding_idx, scale=scale, sparse=sparse, out_dtype=out_dtype, device="meta")
+        module.weight = torch.nn.Parameter(embeddings, requires_grad=not freeze)
+        return module
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         return embedding(input, self.weight, scale=self.scale, padding_idx=self.padding_idx, sparse=self.sparse,

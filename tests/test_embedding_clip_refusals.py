@@ -169,3 +169,9 @@ def test_scaled_embedding_is_a_torch_embedding():
     ref = torch.nn.Embedding(7, 4, padding_idx=2)
     ref.load_state_dict(e.state_dict())
     assert not e.weight[2].any() and "scale=3.0" in repr(e) and e.sparse
+    table = torch.randn(6, 3)
+    f = E.ScaledEmbedding.from_pretrained(table, padding_idx=1, scale=2.0, sparse=True)
+    assert f.weight.data_ptr() == table.data_ptr() and not f.weight.requires_grad
+    assert (f.num_embeddings, f.embedding_dim, f.padding_idx, f.scale, f.sparse) == (6, 3, 1, 2.0, True)
+    with pytest.raises(ValueError, match="2-D"):
+        E.ScaledEmbedding.from_pretrained(table[0])

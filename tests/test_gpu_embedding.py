@@ -366,13 +366,15 @@ def test_autograd_accumulates_and_mixes():
 
 
 # ------------------------------------------------------- streams and graphs
-def test_other_stream_and_graph_replay():
+@pytest.mark.parametrize("n", [300, 1500, 9000, 20000, 40000])
+def test_other_stream_and_graph_replay(n):
+    """Each of the token sorts (one block, a cluster, tiles) on another stream and in two graphs at once."""
     from opendm_b200.embedding import check_errors, embedding, embedding_grad, embedding_row_grad
 
     dev = _dev()
     w = torch.randn(3000, 64, device=dev, generator=_gen(17))
-    ids = _zipf(9000, 3000, 18)
-    grad = torch.randn(9000, 64, device=dev, generator=_gen(19))
+    ids = _zipf(n, 3000, 18)
+    grad = torch.randn(n, 64, device=dev, generator=_gen(19))
     want = (embedding(ids, w), embedding_grad(grad, ids, 3000), embedding_row_grad(grad, ids, 3000))
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -386,7 +388,7 @@ def test_other_stream_and_graph_replay():
     for graph, (i, g) in zip(graphs, inputs):
         with torch.cuda.graph(graph):
             outs.append((embedding(i, w), embedding_grad(g, i, 3000), embedding_row_grad(g, i, 3000)))
-    other_ids, other_grad = _zipf(9000, 3000, 20), torch.randn(9000, 64, device=dev, generator=_gen(21))
+    other_ids, other_grad = _zipf(n, 3000, 20), torch.randn(n, 64, device=dev, generator=_gen(21))
     inputs[1][0].copy_(other_ids)
     inputs[1][1].copy_(other_grad)
     torch.cuda.synchronize()
@@ -674,6 +676,27 @@ def test_optimizer_max_grad_norm_and_coalesced_gradients():
     before = w.detach().clone()
     opt.step()
     assert torch.equal(w, before) and opt.state[w]["step"].item() == 1
+
+
+def test_optimizer_clips_other_norms_of_sparse_gradients():
+    """Norm types that are not folded into the step clip in place, sparse gradients included."""
+    from opendm_b200.optimizer import MuonAdamW, mark_muon_parameters
+
+    model = _Model(True, "torch", torch.float32)
+    mark_muon_parameters(model, predicate=lambda n, p: "layer" in n)
+    opt = MuonAdamW(model, lr=0.01, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.0, sparse_grads=True)
+    model(torch.randint(500, (4, 30), device=_dev(), generator=_gen(98))).backward()
+    dense = [(p.grad.to_dense() if p.grad.is_sparse else p.grad).double() for p in model.parameters()]
+    total = max(float(g.abs().max()) for g in dense)
+    got = opt.clip_grad_norm_(total / 4, norm_type=math.inf)
+    # merged rows add at most 120 entries in fp32, in another order than to_dense()
+    assert abs(float(got) - total) <= 120 * E32 * 4 * total
+    factor = total / 4 / (total + 1e-6)
+    for p, g in zip(model.parameters(), dense):
+        now = (p.grad.to_dense() if p.grad.is_sparse else p.grad).double()
+        assert (now - g * factor).abs().max() <= 600 * E32 * total
+    opt.step()
+    opt.check_device_errors()
 
 
 def test_optimizer_reports_a_bad_token_id():
