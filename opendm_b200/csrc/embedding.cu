@@ -268,6 +268,24 @@ __device__ __forceinline__ uint32_t token_key(const TokenSource& s, int64_t t, i
   return id == s.padding ? static_cast<uint32_t>(s.rows) : static_cast<uint32_t>(id);
 }
 
+// Most of the GPU idles while a block or a cluster sorts. In the dense form,
+// extra blocks of that kernel write zeros over the last rows of the result; the
+// sum writes those of them that have tokens and leaves the rest. 48 MB by 64
+// blocks took the gradient of 16384 tokens (151936 x 2048 bf16) from 120 to 115
+// us; by 32 blocks 126, by 128 118 (they slow the sort), with 64 or 80 MB 117-119.
+// The rows past the count of the row form gained nothing so.
+struct Fill {
+  char* from;  // 16-byte aligned
+  int64_t vectors;
+  int blocks;
+};
+
+__device__ __forceinline__ void fill_zeros(const Fill& f, int block) {
+  uint4* v = reinterpret_cast<uint4*>(f.from);
+  for (int64_t i = int64_t(block) * blockDim.x + threadIdx.x; i < f.vectors; i += int64_t(f.blocks) * blockDim.x)
+    v[i] = make_uint4(0, 0, 0, 0);
+}
+
 __device__ __forceinline__ uint32_t warp_inclusive(uint32_t x) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -367,13 +385,17 @@ __global__ void __launch_bounds__(RS_THREADS) block_sort_kernel(TokenSource src,
                                                                 uint32_t* __restrict__ chunk_base,
                                                                 uint32_t* __restrict__ tile_base,
                                                                 uint32_t* __restrict__ long_count,
-                                                                int64_t* __restrict__ row_count, int* err) {
+                                                                int64_t* __restrict__ row_count, int* err, Fill fill) {
   __shared__ uint32_t skey[RS_THREADS * kPer];
   __shared__ uint16_t spos[RS_THREADS * kPer];
   __shared__ uint16_t counts[RS_WARPS][RS_BINS];
   __shared__ uint16_t base[RS_BINS];
   __shared__ uint32_t sums[RS_WARPS];
   allow_next();
+  if (blockIdx.x > 0) {
+    fill_zeros(fill, blockIdx.x - 1);
+    return;
+  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int e0 = warp * 32 * kPer + lane;
   const uint32_t rows = static_cast<uint32_t>(src.rows), mask = (1u << bits) - 1u;
@@ -450,11 +472,15 @@ template <int kPer>
 __global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(RS_THREADS)
     cluster_sort_kernel(TokenSource src, int n, int passes, int bits, int chunk, uint32_t* __restrict__ out_keys,
                         uint32_t* __restrict__ out_pos, uint32_t* __restrict__ chunk_base,
-                        uint32_t* __restrict__ tile_base, uint32_t* __restrict__ long_count, int* err) {
+                        uint32_t* __restrict__ tile_base, uint32_t* __restrict__ long_count, int* err, Fill fill) {
   extern __shared__ __align__(16) unsigned char raw[];
   ClusterSortShared<kPer>& sh = *reinterpret_cast<ClusterSortShared<kPer>*>(raw);
   constexpr int kHeld = RS_THREADS * kPer;
   allow_next();
+  if (blockIdx.x >= CL_BLOCKS) {  // whole clusters of their own
+    fill_zeros(fill, blockIdx.x - CL_BLOCKS);
+    return;
+  }
   cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
   const unsigned block = cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -720,6 +746,7 @@ struct SumArgs {
   int64_t slices;
   int64_t sum_blocks;
   int64_t zero_rows;  // rows of a warp that writes zeros
+  int64_t filled;     // dense form: the rows from here on were filled with zeros before
   float scale;
   const uint32_t* chunk_base;
   const uint32_t* tile_base;
@@ -787,7 +814,7 @@ __device__ __forceinline__ void zero_rows(O* out, const SumArgs& a, int64_t unit
     if (from + lane < to) a.out_ids[from + lane] = 0;
     return;
   }
-  const int n = static_cast<int>(min(a.zero_rows, a.rows - r0));  // at most 32
+  const int n = static_cast<int>(min(a.zero_rows, a.filled - r0));  // at most 32
   if (n <= 0) return;
   // which of the rows have tokens, a bit each: 32 sorted keys at a time, long runs skipped by a search
   uint32_t taken = 0;
@@ -1055,6 +1082,11 @@ int chunk_for(int64_t tokens, int64_t dim) {
   return chunk;
 }
 
+constexpr int64_t FILL_BLOCK = int64_t(8) << 20, FILL_CLUSTER = int64_t(48) << 20;  // bytes beside either sort
+constexpr int64_t FILL_LEAST = int64_t(1) << 20;
+constexpr int FILL_BLOCKS = 64;  // a multiple of CL_BLOCKS
+static_assert(FILL_BLOCKS % CL_BLOCKS == 0, "whole clusters");
+
 constexpr int64_t kClusterSort = CL_BLOCKS * RS_THREADS * 8;  // tokens; more are sorted by tiles
 
 struct GradLayout {
@@ -1105,7 +1137,7 @@ int run_sum(const void* grad, void* out, const SumArgs& a, unsigned grid, cudaSt
 template <typename G, typename O>
 int run_sum(const void* grad, void* out, SumArgs a, cudaStream_t stream) {
   a.sum_blocks = (a.chunks * a.slices + SUM_WARPS - 1) / SUM_WARPS;
-  const int64_t row_bytes = a.dim * int64_t(sizeof(O)), rows = a.out_ids ? a.cap : a.rows;
+  const int64_t row_bytes = a.dim * int64_t(sizeof(O)), rows = a.out_ids ? a.cap : a.filled;
   a.zero_rows = std::clamp(ZERO_BYTES / row_bytes, int64_t(1), int64_t(32));  // a lane or a bit each
   const int64_t blocks = a.sum_blocks + (rows + a.zero_rows * SUM_WARPS - 1) / (a.zero_rows * SUM_WARPS);
   if (blocks > 0x7fffffffLL) return set_error(MUON_ERR_ARG, "embedding gradient too large");
@@ -1194,23 +1226,38 @@ int launch_embedding_grad(const void* grad, int grad_dtype, const void* ids, int
   SumArgs a{};
   a.tile = HD_TILE;
   int cur = 0;
+  a.filled = rows;
   if (tokens <= kClusterSort) {
     const int n = static_cast<int>(tokens);
+    Fill fill{};
+    if (!out_ids) {
+      const int64_t row_bytes = dim * (out_dtype == MUON_BF16 ? 2 : 4);
+      const int64_t take = std::min((n <= 4 * RS_THREADS ? FILL_BLOCK : FILL_CLUSTER) / row_bytes, rows);
+      const uintptr_t from = reinterpret_cast<uintptr_t>(out) + (rows - take) * row_bytes;
+      if (from % 16 == 0 && take * row_bytes % 16 == 0 && take * row_bytes >= FILL_LEAST) {
+        fill.from = reinterpret_cast<char*>(from);
+        fill.vectors = take * row_bytes / 16;
+        fill.blocks = FILL_BLOCKS;
+        a.filled = rows - take;
+      }
+    }
     auto cluster_sort = [&](auto kernel, int per_thread, size_t smem) {
       if (smem > 48 * 1024 &&
           check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)),
                      "cluster sort attribute"))
         return int(MUON_ERR_CUDA);
-      kernel<<<CL_BLOCKS, RS_THREADS, smem, stream>>>(src, n, passes, per, l.chunk, u32(l.keys[0]), u32(l.pos[0]),
-                                                      u32(l.chunk_base), u32(l.tile_base), counters, err);
+      kernel<<<CL_BLOCKS + fill.blocks, RS_THREADS, smem, stream>>>(src, n, passes, per, l.chunk, u32(l.keys[0]),
+                                                                    u32(l.pos[0]), u32(l.chunk_base),
+                                                                    u32(l.tile_base), counters, err, fill);
       a.tile = RS_THREADS * per_thread;
       a.raw_tiles = CL_BLOCKS;
       return int(MUON_OK);
     };
     int rc = MUON_OK;
     auto block_sort = [&](auto kernel) {
-      kernel<<<1, RS_THREADS, 0, stream>>>(src, n, passes, per, l.chunk, u32(l.keys[0]), u32(l.pos[0]),
-                                           u32(l.chunk_base), u32(l.tile_base), counters, row_count, err);
+      kernel<<<1 + fill.blocks, RS_THREADS, 0, stream>>>(src, n, passes, per, l.chunk, u32(l.keys[0]), u32(l.pos[0]),
+                                                         u32(l.chunk_base), u32(l.tile_base), counters, row_count,
+                                                         err, fill);
     };
     if (n <= RS_THREADS)
       block_sort(block_sort_kernel<1>);
