@@ -498,7 +498,8 @@ int muon_embedding_grad(const void* grad, int grad_dtype, const void* ids, int i
  * Products in fp32, joined in double in a fixed order; elements whose squares leave
  * fp32's range are summed in double, so total overflows or underflows only
  * where its own fp32 value does. `segs` is host memory, read before the call
- * returns; segments must not overlap other segments' outputs. workspace:
+ * returns; outputs must not overlap one another, other segments' gradients or
+ * total_dev. workspace:
  * muon_clip_workspace_bytes(n_segs) bytes, 16-byte aligned. total_dev: one
  * device float, written by muon_total_norm and muon_clip_grads, read by
  * muon_scale_grads (which applies the coefficient of a norm known already). */

@@ -393,9 +393,9 @@ int check_segs(const muon_clip_seg* segs, int64_t n, bool outputs) {
   return MUON_OK;
 }
 
-// Outputs must not share memory with one another or with another segment's
-// gradient: blocks read and write them in no fixed order.
-int check_overlap(const muon_clip_seg* segs, int64_t n) try {
+// Outputs must not share memory with one another, with another segment's
+// gradient or with the norm: blocks read and write them in no fixed order.
+int check_overlap(const muon_clip_seg* segs, int64_t n, const float* norm) try {
   struct Span {
     uintptr_t begin, end;
     int64_t seg;
@@ -409,15 +409,18 @@ int check_overlap(const muon_clip_seg* segs, int64_t n) try {
   std::sort(outs.begin(), outs.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
   for (size_t i = 1; i < outs.size(); ++i)
     if (outs[i].begin < outs[i - 1].end) return set_error(MUON_ERR_ARG, "clipped gradients overlap in memory");
-  for (int64_t i = 0; i < n; ++i) {
-    if (segs[i].numel == 0 || segs[i].grad == segs[i].out) continue;
-    const uintptr_t begin = reinterpret_cast<uintptr_t>(segs[i].grad);
-    const uintptr_t end = begin + segs[i].numel * (segs[i].grad_dtype == MUON_BF16 ? 2 : 4);
+  auto written = [&outs](const void* p, uintptr_t bytes) {
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(p), end = begin + bytes;
     auto after =
         std::lower_bound(outs.begin(), outs.end(), end, [](const Span& s, uintptr_t e) { return s.begin < e; });
-    if (after != outs.begin() && (after - 1)->end > begin)
+    return after != outs.begin() && (after - 1)->end > begin;
+  };
+  for (int64_t i = 0; i < n; ++i) {
+    if (segs[i].numel == 0 || segs[i].grad == segs[i].out) continue;
+    if (written(segs[i].grad, segs[i].numel * (segs[i].grad_dtype == MUON_BF16 ? 2 : 4)))
       return set_error(MUON_ERR_ARG, "gradients overlap the memory they are clipped into");
   }
+  if (written(norm, sizeof(float))) return set_error(MUON_ERR_ARG, "the norm overlaps the clipped gradients");
   return MUON_OK;
 } catch (const std::bad_alloc&) {
   return set_error(MUON_ERR_ARG, "out of host memory");
@@ -547,7 +550,7 @@ int launch_total_norm(const muon_clip_seg* segs, int64_t n_segs, int norm_kind, 
 int launch_clip_grads(const muon_clip_seg* segs, int64_t n_segs, int norm_kind, float max_norm, void* workspace,
                       float* total, cudaStream_t stream) {
   if (int rc = check_segs(segs, n_segs, true)) return rc;
-  if (int rc = check_overlap(segs, n_segs)) return rc;
+  if (int rc = check_overlap(segs, n_segs, total)) return rc;
   if (all_empty(segs, n_segs)) return launch_total_norm(segs, n_segs, norm_kind, workspace, total, stream);
   if (norm_kind < MUON_NORM_2 || norm_kind > MUON_NORM_INF) return set_error(MUON_ERR_ARG, "unknown norm kind");
   if (!total || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u))
@@ -562,7 +565,7 @@ int launch_scale_grads(const muon_clip_seg* segs, int64_t n_segs, float max_norm
                        cudaStream_t stream) {
   if (!total) return set_error(MUON_ERR_ARG, "null norm");
   if (int rc = check_segs(segs, n_segs, true)) return rc;
-  if (int rc = check_overlap(segs, n_segs)) return rc;
+  if (int rc = check_overlap(segs, n_segs, total)) return rc;
   return scale_list(segs, n_segs, 0, nullptr, 0, max_norm, nullptr, total, stream);
 }
 

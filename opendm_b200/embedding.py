@@ -115,7 +115,7 @@ def record_error_check(device: torch.device) -> None:
     if word is not None and word.event is None:
         word.host.copy_(word.word, non_blocking=True)
         word.event = torch.cuda.Event()
-        word.event.record()
+        word.event.record(torch.cuda.current_stream(device))  # of the copy, whichever device is current
 
 
 def poll_errors(device: torch.device) -> None:

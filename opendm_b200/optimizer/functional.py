@@ -258,7 +258,8 @@ def clip_grads_with_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max
                           total_norm: torch.Tensor, foreach: bool | None = None) -> None:
     """Scale the parameters' gradients in place by min(max_norm / (total_norm
     + 1e-6), 1), for a norm known already (one reduced over ranks, say).
-    ``total_norm``: a one-element fp32 tensor on the gradients' device."""
+    ``total_norm``: a one-element fp32 tensor on the gradients' device, in
+    memory of its own."""
     max_norm = _max_norm(max_norm)
     grads = _parameter_grads(parameters)
     if not grads:

@@ -175,3 +175,13 @@ def test_scaled_embedding_is_a_torch_embedding():
     assert (f.num_embeddings, f.embedding_dim, f.padding_idx, f.scale, f.sparse) == (6, 3, 1, 2.0, True)
     with pytest.raises(ValueError, match="2-D"):
         E.ScaledEmbedding.from_pretrained(table[0])
+
+
+def test_a_norm_inside_the_clipped_memory_is_refused(lib):
+    segs, n = _segs((4096, 8192, 16, N.MUON_F32, N.MUON_F32))
+    for inside in (8192, 8200, 8252):
+        total = ctypes.c_void_p(inside)
+        assert lib.muon_scale_grads(segs, n, 1.0, total, None) == N.MUON_ERR_ARG
+        assert "norm" in N.last_error()
+        assert lib.muon_clip_grads(segs, n, N.MUON_NORM_2, 1.0, P, total, None) == N.MUON_ERR_ARG
+        assert "norm" in N.last_error()

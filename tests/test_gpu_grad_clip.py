@@ -200,6 +200,18 @@ def test_known_norm_and_sparse_gradients():
     assert float(get_total_norm([q.grad, q.grad])) > float(get_total_norm([q.grad]))
 
 
+def test_known_norm_among_the_gradients_is_refused():
+    from opendm_b200.optimizer import clip_grads_with_norm_
+
+    p = torch.nn.Parameter(torch.zeros(10, device=_dev()))
+    p.grad = torch.ones(10, device=_dev())
+    with pytest.raises(RuntimeError, match="overlap"):
+        clip_grads_with_norm_([p], 1.0, p.grad[3])
+    assert torch.equal(p.grad, torch.ones_like(p.grad))
+    clip_grads_with_norm_([p], 0.5, p.grad[3].clone())
+    assert float((p.grad - 0.5).abs().max()) <= 1e-6
+
+
 def test_streams_graphs_and_repeat():
     from opendm_b200.optimizer import clip_grads
 
