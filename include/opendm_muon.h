@@ -454,6 +454,8 @@ int muon_adamw_rows(const muon_adamw_rows_seg* seg, double beta1, double beta2, 
                     const float* grad_scale_dev /* or NULL */, void* stream);
 
 /* ------------------------------- (f) token embedding and its gradient
+ * In sections (f), (g) and muon_adamw_rows a pointer that is not aligned to
+ * its elements' size is refused.
  * No counterpart in the reference's optimizer: the lookup whose gradient is
  * the largest tensor of the AdamW group (a vocabulary of 151936 rows against
  * the few thousand distinct tokens of a step), and that gradient in the form

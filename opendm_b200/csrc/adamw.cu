@@ -377,6 +377,10 @@ int launch_adamw_rows(const muon_adamw_rows_seg* seg, double beta1, double beta2
   if (sg.rows == 0 || sg.dim == 0) return MUON_OK;
   if (!sg.param || !sg.exp_avg || !sg.exp_avg_sq || (sg.cap > 0 && (!sg.ids || !sg.values)))
     return set_error(MUON_ERR_ARG, "null AdamW row pointer");
+  if (misaligned(sg.param, sg.param_dtype == MUON_BF16 ? 2 : 4) || misaligned(sg.exp_avg, 4) ||
+      misaligned(sg.exp_avg_sq, 4) || misaligned(sg.ids, 8) || misaligned(sg.count, 8) ||
+      misaligned(sg.values, sg.grad_dtype == MUON_BF16 ? 2 : 4) || misaligned(grad_scale, 4))
+    return set_error(MUON_ERR_ARG, "AdamW row pointer not aligned to its dtype");
   AdamwRowsArgs a{};
   a.exp_avg = sg.exp_avg;
   a.exp_avg_sq = sg.exp_avg_sq;

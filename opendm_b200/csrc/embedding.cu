@@ -1119,6 +1119,7 @@ GradLayout grad_layout(int64_t n, int64_t dim) {
 }
 
 bool float_type(int dtype) { return dtype == MUON_BF16 || dtype == MUON_F32; }
+unsigned bytes_of(int float_dtype) { return float_dtype == MUON_BF16 ? 2 : 4; }
 
 // elements x 4 bytes must fit an int64 with room to spare
 bool too_large(int64_t a, int64_t b) { return b > 0 && a > (int64_t(1) << 58) / b; }
@@ -1169,6 +1170,9 @@ int launch_embedding(const void* weight, int weight_dtype, int64_t rows, int64_t
     return set_error(MUON_ERR_ARG, "embedding too large");
   if (tokens == 0 || dim == 0) return MUON_OK;
   if ((rows > 0 && !weight) || !ids || !out || !err) return set_error(MUON_ERR_ARG, "null embedding pointer");
+  if (misaligned(weight, bytes_of(weight_dtype)) || misaligned(ids, ids_dtype == MUON_I64 ? 8 : 4) ||
+      misaligned(out, bytes_of(out_dtype)) || misaligned(err, 4))
+    return set_error(MUON_ERR_ARG, "embedding pointer not aligned to its dtype");
   const bool wide = ids_dtype == MUON_I64, wb = weight_dtype == MUON_BF16, ob = out_dtype == MUON_BF16;
   using bf = __nv_bfloat16;
   if (wb && ob) return run_lookup<bf, bf>(weight, rows, dim, ld, ids, wide, tokens, scale, out, err, stream);
@@ -1202,6 +1206,9 @@ int launch_embedding_grad(const void* grad, int grad_dtype, const void* ids, int
   if (out_rows * dim > 0 && !out) return set_error(MUON_ERR_ARG, "null embedding gradient output");
   if (tokens > 0 && (!ids || !err || (dim > 0 && !grad)))
     return set_error(MUON_ERR_ARG, "null embedding gradient pointer");
+  if (misaligned(grad, bytes_of(grad_dtype)) || misaligned(ids, ids_dtype == MUON_I64 ? 8 : 4) ||
+      misaligned(out, bytes_of(out_dtype)) || misaligned(out_ids, 8) || misaligned(count, 8) || misaligned(err, 4))
+    return set_error(MUON_ERR_ARG, "embedding gradient pointer not aligned to its dtype");
   const int64_t out_bytes = rows * dim * (out_dtype == MUON_BF16 ? 2 : 4);
   if (tokens == 0 || rows == 0 || dim == 0) {
     if (out_ids) {

@@ -537,8 +537,8 @@ int64_t clip_workspace_bytes(int64_t n_segs) {
 int launch_total_norm(const muon_clip_seg* segs, int64_t n_segs, int norm_kind, void* workspace, float* total,
                       cudaStream_t stream) {
   if (norm_kind < MUON_NORM_2 || norm_kind > MUON_NORM_INF) return set_error(MUON_ERR_ARG, "unknown norm kind");
-  if (!total || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u))
-    return set_error(MUON_ERR_ARG, "null norm output, or workspace missing or misaligned");
+  if (!total || misaligned(total, 4) || !workspace || misaligned(workspace, 16))
+    return set_error(MUON_ERR_ARG, "norm output or workspace missing or misaligned");
   if (int rc = check_segs(segs, n_segs, false)) return rc;
   double* partials = static_cast<double*>(workspace);
   int n = 0;
@@ -553,8 +553,8 @@ int launch_clip_grads(const muon_clip_seg* segs, int64_t n_segs, int norm_kind, 
   if (int rc = check_overlap(segs, n_segs, total)) return rc;
   if (all_empty(segs, n_segs)) return launch_total_norm(segs, n_segs, norm_kind, workspace, total, stream);
   if (norm_kind < MUON_NORM_2 || norm_kind > MUON_NORM_INF) return set_error(MUON_ERR_ARG, "unknown norm kind");
-  if (!total || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u))
-    return set_error(MUON_ERR_ARG, "null norm output, or workspace missing or misaligned");
+  if (!total || misaligned(total, 4) || !workspace || misaligned(workspace, 16))
+    return set_error(MUON_ERR_ARG, "norm output or workspace missing or misaligned");
   double* partials = static_cast<double*>(workspace);
   int n = 0;
   if (int rc = norm_list(segs, n_segs, norm_kind, partials, &n, stream)) return rc;
@@ -563,7 +563,7 @@ int launch_clip_grads(const muon_clip_seg* segs, int64_t n_segs, int norm_kind, 
 
 int launch_scale_grads(const muon_clip_seg* segs, int64_t n_segs, float max_norm, const float* total,
                        cudaStream_t stream) {
-  if (!total) return set_error(MUON_ERR_ARG, "null norm");
+  if (!total || misaligned(total, 4)) return set_error(MUON_ERR_ARG, "norm missing or misaligned");
   if (int rc = check_segs(segs, n_segs, true)) return rc;
   if (int rc = check_overlap(segs, n_segs, total)) return rc;
   return scale_list(segs, n_segs, 0, nullptr, 0, max_norm, nullptr, total, stream);

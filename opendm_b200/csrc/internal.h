@@ -12,6 +12,8 @@ namespace muon {
 
 // Records a failure for muon_last_error() and returns `code`.
 int set_error(int code, const std::string& msg);
+// Whether a pointer's elements of `bytes` would straddle their natural boundary, which faults.
+inline bool misaligned(const void* p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
 int check_cuda(cudaError_t e, const char* what);
 
 int launch_momentum(const muon_momentum_seg* segs_dev, int n_segs, int64_t total_chunks,

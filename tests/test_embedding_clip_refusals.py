@@ -185,3 +185,32 @@ def test_a_norm_inside_the_clipped_memory_is_refused(lib):
         assert "norm" in N.last_error()
         assert lib.muon_clip_grads(segs, n, N.MUON_NORM_2, 1.0, P, total, None) == N.MUON_ERR_ARG
         assert "norm" in N.last_error()
+
+
+def test_misaligned_pointers_are_refused(lib):
+    """Pointers that are no multiple of their element's size would fault in a kernel."""
+    odd, two, four = ctypes.c_void_p(4097), ctypes.c_void_p(4098), ctypes.c_void_p(4100)
+    f32 = {"wd": N.MUON_F32, "od": N.MUON_F32}
+    for bad in ({"weight": odd}, {"out": odd}, {"ids": four}, {"ids": two, "idt": N.MUON_I32}, {"err": two},
+                {"weight": two} | f32, {"out": two} | f32):
+        assert _lookup(lib, **bad) == N.MUON_ERR_ARG, bad
+        assert "aligned" in N.last_error()
+    f32 = {"gd": N.MUON_F32, "od": N.MUON_F32}
+    rows = {"out_ids": P, "count": P}
+    for bad in ({"grad": odd}, {"out": odd}, {"ids": four}, {"ids": two, "idt": N.MUON_I32}, {"err": two},
+                {"grad": two} | f32, {"out": two} | f32, rows | {"out_ids": four}, rows | {"count": four}):
+        assert _grad(lib, **bad) == N.MUON_ERR_ARG, bad
+        assert "aligned" in N.last_error()
+    segs, n = _segs((4096, 8192, 16, N.MUON_F32, N.MUON_F32))
+    assert lib.muon_scale_grads(segs, n, 1.0, two, None) == N.MUON_ERR_ARG
+    assert lib.muon_clip_grads(segs, n, N.MUON_NORM_2, 1.0, P, two, None) == N.MUON_ERR_ARG
+    assert lib.muon_total_norm(segs, n, N.MUON_NORM_2, P, two, None) == N.MUON_ERR_ARG
+    good = {"param": 4096, "exp_avg": 4096, "exp_avg_sq": 4096, "ids": 4096, "values": 4096, "count": 4096, "rows": 4,
+            "dim": 8, "cap": 2, "param_dtype": N.MUON_F32, "grad_dtype": N.MUON_F32}
+    for key, at in (("param", 4098), ("exp_avg", 4098), ("exp_avg_sq", 4098), ("ids", 4100), ("values", 4098),
+                    ("count", 4100)):
+        s = N.AdamwRowsSeg(**(good | {key: at}))
+        assert lib.muon_adamw_rows(ctypes.byref(s), 0.9, 0.95, 1e-8, 1.0, None, None) == N.MUON_ERR_ARG, key
+        assert "aligned" in N.last_error()
+    s = N.AdamwRowsSeg(**good)
+    assert lib.muon_adamw_rows(ctypes.byref(s), 0.9, 0.95, 1e-8, 1.0, two, None) == N.MUON_ERR_ARG
