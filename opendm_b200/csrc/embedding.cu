@@ -581,13 +581,11 @@ __global__ void __launch_bounds__(RS_THREADS) radix_count_kernel(TokenSource src
   hist[int64_t(blockIdx.x) * RS_BINS + threadIdx.x] = h[threadIdx.x];
 }
 
-__global__ void __launch_bounds__(RS_THREADS) radix_scatter_kernel(TokenSource src, const uint32_t* __restrict__ keys,
-                                                                   const uint32_t* __restrict__ positions, int64_t n,
-                                                                   int shift, int bits, int64_t tiles,
-                                                                   const uint32_t* __restrict__ hist,
-                                                                   uint32_t* __restrict__ next_hist,
-                                                                   uint32_t* __restrict__ out_keys,
-                                                                   uint32_t* __restrict__ out_pos) {
+__global__ void __launch_bounds__(RS_THREADS) radix_scatter_kernel(TokenSource src, const uint32_t* keys,
+                                                                   const uint32_t* positions, int64_t n, int shift,
+                                                                   int bits, int64_t tiles, const uint32_t* hist,
+                                                                   uint32_t* next_hist, uint32_t* out_keys,
+                                                                   uint32_t* out_pos) {
   __shared__ uint16_t counts[RS_WARPS][RS_BINS];
   __shared__ uint32_t base[RS_BINS];
   __shared__ uint32_t sums[RS_WARPS];
@@ -649,10 +647,9 @@ __global__ void __launch_bounds__(RS_THREADS) radix_scatter_kernel(TokenSource s
 // finish), and their number.
 constexpr int HD_THREADS = 1024;
 
-__global__ void __launch_bounds__(HD_THREADS) heads_kernel(const uint32_t* __restrict__ keys, int64_t n,
-                                                           uint32_t rows, int chunk, uint32_t* __restrict__ chunk_base,
-                                                           uint32_t* tile_base, uint32_t* ticket,
-                                                           int64_t* __restrict__ row_count) {
+__global__ void __launch_bounds__(HD_THREADS) heads_kernel(const uint32_t* keys, int64_t n, uint32_t rows, int chunk,
+                                                           uint32_t* chunk_base, uint32_t* tile_base, uint32_t* ticket,
+                                                           int64_t* row_count) {
   constexpr int kWarps = HD_THREADS / 32, kRounds = HD_TILE / HD_THREADS;
   __shared__ uint32_t warp_sum[kWarps];
   __shared__ uint32_t last;
@@ -865,7 +862,7 @@ __device__ __forceinline__ void copy_async_wait() {
 // blocks 117.
 template <int kE, typename G, typename O>
 __global__ void __launch_bounds__(SUM_THREADS, kE * sizeof(G) >= 4 ? 1 : 6)
-    sum_kernel(const G* __restrict__ grad, O* __restrict__ out, const SumArgs a) {
+    sum_kernel(const G* grad, O* out, const SumArgs a) {
   constexpr bool kRing = kE * sizeof(G) >= 4;
   constexpr int kStages = SUM_STAGE_BYTES / (kSlice * int(sizeof(G)));
   constexpr int kGroups = kVec / kE, kGroupBytes = kE * sizeof(G);
@@ -1027,7 +1024,7 @@ __global__ void __launch_bounds__(SUM_THREADS, kE * sizeof(G) >= 4 ? 1 : 6)
 // One block per (long run, slice): the run's partial rows, split evenly over
 // the warps in chunk order, then the warps' sums in order.
 template <int kE, typename O>
-__global__ void __launch_bounds__(SUM_THREADS) join_kernel(O* __restrict__ out, const SumArgs a) {
+__global__ void __launch_bounds__(SUM_THREADS) join_kernel(O* out, const SumArgs a) {
   __shared__ float red[SUM_WARPS][kSlice];
   wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

@@ -324,9 +324,8 @@ __device__ __forceinline__ void scale_groups(const void* src, bool sbf, void* ds
 
 template <int N, int kIters>
 __global__ void __launch_bounds__(GC_THREADS, kBlocksPerSm)
-    list_scale_kernel(const __grid_constant__ ClipTable<N> t, int kind, const double* __restrict__ partials,
-                      int n_partials, float max_norm, float* __restrict__ total_out,
-                      const float* __restrict__ total_in) {
+    list_scale_kernel(const __grid_constant__ ClipTable<N> t, int kind, const double* partials, int n_partials,
+                      float max_norm, float* total_out, const float* total_in) {
   constexpr int kChunk = kIters * GC_STEP;
   __shared__ double red[GC_THREADS / 32];
   wait_previous();

@@ -55,7 +55,10 @@ int launch_momentum_f16(const muon_momentum_f16_seg* segs_dev, int n_segs, int64
 
 // Launches `kernel` so that it may start while the kernel before it on the
 // stream (one of this library that calls allow_next()) drains; it has to call
-// wait_previous() before it touches memory.
+// wait_previous() before it touches memory. Its pointers are never
+// __restrict__: const ones would promise that nothing writes their memory
+// while the kernel runs, which its predecessor does until that wait, and so
+// let loads use the non-coherent path or move above it.
 template <typename... Params, typename... Args>
 int launch_overlapped(const char* what, void (*kernel)(Params...), unsigned grid, unsigned block, cudaStream_t stream,
                       Args... args) {
