@@ -353,6 +353,7 @@ __device__ __forceinline__ uint32_t scan_warps(uint16_t (*counts)[RS_BINS]) {
   return run;
 }
 
+// counts: aligned to a word, which its element type alone does not ask for
 __device__ __forceinline__ void clear_counts(uint16_t (*counts)[RS_BINS]) {
   uint32_t* words = reinterpret_cast<uint32_t*>(counts);
 #pragma unroll
@@ -387,9 +388,9 @@ __global__ void __launch_bounds__(RS_THREADS) block_sort_kernel(TokenSource src,
                                                                 uint32_t* __restrict__ long_count,
                                                                 int64_t* __restrict__ row_count, int* err, Fill fill) {
   __shared__ uint32_t skey[RS_THREADS * kPer];
-  __shared__ uint16_t spos[RS_THREADS * kPer];
-  __shared__ uint16_t counts[RS_WARPS][RS_BINS];
-  __shared__ uint16_t base[RS_BINS];
+  __shared__ __align__(16) uint16_t spos[RS_THREADS * kPer];
+  __shared__ __align__(16) uint16_t counts[RS_WARPS][RS_BINS];
+  __shared__ __align__(16) uint16_t base[RS_BINS];
   __shared__ uint32_t sums[RS_WARPS];
   allow_next();
   if (blockIdx.x > 0) {
@@ -462,7 +463,7 @@ constexpr int CL_BLOCKS = 8;
 template <int kPer>
 struct ClusterSortShared {
   uint2 recv[RS_THREADS * kPer];  // (key, position) that this block holds after a pass
-  uint16_t counts[RS_WARPS][RS_BINS];
+  __align__(16) uint16_t counts[RS_WARPS][RS_BINS];
   uint32_t totals[RS_BINS];
   uint32_t base[RS_BINS];
   uint32_t sums[RS_WARPS];
@@ -586,7 +587,7 @@ __global__ void __launch_bounds__(RS_THREADS) radix_scatter_kernel(TokenSource s
                                                                    int bits, int64_t tiles, const uint32_t* hist,
                                                                    uint32_t* next_hist, uint32_t* out_keys,
                                                                    uint32_t* out_pos) {
-  __shared__ uint16_t counts[RS_WARPS][RS_BINS];
+  __shared__ __align__(16) uint16_t counts[RS_WARPS][RS_BINS];
   __shared__ uint32_t base[RS_BINS];
   __shared__ uint32_t sums[RS_WARPS];
   allow_next();
@@ -1025,7 +1026,7 @@ __global__ void __launch_bounds__(SUM_THREADS, kE * sizeof(G) >= 4 ? 1 : 6)
 // the warps in chunk order, then the warps' sums in order.
 template <int kE, typename O>
 __global__ void __launch_bounds__(SUM_THREADS) join_kernel(O* out, const SumArgs a) {
-  __shared__ float red[SUM_WARPS][kSlice];
+  __shared__ __align__(16) float red[SUM_WARPS][kSlice];  // stored in vectors
   wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t pitch = a.slices * kSlice;

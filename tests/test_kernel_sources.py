@@ -44,3 +44,14 @@ def test_overlapped_launches_are_of_kernels_that_wait():
             assert m.group(1) in waiting, m.group(1)
             found.add(m.group(1))
     assert found == {"radix_scatter_kernel", "heads_kernel", "sum_kernel", "join_kernel", "list_scale_kernel"}
+
+
+def test_shared_arrays_of_narrow_types_state_their_alignment():
+    """Shared arrays of floats, 16-bit counts and bytes are stored and cleared in wider words, which fault where the
+    array starts between two of them; a declaration alone promises no more than its element's alignment."""
+    code = "".join(map(_code, [p for p in SOURCES if p.stem in ("embedding", "grad_clip")]))
+    declared = re.findall(r"__shared__([^;=]*?)\b(float|uint16_t|unsigned char)\s+(\w+)\[", code)
+    declared += re.findall(r"\n((?: *__align__\(16\))? *)(uint16_t)\s+(counts)\[RS_WARPS\]\[RS_BINS\];", code)
+    assert {"red", "counts", "ring", "raw"} <= {name for _, _, name in declared}
+    for qualifiers, _, name in declared:
+        assert "__align__(16)" in qualifiers, name
