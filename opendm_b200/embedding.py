@@ -105,6 +105,7 @@ def check_errors(device: torch.device | int | None = None) -> None:
             continue
         with torch.cuda.device(index):
             torch.cuda.synchronize()
+            word.event = None  # a copy queued before shows no more than the word itself
             code = c_int(0)
             N.check(N.lib().muon_read_error(word.pointer, byref(code), raw_stream(index)), "embedding")
 

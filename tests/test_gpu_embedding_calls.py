@@ -1,0 +1,52 @@
+"""GPU tests of calls around the embedding, clipping and row-gradient AdamW kernels: errors, aliases, modes."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return torch.device("cuda", 0)
+
+
+def _gen(seed):
+    return torch.Generator(device=_dev()).manual_seed(seed)
+
+
+def _model_and_optimizer(**options):
+    from opendm_b200.embedding import ScaledEmbedding
+    from opendm_b200.optimizer import MuonAdamW, mark_muon_parameters
+
+    model = torch.nn.Module()
+    model.embed = ScaledEmbedding(500, 64, sparse=True, device=_dev())
+    model.layer = torch.nn.Linear(64, 128, bias=False, device=_dev())
+    mark_muon_parameters(model, predicate=lambda n, p: "layer" in n)
+    return model, MuonAdamW(model, lr=0.01, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.0, sparse_grads=True, **options)
+
+
+def _backward(model, ids, scale=1.0):
+    (model.layer(model.embed(ids.to(_dev()))) * scale).square().mean().backward()
+
+
+def test_a_token_id_error_is_raised_once():
+    model, opt = _model_and_optimizer()
+    _backward(model, torch.tensor([1, 500, 2]))
+    opt.step()  # queues a copy of the error word
+    with pytest.raises(RuntimeError, match="token id out of range"):
+        opt.check_device_errors()
+    opt.check_device_errors()
+    for _ in range(2):  # the error was raised; these are healthy steps
+        opt.zero_grad(set_to_none=True)
+        _backward(model, torch.tensor([1, 2, 3]))
+        opt.step()
+    opt.check_device_errors()
+    _backward(model, torch.tensor([-1]))
+    opt.step()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="token id out of range"):
+        opt.clip_grad_norm_(1.0)
+    opt.step()
+    opt.check_device_errors()
