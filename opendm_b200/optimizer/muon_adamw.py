@@ -396,7 +396,8 @@ class MuonAdamW(torch.optim.Optimizer):
         with torch's arithmetic (norm type 2); the next ``step()`` scales every
         gradient by the coefficient as its kernels read it, so ``p.grad``
         keeps its unclipped values until then. Returns the total norm (a 0-d
-        tensor, bf16 when every gradient is bf16, as torch's). Other norm
+        tensor, bf16 when every gradient is bf16, as torch's); a ``step()``
+        that raises drops it, so clip again before the next. Other norm
         types, or parameters split over ranks (FSDP, whose own
         ``clip_grad_norm_`` reduces across ranks), run torch's function."""
         grads = [p.grad for g in self.param_groups for p in g["params"] if p.grad is not None]
@@ -430,14 +431,15 @@ class MuonAdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
-        if closure is not None:
-            with torch.enable_grad():
-                loss = closure()
         try:
+            if closure is not None:
+                with torch.enable_grad():
+                    loss = closure()
             self._row_grads = self._merge_row_grads()
             self._clipped_step()
         finally:
             self._row_grads = {}
+            self._pending_clip = None  # of a step that raised too: its coefficient is no other batch's
         if self.sparse_grads:
             emb.record_error_check(self._device_for_params(self.param_groups[0]["params"]))
         return loss

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from opendm_b200 import embedding as E
+from opendm_b200.optimizer import MuonAdamW, mark_muon_parameters
 
 
 class _Word:
@@ -64,3 +65,25 @@ def test_a_reported_token_id_error_is_not_raised_again(word):
         E.poll_errors(device)
     E.poll_errors(device)
     E.check_errors(0)
+
+
+def _sparse_model():
+    m = torch.nn.Module()
+    m.embed = torch.nn.Embedding(10, 4, sparse=True)
+    m.layer = torch.nn.Linear(4, 4, bias=False)
+    mark_muon_parameters(m, predicate=lambda n, p: "layer" in n)
+    return m, MuonAdamW(m, lr=1e-3, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.0, sparse_grads=True)
+
+
+@pytest.mark.parametrize("closure", [False, True])
+def test_a_step_that_raises_drops_its_clip(closure):
+    m, opt = _sparse_model()
+    opt._pending_clip = torch.tensor([2.0, 0.5])
+
+    def fail():
+        raise RuntimeError("CUDA")
+
+    m.embed(torch.tensor([1, 2])).sum().backward()
+    with pytest.raises(RuntimeError, match="CUDA"):  # in the closure, or in the merge, which has no CPU path
+        opt.step(fail) if closure else opt.step()
+    assert opt._pending_clip is None

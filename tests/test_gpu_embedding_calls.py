@@ -50,3 +50,20 @@ def test_a_token_id_error_is_raised_once():
         opt.clip_grad_norm_(1.0)
     opt.step()
     opt.check_device_errors()
+
+
+def test_the_clip_of_an_abandoned_step_is_not_used_later():
+    model, opt = _model_and_optimizer(max_grad_norm=1e-3)
+    _backward(model, torch.tensor([-1]))
+    opt.step()
+    torch.cuda.synchronize()
+    # a clip that leaves the pending coefficient behind: the late error is raised by the step
+    opt._pending_clip = torch.tensor([1.0, 0.0], device=_dev())
+    with pytest.raises(RuntimeError, match="token id out of range"):
+        opt.step()
+    opt.zero_grad(set_to_none=True)
+    _backward(model, torch.tensor([1, 2, 3]), 100.0)
+    total = sum(float(p.grad.to_dense().double().square().sum()) for p in model.parameters()) ** 0.5
+    opt.step()  # with a coefficient of 0 the norm would not be taken and the moments would stay as they were
+    assert abs(float(opt.last_grad_norm) - total) <= 1e-5 * total
+    assert bool(opt.state[model.embed.weight]["exp_avg"][1:4].any())
