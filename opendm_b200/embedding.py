@@ -27,6 +27,7 @@ from ctypes import byref, c_int
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -139,6 +140,17 @@ def _code(table: dict, dtype: torch.dtype, what: str) -> int:
     return code
 
 
+def has_tangent(tensors) -> bool:
+    """Whether one of the tensors carries a forward-mode derivative (outside of a dual level none does)."""
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def refuse_derivatives(what: str, tensors) -> None:
+    """Raise where autograd would have to follow a call that reads or writes its tensors by pointer."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors) or has_tangent(tensors):
+        raise RuntimeError(f"{what} records no derivatives: detach its tensors, or call it under torch.no_grad()")
+
+
 def on_device(index: int, call, *args):
     """Run ``call`` with the device current (the usual case costs one query)."""
     if torch.cuda.current_device() == index:
@@ -174,6 +186,8 @@ def _lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float, out_dtype: to
 
 def _gradient(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: float, padding_idx: int | None,
               dtype: torch.dtype | None, as_rows: bool):
+    if has_tangent((grad,)):
+        raise RuntimeError("the embedding's gradient has no forward-mode derivative")
     index = device_index(grad)
     if ids.get_device() != index:
         raise RuntimeError(f"ids are on {ids.device}, the gradient on {grad.device}")
@@ -216,7 +230,9 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, *, scal
                    padding_idx: int | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
     """Dense ``[num_rows, dim]`` gradient of an embedding weight from the
     gradient ``[*ids.shape, dim]`` of its lookup; ``dtype``: of the result
-    (default: the gradient's). Tokens equal to ``padding_idx`` are left out."""
+    (default: the gradient's). Tokens equal to ``padding_idx`` are left out.
+    Not differentiable: a gradient that requires grad is refused."""
+    refuse_derivatives("embedding_grad", (grad,))
     return _gradient(grad, ids, num_rows, float(scale), padding_idx, dtype, as_rows=False)
 
 
@@ -225,6 +241,7 @@ def embedding_row_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, *, 
     """``embedding_grad`` as the rows of the tokens only: min(tokens,
     num_rows) entries, the distinct ids first and zeros behind them. The host
     never waits for the number of distinct ids."""
+    refuse_derivatives("embedding_row_grad", (grad,))
     return _gradient(grad, ids, num_rows, float(scale), padding_idx, dtype, as_rows=True)
 
 
@@ -232,8 +249,16 @@ class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, ids, scale, padding_idx, sparse, out_dtype):
         ctx.save_for_backward(ids)
+        ctx.save_for_forward(ids)
         ctx.args = (weight.shape[0], scale, padding_idx, sparse, weight.dtype)
+        ctx.out_dtype = out_dtype
         return _lookup(ids, weight, scale, out_dtype)
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):  # the lookup is linear in the weight
+        ids, = ctx.saved_tensors
+        _, scale, padding_idx, sparse, _ = ctx.args
+        return embedding(ids, tangent, scale=scale, padding_idx=padding_idx, sparse=sparse, out_dtype=ctx.out_dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -249,13 +274,14 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, pa
     """``round(scale * weight[ids])`` of shape ``[*ids.shape, dim]``.
 
     The product is fp32, rounded once to ``out_dtype`` (default: the
-    weight's). Differentiable in ``weight``: the gradient is dense, or a
-    sparse COO tensor with ``sparse=True``; ``padding_idx`` gets none."""
+    weight's). Differentiable in ``weight``, once in reverse mode and in
+    forward mode: the gradient is dense, or a sparse COO tensor with
+    ``sparse=True``; ``padding_idx`` gets none."""
     scale = float(scale)
     out_dtype = out_dtype or weight.dtype
     if padding_idx is not None and not 0 <= int(padding_idx) < weight.shape[0]:
         raise ValueError(f"padding_idx {padding_idx} is not one of {weight.shape[0]} rows")
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if torch.is_grad_enabled() and weight.requires_grad or has_tangent((weight,)):
         return _EmbeddingFn.apply(weight, ids, scale, padding_idx, bool(sparse), out_dtype)
     return _lookup(ids, weight, scale, out_dtype)
 

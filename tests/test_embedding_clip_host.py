@@ -5,6 +5,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad as fw
 
 from opendm_b200 import embedding as E
 from opendm_b200.optimizer import MuonAdamW, mark_muon_parameters
@@ -87,3 +88,40 @@ def test_a_step_that_raises_drops_its_clip(closure):
     with pytest.raises(RuntimeError, match="CUDA"):  # in the closure, or in the merge, which has no CPU path
         opt.step(fail) if closure else opt.step()
     assert opt._pending_clip is None
+
+
+def _formula(ids, weight, scale, out_dtype):
+    with torch.no_grad():
+        return (weight.detach()[ids].float() * scale).to(out_dtype)
+
+
+def test_the_lookup_has_a_forward_mode_derivative(monkeypatch):
+    monkeypatch.setattr(E, "_lookup", _formula)
+    w, t = torch.randn(7, 3), torch.randn(7, 3)
+    ids = torch.tensor([[1, 6], [1, 0]])
+    for requires in (False, True):
+        w.requires_grad_(requires)
+        with fw.dual_level():
+            primal, tangent = fw.unpack_dual(E.embedding(ids, fw.make_dual(w, t), scale=2.0, padding_idx=1))
+            assert torch.equal(primal, w[ids] * 2) and torch.equal(tangent, t[ids] * 2)
+            assert fw.unpack_dual(E.embedding(ids, w)).tangent is None
+    # a tangent that requires grad keeps its graph
+    t.requires_grad_()
+    with fw.dual_level():
+        tangent = fw.unpack_dual(E.embedding(ids, fw.make_dual(w.detach(), t))).tangent
+        assert tangent.requires_grad
+        with torch.no_grad():
+            assert torch.equal(fw.unpack_dual(E.embedding(ids, fw.make_dual(w.detach(), t.detach()))).tangent, t[ids])
+
+
+def test_gradients_record_no_derivatives():
+    g, ids = torch.zeros(3, 8, requires_grad=True), torch.zeros(3, dtype=torch.long)
+    for call in (E.embedding_grad, E.embedding_row_grad):
+        with pytest.raises(RuntimeError, match="no derivatives"):
+            call(g, ids, 4)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):  # gets as far as the device check
+            call(g, ids, 4)
+        with fw.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match="no derivatives"):
+            call(fw.make_dual(g.detach(), torch.ones(3, 8)), ids, 4)
+    with fw.dual_level(), pytest.raises(RuntimeError, match="no forward-mode"):  # as a backward pass asks for it
+        E._gradient(fw.make_dual(g.detach(), torch.ones(3, 8)), ids, 4, 1.0, None, None, as_rows=False)

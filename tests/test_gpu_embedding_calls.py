@@ -67,3 +67,50 @@ def test_the_clip_of_an_abandoned_step_is_not_used_later():
     opt.step()  # with a coefficient of 0 the norm would not be taken and the moments would stay as they were
     assert abs(float(opt.last_grad_norm) - total) <= 1e-5 * total
     assert bool(opt.state[model.embed.weight]["exp_avg"][1:4].any())
+
+
+@pytest.mark.parametrize("sparse", [False, True])
+def test_forward_mode_of_the_lookup(sparse):
+    from torch.autograd import forward_ad as fw
+
+    from opendm_b200.embedding import ScaledEmbedding, embedding
+
+    w = torch.randn(20, 12, device=_dev(), generator=_gen(1))
+    t = torch.randn(20, 12, device=_dev(), generator=_gen(2))
+    ids = torch.randint(20, (4, 9), device=_dev(), generator=_gen(3))
+    for weight in (w, w.clone().requires_grad_()):
+        with fw.dual_level():
+            out = embedding(ids, fw.make_dual(weight, t), scale=0.5, padding_idx=3, sparse=sparse)
+            primal, tangent = fw.unpack_dual(out)
+            assert torch.equal(primal, w[ids] * 0.5) and torch.equal(tangent, t[ids] * 0.5)
+    # as torch's own module has it, the padding row's tangent included
+    mod = ScaledEmbedding.from_pretrained(w, padding_idx=3, sparse=sparse)
+    ref = torch.nn.Embedding.from_pretrained(w, padding_idx=3)
+    with fw.dual_level():
+        tangents = []
+        for m in (mod, ref):
+            out = torch.func.functional_call(m, {"weight": fw.make_dual(w, t)}, (ids,))
+            tangents.append(fw.unpack_dual(out).tangent)
+        assert torch.equal(*tangents)
+    # the derivative of a gradient along a tangent is refused, not dropped
+    p = w.clone().requires_grad_()
+    with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        loss = embedding(ids, fw.make_dual(p, t), sparse=sparse).square().sum()
+        torch.autograd.grad(loss, p)
+    # function transforms are refused
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: embedding(ids, x), (w,), (t,))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda x: embedding(ids, x).sum())(w)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda x: embedding(ids, x))(w[None])
+
+
+def test_second_derivatives_are_refused():
+    from opendm_b200.embedding import embedding
+
+    p = torch.randn(20, 12, device=_dev(), generator=_gen(1), requires_grad=True)
+    ids = torch.randint(20, (9,), device=_dev(), generator=_gen(3))
+    g, = torch.autograd.grad(embedding(ids, p).square().sum(), p, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
