@@ -12,7 +12,9 @@ gradients and for row gradients (``opendm_b200.embedding.RowGrad``).
 
 All run sm_100a kernels on the current stream of the tensors' device; CPU
 tensors raise. Nothing is read back unless asked for (``error_if_nonfinite``),
-and the norm and clipping calls can be captured into a CUDA graph.
+and the norm and clipping calls can be captured into a CUDA graph. What a call
+writes counts as changed in place for autograd: a backward pass that saved the
+old values raises.
 """
 
 from __future__ import annotations
@@ -23,6 +25,7 @@ from collections.abc import Iterable
 from operator import attrgetter, or_
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .. import _native as N
 from ..embedding import RowGrad, device_index, embedding_row_grad, on_device, raw_stream
@@ -162,7 +165,9 @@ def _clip(grads: list[torch.Tensor], outs: list[torch.Tensor] | None, max_norm: 
     if outs is None:
         outs = grads
     if all(map(_CONTIGUOUS, grads)) and (outs is grads or all(map(_CONTIGUOUS, outs))):
-        return _apply(grads, outs, max_norm, norm_type, total)
+        norm = _apply(grads, outs, max_norm, norm_type, total)
+        increment_version(outs)  # autograd has to see what was written by pointer
+        return norm
     # Other strides: elementwise work needs only that both sides agree on the
     # order of elements, else a contiguous copy is scaled and copied back.
     src, dst, back = [], [], []
@@ -184,6 +189,7 @@ def _clip(grads: list[torch.Tensor], outs: list[torch.Tensor] | None, max_norm: 
     with torch.no_grad():
         for o, d in back:
             o.copy_(d)
+    increment_version(outs)
     return norm
 
 
@@ -295,3 +301,4 @@ def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor],
     index = device_index(params[0])
     on_device(index, lambda: engine_for(params[0].device, "fp16").adamw(
         items, lr=float(lr), beta1=float(beta1), beta2=float(beta2), eps=float(eps), weight_decay=float(weight_decay)))
+    increment_version([*params, *exp_avgs, *exp_avg_sqs])

@@ -8,6 +8,8 @@ import torch
 from torch.autograd import forward_ad as fw
 
 from opendm_b200 import embedding as E
+from opendm_b200 import optimizer as O
+from opendm_b200.optimizer import functional
 from opendm_b200.optimizer import MuonAdamW, mark_muon_parameters
 
 
@@ -125,3 +127,43 @@ def test_gradients_record_no_derivatives():
             call(fw.make_dual(g.detach(), torch.ones(3, 8)), ids, 4)
     with fw.dual_level(), pytest.raises(RuntimeError, match="no forward-mode"):  # as a backward pass asks for it
         E._gradient(fw.make_dual(g.detach(), torch.ones(3, 8)), ids, 4, 1.0, None, None, as_rows=False)
+
+
+def test_writes_by_pointer_bump_version_counters(monkeypatch):
+    monkeypatch.setattr(functional, "_apply", lambda grads, *_: torch.tensor(1.0))
+    a, b, out = torch.ones(3, 4), torch.ones(4, 6)[:, ::2], torch.ones(3, 4)
+    O.clip_grads([a, b], 1.0)
+    assert a._version == 1 and b._version >= 1 and b._base._version == b._version
+    O.clip_grads([a], 1.0, out=[out])
+    assert a._version == 1 and out._version == 1
+    p = torch.nn.Parameter(torch.ones(3, 4))
+    p.grad = a
+    O.clip_grad_norm_([p], 1.0)
+    O.clip_grads_with_norm_(p, 1.0, torch.tensor(2.0))
+    assert a._version == 3 and p._version == 0
+    p.grad = torch.sparse_coo_tensor([[0, 2]], torch.ones(2, 4), (3, 4))
+    O.clip_grads_with_norm_(p, 1.0, torch.tensor(2.0))
+    assert p.grad._version == 1
+    x = torch.ones(3, requires_grad=True)
+    g, = torch.autograd.grad((x ** 3).sum(), x, create_graph=True)
+    y = (g ** 2).sum()
+    with torch.no_grad():
+        O.clip_grads([g], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_adamw_bumps_version_counters(monkeypatch):
+    class Engine:
+        def adamw(self, items, **_):
+            pass
+
+    monkeypatch.setattr(functional, "device_index", lambda t: 0)
+    monkeypatch.setattr(functional, "on_device", lambda index, call: call())
+    monkeypatch.setattr(functional, "engine_for", lambda *_: Engine())
+    p, g, m, v = torch.nn.Parameter(torch.ones(3)), torch.ones(3), torch.zeros(3), torch.zeros(3)
+    y = (p ** 2).sum()
+    O.adamw([p], [g], [m], [v], [1], lr=0.1, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0)
+    assert [t._version for t in (p, g, m, v)] == [1, 0, 1, 1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()

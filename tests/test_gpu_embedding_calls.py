@@ -114,3 +114,32 @@ def test_second_derivatives_are_refused():
     g, = torch.autograd.grad(embedding(ids, p).square().sum(), p, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.sum().backward()
+
+
+def test_autograd_sees_what_clipping_and_adamw_write():
+    from opendm_b200.optimizer import adamw, clip_grads
+
+    x = torch.ones(300, device=_dev(), requires_grad=True)
+    g, = torch.autograd.grad((x ** 3).sum(), x, create_graph=True)
+    y = (g ** 2).sum()
+    with torch.no_grad():
+        clip_grads([g], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    y = (x ** 2).sum()
+    m, v = torch.zeros(300, device=_dev()), torch.zeros(300, device=_dev())
+    adamw([x], [torch.ones(300, device=_dev())], [m], [v], [1], lr=0.1, beta1=0.9, beta2=0.95, eps=1e-8,
+          weight_decay=0.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    # a loop of forward, backward, clip and update stays as it is; so do inference tensors
+    w = torch.nn.Parameter(torch.ones(8, 8, device=_dev()))
+    m, v = torch.zeros_like(w), torch.zeros_like(w)
+    for step in (1, 2):
+        w.grad = None
+        (w @ w).sum().backward()
+        clip_grads([w.grad], 1.0)
+        adamw([w], [w.grad], [m], [v], [step], lr=0.1, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0)
+    with torch.inference_mode():
+        t = torch.full((4,), 2.0, device=_dev())
+        assert float(clip_grads([t], 1.0)) == 4.0 and float((t - 0.5).abs().max()) <= 1e-6
