@@ -25,6 +25,7 @@ from __future__ import annotations
 
 from ctypes import byref, c_int
 from dataclasses import dataclass
+from operator import attrgetter
 
 import torch
 from torch.autograd import forward_ad
@@ -32,6 +33,7 @@ from torch.autograd import forward_ad
 from . import _native as N
 
 _FLOAT_CODE = {torch.bfloat16: N.MUON_BF16, torch.float32: N.MUON_F32}
+_REQUIRES_GRAD = attrgetter("requires_grad")
 _INDEX_CODE = {torch.int32: N.MUON_I32, torch.int64: N.MUON_I64}
 
 
@@ -147,7 +149,7 @@ def has_tangent(tensors) -> bool:
 
 def refuse_derivatives(what: str, tensors) -> None:
     """Raise where autograd would have to follow a call that reads or writes its tensors by pointer."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors) or has_tangent(tensors):
+    if torch.is_grad_enabled() and any(map(_REQUIRES_GRAD, tensors)) or has_tangent(tensors):
         raise RuntimeError(f"{what} records no derivatives: detach its tensors, or call it under torch.no_grad()")
 
 

@@ -22,13 +22,15 @@ from __future__ import annotations
 import math
 from array import array
 from collections.abc import Iterable
+from itertools import chain
 from operator import attrgetter, or_
 
 import torch
 from torch.autograd.graph import increment_version
 
 from .. import _native as N
-from ..embedding import RowGrad, device_index, embedding_row_grad, on_device, raw_stream
+from ..embedding import (RowGrad, device_index, embedding_row_grad, has_tangent, on_device, raw_stream,
+                         refuse_derivatives)
 from ..engine import AdamItem, engine_for
 
 _CODE = {torch.bfloat16: N.MUON_BF16, torch.float32: N.MUON_F32}
@@ -111,6 +113,8 @@ def get_total_norm(tensors: torch.Tensor | Iterable[torch.Tensor], norm_type: fl
     ``foreach`` is accepted for torch's signature and changes nothing."""
     kind = _norm_kind(norm_type)
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if has_tangent(tensors):
+        raise RuntimeError("the norm of a list has no forward-mode derivative")
     if not tensors:
         return torch.tensor(0.0)
     index = _check_grads(tensors, "tensors")
@@ -164,6 +168,9 @@ def _clip(grads: list[torch.Tensor], outs: list[torch.Tensor] | None, max_norm: 
           total: torch.Tensor | None) -> torch.Tensor:
     if outs is None:
         outs = grads
+    else:
+        refuse_derivatives("gradient clipping", outs)
+    refuse_derivatives("gradient clipping", grads)
     if all(map(_CONTIGUOUS, grads)) and (outs is grads or all(map(_CONTIGUOUS, outs))):
         norm = _apply(grads, outs, max_norm, norm_type, total)
         increment_version(outs)  # autograd has to see what was written by pointer
@@ -198,7 +205,8 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *, norm_type: flo
     """Scale ``grads`` by min(max_norm / (total + 1e-6), 1), in place or into
     ``out`` (same shapes, bfloat16 or float32 each), and return the total
     norm of ``grads``, a 0-d fp32 tensor. In place, a tensor that appears
-    twice counts and is scaled once."""
+    twice counts and is scaled once. Nothing is recorded for autograd:
+    tensors that require grad are refused outside of ``torch.no_grad()``."""
     max_norm = _max_norm(max_norm)
     _norm_kind(norm_type)
     grads = list(grads)
@@ -290,6 +298,9 @@ def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor],
         raise ValueError("adamw parameters must be distinct")
     if min(steps) < 1:
         raise ValueError("adamw steps count from 1")
+    values = (g.values if isinstance(g, RowGrad) else g for g in grads)
+    if has_tangent(t for t in chain(params, values, exp_avgs, exp_avg_sqs) if isinstance(t, torch.Tensor)):
+        raise RuntimeError("adamw has no forward-mode derivative")
     for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
         if isinstance(g, RowGrad):
             continue  # checked by the engine

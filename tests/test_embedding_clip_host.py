@@ -167,3 +167,27 @@ def test_adamw_bumps_version_counters(monkeypatch):
     assert [t._version for t in (p, g, m, v)] == [1, 0, 1, 1]
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_clipping_refuses_derivatives(monkeypatch):
+    monkeypatch.setattr(functional, "_apply", lambda grads, *_: torch.tensor(1.0))
+    g, r, out = torch.ones(3), torch.ones(3, requires_grad=True), torch.ones(3)
+    for grads, outs in (([g, r], None), ([r], [out]), ([g], [r]), ([r * 2], None)):
+        with pytest.raises(RuntimeError, match="no derivatives"):
+            O.clip_grads(grads, 1.0, out=outs)
+        with torch.no_grad():
+            O.clip_grads(grads, 1.0, out=outs)
+    p = torch.nn.Parameter(torch.ones(3))
+    p.grad = r * 2  # as backward(create_graph=True) leaves it: torch clips it too
+    O.clip_grad_norm_(p, 1.0)
+    with fw.dual_level():
+        dual = fw.make_dual(torch.ones(3), torch.ones(3))
+        O.clip_grads([g], 1.0)
+        for call in (lambda: O.clip_grads([g, dual], 1.0), lambda: O.clip_grads([g], 1.0, out=[dual]),
+                     lambda: O.get_total_norm([g, dual]),
+                     lambda: O.adamw([dual], [g], [g], [g], [1], lr=0.1, beta1=0.9, beta2=0.95, eps=1e-8,
+                                     weight_decay=0.0),
+                     lambda: O.adamw([p], [E.RowGrad(3, g, dual)], [g], [g], [1], lr=0.1, beta1=0.9, beta2=0.95,
+                                     eps=1e-8, weight_decay=0.0)):
+            with pytest.raises(RuntimeError, match="derivative"):
+                call()
