@@ -28,6 +28,7 @@ the tensors are not on an sm_100 device.
 from __future__ import annotations
 
 import math
+import threading
 from ctypes import byref, c_float, c_int, c_void_p, sizeof
 from dataclasses import dataclass
 
@@ -97,16 +98,18 @@ class _TableCache:
     def __init__(self, device: torch.device, capacity: int = 64):
         self.device, self.capacity = device, capacity
         self._tables: dict[bytes, torch.Tensor] = {}
+        self._lock = threading.Lock()
 
     def get(self, raw: bytes, key: bytes | None = None) -> torch.Tensor:
         """The device copy of `raw`, cached under `key` (default: `raw`)."""
         key = raw if key is None else key
-        t = self._tables.pop(key, None)
-        if t is None:
-            t = _upload(raw, self.device)
-            while len(self._tables) >= self.capacity:
-                self._tables.pop(next(iter(self._tables)))
-        self._tables[key] = t  # most recently used last
+        with self._lock:
+            t = self._tables.pop(key, None)
+            if t is None:
+                t = _upload(raw, self.device)
+                while len(self._tables) >= self.capacity:
+                    self._tables.pop(next(iter(self._tables)))
+            self._tables[key] = t  # most recently used last
         t.record_stream(torch.cuda.current_stream(self.device))  # reused later by kernels on this stream
         return t
 
@@ -223,13 +226,23 @@ class CudaMuonEngine:
         self._err_host = torch.zeros(1, dtype=torch.int32).pin_memory()
         self._err_event = None
         self.kernel_launches = 0  # launches issued by this engine (for benchmarks)
-        # Device float (or None): gradient-norm clipping coefficient that the
-        # momentum and AdamW kernels apply to every gradient they read.
-        self.grad_scale: torch.Tensor | None = None
+        self._local = threading.local()  # grad_scale
         self.ns_launches_per_run = 0  # Newton-Schulz launches of the last plan run
         # When a list, (name, start, end) CUDA events are appended around the
         # momentum, Newton-Schulz and AdamW launches (benchmark instrumentation).
         self.profile_events: list | None = None
+
+    @property
+    def grad_scale(self) -> torch.Tensor | None:
+        """Device float (or None): gradient-norm clipping coefficient that the
+        momentum and AdamW kernels apply to every gradient they read. Of the
+        calling thread: optimizers and ``adamw`` calls of other threads share
+        the engine, not the coefficient of a step under way."""
+        return getattr(self._local, "grad_scale", None)
+
+    @grad_scale.setter
+    def grad_scale(self, value: torch.Tensor | None) -> None:
+        self._local.grad_scale = value
 
     def _event_pair(self, name: str):
         """Start a phase: an NVTX range always, and a pair of CUDA events when

@@ -2,6 +2,7 @@
 
 import contextlib
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -9,6 +10,7 @@ from torch.autograd import forward_ad as fw
 
 from opendm_b200 import embedding as E
 from opendm_b200 import optimizer as O
+from opendm_b200.engine import CudaMuonEngine
 from opendm_b200.optimizer import functional
 from opendm_b200.optimizer import MuonAdamW, mark_muon_parameters
 
@@ -191,3 +193,14 @@ def test_clipping_refuses_derivatives(monkeypatch):
                                      eps=1e-8, weight_decay=0.0)):
             with pytest.raises(RuntimeError, match="derivative"):
                 call()
+
+
+def test_a_step_keeps_its_clip_coefficient_to_its_thread():
+    engine = object.__new__(CudaMuonEngine)
+    engine._local = threading.local()
+    seen = []
+    engine.grad_scale = 0.5
+    other = threading.Thread(target=lambda: seen.append(engine.grad_scale))
+    other.start()
+    other.join()
+    assert seen == [None] and engine.grad_scale == 0.5

@@ -143,3 +143,34 @@ def test_autograd_sees_what_clipping_and_adamw_write():
     with torch.inference_mode():
         t = torch.full((4,), 2.0, device=_dev())
         assert float(clip_grads([t], 1.0)) == 4.0 and float((t - 0.5).abs().max()) <= 1e-6
+
+
+def test_adamw_beside_a_clipped_step_of_another_thread():
+    """The engine is shared by the process; the coefficient of one thread's step is not another's."""
+    import threading
+
+    from opendm_b200.engine import engine_for
+    from opendm_b200.optimizer import adamw
+
+    dev = _dev()
+    kw = dict(lr=0.02, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0)
+    g = torch.randn(64, 8, device=dev, generator=_gen(1))
+    results = []
+
+    def update():
+        p, m, v = (torch.zeros(64, 8, device=dev) for _ in range(3))
+        adamw([p], [g], [m], [v], [1], **kw)
+        results.append((p, m, v))
+
+    update()
+    engine = engine_for(dev, "fp16")
+    engine.grad_scale = torch.zeros(1, device=dev)
+    try:
+        torch.cuda.synchronize()
+        other = threading.Thread(target=update)
+        other.start()
+        other.join()
+    finally:
+        engine.grad_scale = None
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and bool(results[0][1].any())
