@@ -23,6 +23,7 @@ the gradient leaves it out, and the device's error word is set, which
 
 from __future__ import annotations
 
+import threading
 from ctypes import byref, c_int
 from dataclasses import dataclass
 from operator import attrgetter
@@ -68,6 +69,7 @@ class _ErrorWord:
 
 
 _WORDS: dict[int, _ErrorWord] = {}
+_WORDS_LOCK = threading.Lock()
 
 # The current stream's handle: torch.cuda.current_stream(index).cuda_stream without its
 # Stream object where this torch has the call (0.1 us instead of 1.2).
@@ -88,9 +90,13 @@ def _error_word(index: int) -> _ErrorWord:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the first embedding call on a device allocates its error word: make one call "
                                "before capturing a graph")
-        N.check(N.lib().muon_device_check(index), "muon_device_check")
-        word = _WORDS[index] = _ErrorWord(torch.device("cuda", index))
-        torch.cuda.current_stream(index).synchronize()  # zeroed before any stream uses it
+        with _WORDS_LOCK:  # kernels keep the pointer: a device's word is made once
+            word = _WORDS.get(index)
+            if word is None:
+                N.check(N.lib().muon_device_check(index), "muon_device_check")
+                word = _ErrorWord(torch.device("cuda", index))
+                torch.cuda.current_stream(index).synchronize()  # zeroed before any stream uses it
+                _WORDS[index] = word
     return word
 
 

@@ -3,6 +3,7 @@
 import contextlib
 import ctypes
 import threading
+import time
 
 import pytest
 import torch
@@ -204,3 +205,30 @@ def test_a_step_keeps_its_clip_coefficient_to_its_thread():
     other.start()
     other.join()
     assert seen == [None] and engine.grad_scale == 0.5
+
+
+def test_threads_that_make_the_first_call_share_one_error_word(monkeypatch):
+    class Library:
+        def muon_device_check(self, index):
+            return E.N.MUON_OK
+
+    class Stream:
+        def synchronize(self):
+            time.sleep(0.05)
+
+    class Slow:
+        def __init__(self, device):
+            time.sleep(0.05)
+
+    monkeypatch.setattr(E.N, "lib", lambda: Library())
+    monkeypatch.setattr(E, "_WORDS", {})
+    monkeypatch.setattr(E, "_ErrorWord", Slow)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda index: Stream())
+    words = []
+    threads = [threading.Thread(target=lambda: words.append(E._error_word(0))) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(words) == 4 and len(set(map(id, words))) == 1 and E._WORDS[0] is words[0]
