@@ -37,7 +37,7 @@ _CODE = {torch.bfloat16: N.MUON_BF16, torch.float32: N.MUON_F32}
 # The lists are long and each call is short: what is asked of every tensor goes through map.
 _POINTER, _NUMEL, _DEVICE = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
 _CONTIGUOUS, _SIZE = torch.Tensor.is_contiguous, torch.Tensor.size
-_DTYPE = attrgetter("dtype")
+_DTYPE, _NBYTES = attrgetter("dtype"), attrgetter("nbytes")
 _NORMS = {2.0: N.MUON_NORM_2, 1.0: N.MUON_NORM_1, math.inf: N.MUON_NORM_INF}
 
 
@@ -283,19 +283,34 @@ def clip_grads_with_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max
     _clip([g if g.layout is torch.strided else g._values() for g in grads], None, max_norm, None, total_norm)
 
 
+def _shares_memory(written: list[torch.Tensor], read: list[torch.Tensor]) -> bool:
+    """Whether a written contiguous tensor overlaps another written or read one."""
+    tensors = written + read
+    kinds = [True] * len(written) + [False] * len(read)
+    spans = sorted(span for span in zip(map(_POINTER, tensors), map(_NBYTES, tensors), kinds) if span[1])
+    end = written_end = 0  # of the spans before
+    for begin, size, writes in spans:
+        if begin < (end if writes else written_end):
+            return True
+        end = max(end, begin + size)
+        if writes:
+            written_end = end
+    return False
+
+
 def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor], exp_avg_sqs: list[torch.Tensor],
           steps: list[float], *, lr: float, beta1: float, beta2: float, eps: float, weight_decay: float) -> None:
     """One AdamW update of each parameter, in place with its fp32 moments
     (``MuonAdamW``'s AdamW group, decoupled weight decay). ``grads``: dense
     tensors, or RowGrads for parameters whose gradient is zero outside some
     rows: the same results at the cost of those rows. ``steps``: the step
-    count of each, this step included."""
+    count of each, this step included. What is written may share memory with
+    nothing else in the lists; empty parameters may be listed any number of
+    times."""
     if not len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(steps):
         raise ValueError("adamw lists must have one entry per parameter")
     if not params:
         return
-    if len(set(map(_POINTER, params))) != len(params):
-        raise ValueError("adamw parameters must be distinct")
     if min(steps) < 1:
         raise ValueError("adamw steps count from 1")
     values = (g.values if isinstance(g, RowGrad) else g for g in grads)
@@ -308,8 +323,12 @@ def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor],
             raise RuntimeError("adamw takes a dense gradient of its parameter's shape, or a RowGrad")
         if any(t.dtype != torch.float32 or t.shape != p.shape or not t.is_contiguous() for t in (m, v)):
             raise RuntimeError("AdamW moments must be contiguous float32 tensors of their parameter's shape")
-    items = list(map(AdamItem, params, grads, exp_avgs, exp_avg_sqs, map(float, steps)))
     index = device_index(params[0])
+    reads = chain.from_iterable((g.ids, g.values) if isinstance(g, RowGrad) else (g,) for g in grads)
+    if _shares_memory([*params, *exp_avgs, *exp_avg_sqs], [t for t in reads if t.is_contiguous()]):  # others are copied
+        raise ValueError("adamw parameters and moments must be distinct: no two of them, and no gradient, may share "
+                         "memory")
+    items = list(map(AdamItem, params, grads, exp_avgs, exp_avg_sqs, map(float, steps)))
     on_device(index, lambda: engine_for(params[0].device, "fp16").adamw(
         items, lr=float(lr), beta1=float(beta1), beta2=float(beta2), eps=float(eps), weight_decay=float(weight_decay)))
     increment_version([*params, *exp_avgs, *exp_avg_sqs])

@@ -156,14 +156,25 @@ def test_writes_by_pointer_bump_version_counters(monkeypatch):
         y.backward()
 
 
-def test_adamw_bumps_version_counters(monkeypatch):
+@pytest.fixture
+def adam_items(monkeypatch):
+    """The items that adamw hands to its engine."""
+    seen = []
+
     class Engine:
         def adamw(self, items, **_):
-            pass
+            seen.extend(items)
 
     monkeypatch.setattr(functional, "device_index", lambda t: 0)
     monkeypatch.setattr(functional, "on_device", lambda index, call: call())
     monkeypatch.setattr(functional, "engine_for", lambda *_: Engine())
+    return seen
+
+
+ADAM = dict(lr=0.1, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0)
+
+
+def test_adamw_bumps_version_counters(adam_items):
     p, g, m, v = torch.nn.Parameter(torch.ones(3)), torch.ones(3), torch.zeros(3), torch.zeros(3)
     y = (p ** 2).sum()
     O.adamw([p], [g], [m], [v], [1], lr=0.1, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0)
@@ -232,3 +243,28 @@ def test_threads_that_make_the_first_call_share_one_error_word(monkeypatch):
     for t in threads:
         t.join()
     assert len(words) == 4 and len(set(map(id, words))) == 1 and E._WORDS[0] is words[0]
+
+
+def test_adamw_lists_may_not_share_memory(adam_items):
+    empty = [torch.zeros(0) for _ in range(2)]
+    O.adamw(empty, empty, empty, empty, [1, 1], **ADAM)
+    O.adamw([empty[0], empty[0]], empty, empty, empty, [1, 1], **ADAM)
+    assert len(adam_items) == 4
+    buf = torch.zeros(12 * 6)
+    p, q, m, n, v, w, g, h = buf.view(12, 6)[:8]
+    ids = torch.zeros(1, dtype=torch.long)
+
+    def call(params=(p, q), grads=(g, h), exp_avgs=(m, n), exp_avg_sqs=(v, w)):
+        O.adamw(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), [1, 1], **ADAM)
+
+    call()  # neighbours in one buffer
+    call(grads=(g, g))  # what is only read may be shared
+    call(grads=(buf[36:48].view(6, 2)[:, 0], buf[0:12].view(6, 2)[:, 1]))  # read through a copy
+    del adam_items[:]
+    for bad in ({"params": (p, p)}, {"params": (p, buf[3:9])}, {"params": (buf[3:9], p)}, {"exp_avgs": (m, m)},
+                {"exp_avgs": (m, v)}, {"exp_avg_sqs": (v, buf[31:37])}, {"grads": (g, q)}, {"grads": (buf[3:9], h)},
+                {"grads": (g, E.RowGrad(1, ids, buf[2:8].view(1, 6)))},
+                {"params": (p, torch.zeros(6).view(2, 3)), "grads": (g, E.RowGrad(2, ids, buf[1:4].view(1, 3)))}):
+        with pytest.raises(ValueError, match="share memory"):
+            call(**({"params": (p, q)} | bad))
+    assert not adam_items

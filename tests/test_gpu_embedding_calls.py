@@ -174,3 +174,18 @@ def test_adamw_beside_a_clipped_step_of_another_thread():
         engine.grad_scale = None
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(*results)) and bool(results[0][1].any())
+
+
+def test_adamw_takes_empty_parameters_and_refuses_shared_memory():
+    from opendm_b200.embedding import RowGrad
+    from opendm_b200.optimizer import adamw
+
+    dev = _dev()
+    kw = dict(lr=0.02, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0)
+    p, m, v, g = (torch.ones(40, 8, device=dev) for _ in range(4))
+    e = [torch.zeros(0, 8, device=dev) for _ in range(2)]
+    rows = RowGrad(0, torch.zeros(0, dtype=torch.long, device=dev), e[0])
+    adamw([e[0], p, e[1], e[0]], [e[0], g, e[1], rows], [e[0], m, e[1], e[1]], [e[0], v, e[1], e[1]], [1] * 4, **kw)
+    assert bool((p < 1).all())
+    with pytest.raises(ValueError, match="share memory"):
+        adamw([p[:20], p[10:30]], [g[:20], g[:20]], [m[:20], m[20:]], [v[:20], v[20:]], [1, 1], **kw)
