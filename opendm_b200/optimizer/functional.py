@@ -62,6 +62,65 @@ def _dense_storage(t: torch.Tensor) -> bool:
     return True
 
 
+def _steps(a: torch.Tensor, b: torch.Tensor) -> list[tuple[int, int, int]]:
+    """Per stride in bytes, descending, the least and greatest step between an element of ``a`` and one of ``b``."""
+    reach: dict[int, list[int]] = {}
+    for t, side in ((a, 0), (b, 1)):
+        for stride, size in zip(t.stride(), t.shape):
+            if size > 1:
+                ends = reach.setdefault(stride * t.element_size(), [0, 0])
+                ends[side] += (size - 1) * (1 if side else -1)
+    return [(stride, *reach[stride]) for stride in sorted(reach, reverse=True)]
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether elements of two strided tensors share memory, or, of a tensor and itself, two different ones.
+
+    Elements i of a and j of b do where the distance of their addresses,
+    b - a + sum of (steps x stride), lies in (-size of b's, size of a's): a
+    search over the steps of each stride, widest first, that drops what the
+    narrower ones cannot bring back. Views of one buffer leave it two or three
+    choices a stride; past 10000 it gives up and answers yes."""
+    steps, same, left = _steps(a, b), a is b, 10000
+    if same and (sum(n > 1 for n in a.shape) > len(steps) or steps and steps[-1][0] == 0):
+        return True  # two dimensions of one stride, or one that does not move
+    narrower = [(0, 0)]  # what the strides behind each one reach
+    for stride, low, high in reversed(steps):
+        narrower.append((narrower[-1][0] + stride * low, narrower[-1][1] + stride * high))
+    narrower.reverse()
+
+    def search(k: int, low: int, high: int, moved: bool) -> bool:  # can steps k on sum to [low, high]?
+        nonlocal left
+        left -= 1
+        if left < 0:
+            return True
+        if k == len(steps):
+            return low <= 0 <= high and moved
+        stride, least, most = steps[k]
+        if stride == 0:
+            return search(k + 1, low, high, moved)
+        down, up = narrower[k + 1]
+        first, last = max(least, -((up - low) // stride)), min(most, (high - down) // stride)
+        return any(search(k + 1, low - x * stride, high - x * stride, moved or x != 0) for x in range(first, last + 1))
+
+    apart = b.data_ptr() - a.data_ptr()
+    return search(0, 1 - b.element_size() - apart, a.element_size() - 1 - apart, not same)
+
+
+def _check_overlap(outs: list[torch.Tensor]) -> None:
+    """Raise where two of the tensors share memory, or two elements of one do."""
+    spans = []  # address behind the last byte, tensor; of those before that may still be met
+    for t in sorted((t for t in outs if t.numel()), key=_POINTER):
+        begin = t.data_ptr()
+        if not t.is_contiguous() and _meet(t, t):
+            raise RuntimeError("a tensor whose elements overlap in memory cannot be clipped into")
+        spans = [(end, other) for end, other in spans if end > begin]
+        if any(_meet(other, t) for _, other in spans):
+            raise RuntimeError("clipped gradients overlap in memory")
+        reach = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        spans.append((begin + (reach + 1) * t.element_size(), t))
+
+
 def _check_grads(grads: list[torch.Tensor], what: str) -> int:
     """Device index of the list; raises where a tensor is on another."""
     index = device_index(grads[0])
@@ -176,7 +235,8 @@ def _clip(grads: list[torch.Tensor], outs: list[torch.Tensor] | None, max_norm: 
         increment_version(outs)  # autograd has to see what was written by pointer
         return norm
     # Other strides: elementwise work needs only that both sides agree on the
-    # order of elements, else a contiguous copy is scaled and copied back.
+    # order of elements, else a contiguous copy is scaled and copied back, past
+    # the library's own check of overlaps.
     src, dst, back = [], [], []
     for g, o in zip(grads, outs):
         dense, _ = _dense_storage(g), _dense_storage(o)
@@ -192,6 +252,8 @@ def _clip(grads: list[torch.Tensor], outs: list[torch.Tensor] | None, max_norm: 
         else:
             dst.append(torch.empty(o.shape, dtype=o.dtype, device=o.device))
             back.append((o, dst[-1]))
+    if back:
+        _check_overlap(outs if total is None else [*outs, total])
     norm = _apply(src, dst, max_norm, norm_type, total)
     with torch.no_grad():
         for o, d in back:

@@ -2,6 +2,7 @@
 
 import contextlib
 import ctypes
+import random
 import threading
 import time
 
@@ -268,3 +269,51 @@ def test_adamw_lists_may_not_share_memory(adam_items):
         with pytest.raises(ValueError, match="share memory"):
             call(**({"params": (p, q)} | bad))
     assert not adam_items
+
+
+def _addresses(t):
+    at = torch.zeros((), dtype=torch.long)
+    for size, stride in zip(t.shape, t.stride()):
+        at = at[..., None] + torch.arange(size) * stride
+    at = t.data_ptr() + at.reshape(-1) * t.element_size()
+    return (at[:, None] + torch.arange(t.element_size())).reshape(-1)
+
+
+def test_overlaps_of_strided_tensors_are_found_exactly():
+    """Against all addresses, over random views of one buffer."""
+    rng = random.Random(1)
+    raw = torch.zeros(4000, dtype=torch.uint8)
+    met = 0
+    for _ in range(3000):
+        a, b = (torch.as_strided(raw.view(rng.choice([torch.bfloat16, torch.float32])), shape, stride, offset)
+                for shape, stride, offset in
+                [([rng.randint(1, 5) for _ in range(d)], [rng.choice([1, 2, 3, 5, 8, 40]) for _ in range(d)],
+                  rng.randint(0, 60)) for d in (rng.randint(0, 3), rng.randint(0, 3))])
+        want = bool(torch.isin(_addresses(a), _addresses(b)).any())
+        assert functional._meet(a, b) == want == functional._meet(b, a)
+        assert functional._meet(a, a) == (_addresses(a).unique().numel() < _addresses(a).numel())
+        met += want
+    assert 300 < met < 2700
+
+
+def test_overlapping_strided_gradients_are_refused(monkeypatch):
+    monkeypatch.setattr(functional, "_apply", lambda grads, *_: torch.tensor(1.0))
+    buf = torch.ones(20, 12)
+    O.clip_grads([buf[:, :4], buf[:, 4:7], buf[:, 7:]], 1.0)
+    O.clip_grads([buf[::2], buf[1::2]], 1.0)
+    O.clip_grads([buf[:, ::2].t(), buf[:, 1::2]], 1.0)
+    O.clip_grads([buf[:, :0], buf[:, :4]], 1.0)
+    out = torch.ones(20, 12)
+    for grads, outs in (([buf[:, :4], buf[:, 2:6]], None), ([buf[:, :4], buf[3]], None), ([buf, buf[:, 3:5]], None),
+                        ([buf[:, :4].t(), buf[:, 3:]], None), ([buf[::2], buf[4]], None),
+                        ([torch.ones(20, 4)] * 2, [out[:, :4], out[:, 3:7]]),
+                        ([torch.ones(8, 3)], [out.view(-1).as_strided((8, 3), (2, 1))])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            O.clip_grads(grads, 1.0, out=outs)
+    p = torch.nn.Parameter(torch.ones(20, 4))
+    p.grad = buf[:, :4]
+    O.clip_grads_with_norm_(p, 1.0, buf[0, 4])
+    with pytest.raises(RuntimeError, match="overlap"):
+        O.clip_grads_with_norm_(p, 1.0, buf[0, 3])
+    with pytest.raises(RuntimeError, match="expanded"):
+        O.clip_grads([torch.ones(1).expand(5)], 1.0)

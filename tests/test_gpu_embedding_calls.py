@@ -189,3 +189,18 @@ def test_adamw_takes_empty_parameters_and_refuses_shared_memory():
     assert bool((p < 1).all())
     with pytest.raises(ValueError, match="share memory"):
         adamw([p[:20], p[10:30]], [g[:20], g[:20]], [m[:20], m[20:]], [v[:20], v[20:]], [1, 1], **kw)
+
+
+def test_strided_gradients_that_overlap_are_refused_and_others_clipped():
+    from opendm_b200.optimizer import clip_grads
+
+    buf = torch.randn(64, 48, device=_dev(), generator=_gen(1))
+    ref = buf.clone()
+    with pytest.raises(RuntimeError, match="overlap"):
+        clip_grads([buf[:, :20], buf[:, 10:30]], 1.0)
+    assert torch.equal(buf, ref)
+    total = clip_grads([buf[:, :20], buf[:, 20:30], buf[:, 30:].t()], 1.0)
+    want = ref.double().norm()
+    # five half steps of fp32 in the norm, one each in the coefficient and the product
+    assert abs(float(total) - float(want)) <= 9 * 2.0 ** -24 * float(want)
+    assert ((buf.double() - ref.double() / (want + 1e-6)).abs() <= ref.double().abs() / want * 11 * 2.0 ** -24).all()
