@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_kernel(const W* __restrict_
   const uint32_t col0 = uint32_t(base - row0 * groups);
   const int64_t left = tokens * groups - base;
   uint4 raw[LK_PER][kWords];
+  uint32_t bad = 0;  // a bit a group
 #pragma unroll
   for (int i = 0; i < LK_PER; ++i) {
     const uint32_t o = i * LK_THREADS + threadIdx.x, c = col0 + o, over = c / groups;
@@ -151,6 +152,7 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_kernel(const W* __restrict_
     const uint32_t group = c - over * groups;
     const int64_t id = load_id(ids, wide, row0 + over);
     if (id < 0 || id >= rows) {
+      bad |= 1u << i;
 #pragma unroll
       for (int q = 0; q < kWords; ++q) raw[i][q] = make_uint4(0, 0, 0, 0);
       if (group == 0) record_error(err, MUON_DEV_BAD_INDEX);
@@ -164,10 +166,11 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_kernel(const W* __restrict_
   for (int i = 0; i < LK_PER; ++i) {
     const uint32_t o = i * LK_THREADS + threadIdx.x;
     if (o >= left) continue;
+    const float by = bad >> i & 1u ? 0.f : scale;  // zeros times an infinite scale would be NaN
     float v[kVec];
     load_group<kVec>(reinterpret_cast<const W*>(raw[i]), v);
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) v[k] *= scale;
+    for (int k = 0; k < kVec; ++k) v[k] *= by;
     store_group<kVec>(out + (base + o) * kVec, v);
   }
 }
@@ -190,6 +193,7 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_rows_kernel(const W* __rest
   if (t >= tokens) return;
   const int64_t id = load_id(ids, wide, t);
   const bool ok = id >= 0 && id < rows;
+  const float by = ok ? scale : 0.f;  // as above
   if (!ok && part == 0 && lane == 0) record_error(err, MUON_DEV_BAD_INDEX);
   const int64_t c0 = part * LK_COLS;
   const int n = static_cast<int>(min(int64_t(LK_COLS), dim - c0)) - lane * kE;  // columns from this lane's first on
@@ -206,7 +210,7 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_rows_kernel(const W* __rest
 #pragma unroll
     for (int k = 0; k < kGroups; ++k) {
 #pragma unroll
-      for (int i = 0; i < kE; ++i) v[k][i] *= scale;
+      for (int i = 0; i < kE; ++i) v[k][i] *= by;
       if (at + k * kStep < n) store_group<kE>(dst + at + k * kStep, v[k]);
     }
   }

@@ -204,3 +204,17 @@ def test_strided_gradients_that_overlap_are_refused_and_others_clipped():
     # five half steps of fp32 in the norm, one each in the coefficient and the product
     assert abs(float(total) - float(want)) <= 9 * 2.0 ** -24 * float(want)
     assert ((buf.double() - ref.double() / (want + 1e-6)).abs() <= ref.double().abs() / want * 11 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("nan"), -2.0])
+def test_rows_of_bad_ids_are_zeros_for_every_scale(scale):
+    from opendm_b200.embedding import check_errors, embedding
+
+    for dim in (16, 20, 33):  # in groups of eight, four and single elements
+        w = torch.ones(10, dim, device=_dev())
+        got = embedding(torch.tensor([3, 10, -1, 9], device=_dev()), w, scale=scale)
+        with pytest.raises(RuntimeError, match="token id out of range"):
+            check_errors()
+        assert not got[1:3].any() and not got[1:3].isnan().any()
+        assert torch.equal(got[[0, 3]].isnan(), torch.full((2, dim), scale != scale, device=_dev()))
+        assert scale != scale or bool((got[[0, 3]] == scale).all())
