@@ -368,7 +368,8 @@ def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor],
     rows: the same results at the cost of those rows. ``steps``: the step
     count of each, this step included. What is written may share memory with
     nothing else in the lists; empty parameters may be listed any number of
-    times."""
+    times. With RowGrads only, a call can be captured into a graph (which
+    keeps its step size); with dense gradients it raises there."""
     if not len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(steps):
         raise ValueError("adamw lists must have one entry per parameter")
     if not params:
@@ -390,7 +391,15 @@ def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor],
     if _shares_memory([*params, *exp_avgs, *exp_avg_sqs], [t for t in reads if t.is_contiguous()]):  # others are copied
         raise ValueError("adamw parameters and moments must be distinct: no two of them, and no gradient, may share "
                          "memory")
+    dense = not all(isinstance(g, RowGrad) for g in grads)
     items = list(map(AdamItem, params, grads, exp_avgs, exp_avg_sqs, map(float, steps)))
-    on_device(index, lambda: engine_for(params[0].device, "fp16").adamw(
-        items, lr=float(lr), beta1=float(beta1), beta2=float(beta2), eps=float(eps), weight_decay=float(weight_decay)))
+
+    def call():
+        if dense and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("adamw of dense gradients uploads a table, which a captured graph would read again: "
+                               "it cannot be captured")
+        engine_for(params[0].device, "fp16").adamw(items, lr=float(lr), beta1=float(beta1), beta2=float(beta2),
+                                                   eps=float(eps), weight_decay=float(weight_decay))
+
+    on_device(index, call)
     increment_version([*params, *exp_avgs, *exp_avg_sqs])

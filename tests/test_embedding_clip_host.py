@@ -169,6 +169,7 @@ def adam_items(monkeypatch):
     monkeypatch.setattr(functional, "device_index", lambda t: 0)
     monkeypatch.setattr(functional, "on_device", lambda index, call: call())
     monkeypatch.setattr(functional, "engine_for", lambda *_: Engine())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     return seen
 
 
@@ -317,3 +318,14 @@ def test_overlapping_strided_gradients_are_refused(monkeypatch):
         O.clip_grads_with_norm_(p, 1.0, buf[0, 3])
     with pytest.raises(RuntimeError, match="expanded"):
         O.clip_grads([torch.ones(1).expand(5)], 1.0)
+
+
+def test_adamw_of_dense_gradients_is_not_captured(adam_items, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    p, q, g, m, n, v, w = (torch.zeros(4, 2) for _ in range(7))
+    rows = E.RowGrad(4, torch.zeros(1, dtype=torch.long), torch.zeros(1, 2))
+    O.adamw([p], [rows], [m], [v], [1], **ADAM)
+    assert len(adam_items) == 1
+    with pytest.raises(RuntimeError, match="captured"):
+        O.adamw([p, q], [rows, g], [m, n], [v, w], [1, 1], **ADAM)
+    assert len(adam_items) == 1

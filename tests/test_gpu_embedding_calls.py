@@ -218,3 +218,30 @@ def test_rows_of_bad_ids_are_zeros_for_every_scale(scale):
         assert not got[1:3].any() and not got[1:3].isnan().any()
         assert torch.equal(got[[0, 3]].isnan(), torch.full((2, dim), scale != scale, device=_dev()))
         assert scale != scale or bool((got[[0, 3]] == scale).all())
+
+
+def test_adamw_rows_in_a_captured_graph():
+    from opendm_b200.embedding import embedding_row_grad
+    from opendm_b200.optimizer import adamw
+
+    dev = _dev()
+    kw = dict(lr=0.02, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.01)
+    start = torch.randn(300, 24, device=dev, generator=_gen(1))
+    ids, grad = torch.randint(300, (50,), device=dev, generator=_gen(2)), torch.randn(50, 24, device=dev)
+    p, m, v = start.clone(), torch.zeros_like(start), torch.zeros_like(start)
+    adamw([p], [embedding_row_grad(grad, ids, 300)], [m], [v], [1], **kw)  # makes the engine and the error word
+    want = [t.clone() for t in (p, m, v)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        adamw([p], [embedding_row_grad(grad, ids, 300)], [m], [v], [1], **kw)
+    p.copy_(start), m.zero_(), v.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((p, m, v), want))
+    ids.copy_(torch.randint(300, (50,), device=dev, generator=_gen(3)))
+    for t, u in zip(want, (p, m, v)):
+        t.copy_(u)
+    graph.replay()
+    adamw([want[0]], [embedding_row_grad(grad, ids, 300)], [want[1]], [want[2]], [1], **kw)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((p, m, v), want))
