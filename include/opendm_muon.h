@@ -433,7 +433,7 @@ int muon_adamw_scaled(const muon_adamw_seg* segs_dev, int n_segs, int64_t total_
  * row numbers, of which the first *count (all, when count is NULL; never more
  * than cap) are used; an id outside [0, rows) matches no row. values:
  * [cap][dim] of grad_dtype. exp_avg and exp_avg_sq are fp32, updated in place
- * like param. */
+ * like param; the three may share memory with none of the other buffers. */
 typedef struct muon_adamw_rows_seg {
   void* param;           /* [rows][dim] of param_dtype */
   float* exp_avg;        /* [rows][dim] */

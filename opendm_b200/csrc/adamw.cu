@@ -369,7 +369,7 @@ int launch_adamw_rows(const muon_adamw_rows_seg* seg, double beta1, double beta2
   if (!seg) return set_error(MUON_ERR_ARG, "null AdamW row segment");
   const muon_adamw_rows_seg& sg = *seg;
   if (sg.rows < 0 || sg.dim < 0 || sg.cap < 0 || sg.cap > 0x7fffffffLL || sg.dim > 0x7fff0000LL ||
-      (sg.dim > 0 && sg.rows > (int64_t(1) << 43) / sg.dim))
+      (sg.dim > 0 && (sg.rows > (int64_t(1) << 43) / sg.dim || sg.cap > (int64_t(1) << 58) / sg.dim)))
     return set_error(MUON_ERR_ARG, "AdamW row sizes out of range");
   if ((sg.param_dtype != MUON_BF16 && sg.param_dtype != MUON_F32) ||
       (sg.grad_dtype != MUON_BF16 && sg.grad_dtype != MUON_F32))
@@ -381,6 +381,25 @@ int launch_adamw_rows(const muon_adamw_rows_seg* seg, double beta1, double beta2
       misaligned(sg.exp_avg_sq, 4) || misaligned(sg.ids, 8) || misaligned(sg.count, 8) ||
       misaligned(sg.values, sg.grad_dtype == MUON_BF16 ? 2 : 4) || misaligned(grad_scale, 4))
     return set_error(MUON_ERR_ARG, "AdamW row pointer not aligned to its dtype");
+  // Blocks read and write in no fixed order: what one writes nothing else may touch.
+  struct Span {
+    const void* at;
+    int64_t bytes;
+  };
+  const int64_t numel = sg.rows * sg.dim, param_size = sg.param_dtype == MUON_BF16 ? 2 : 4;
+  const Span spans[] = {{sg.param, numel * param_size},
+                        {sg.exp_avg, numel * 4},
+                        {sg.exp_avg_sq, numel * 4},
+                        {sg.ids, sg.cap * 8},
+                        {sg.values, sg.cap * sg.dim * (sg.grad_dtype == MUON_BF16 ? 2 : 4)},
+                        {sg.count, sg.count ? 8 : 0},
+                        {grad_scale, grad_scale ? 4 : 0}};
+  for (int i = 0; i < 3; ++i)
+    for (int j = i + 1; j < 7; ++j) {
+      const uintptr_t x = reinterpret_cast<uintptr_t>(spans[i].at), y = reinterpret_cast<uintptr_t>(spans[j].at);
+      if (spans[j].bytes > 0 && x < y + spans[j].bytes && y < x + spans[i].bytes)
+        return set_error(MUON_ERR_ARG, "AdamW row buffers share memory");
+    }
   AdamwRowsArgs a{};
   a.exp_avg = sg.exp_avg;
   a.exp_avg_sq = sg.exp_avg_sq;
@@ -389,7 +408,7 @@ int launch_adamw_rows(const muon_adamw_rows_seg* seg, double beta1, double beta2
   a.rows = sg.rows;
   a.dim = sg.dim;
   a.cap = sg.cap;
-  a.numel = sg.rows * sg.dim;
+  a.numel = numel;
   a.beta1w = static_cast<float>(1.0 - beta1);
   a.beta2 = static_cast<float>(beta2);
   a.one_minus_beta2 = static_cast<float>(1.0 - beta2);

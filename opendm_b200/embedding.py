@@ -148,9 +148,14 @@ def _code(table: dict, dtype: torch.dtype, what: str) -> int:
     return code
 
 
+def in_dual_level() -> bool:
+    """Whether tensors can carry forward-mode derivatives here."""
+    return forward_ad._current_level >= 0
+
+
 def has_tangent(tensors) -> bool:
-    """Whether one of the tensors carries a forward-mode derivative (outside of a dual level none does)."""
-    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    """Whether one of the tensors carries a forward-mode derivative."""
+    return in_dual_level() and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def refuse_derivatives(what: str, tensors) -> None:

@@ -29,7 +29,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from .. import _native as N
-from ..embedding import (RowGrad, device_index, embedding_row_grad, has_tangent, on_device, raw_stream,
+from ..embedding import (RowGrad, device_index, embedding_row_grad, has_tangent, in_dual_level, on_device, raw_stream,
                          refuse_derivatives)
 from ..engine import AdamItem, engine_for
 
@@ -130,9 +130,12 @@ def _check_grads(grads: list[torch.Tensor], what: str) -> int:
 
 
 def _codes(grads: list[torch.Tensor]) -> list[int]:
-    codes = list(map(_CODE.get, map(_DTYPE, grads)))
+    kinds = list(map(_DTYPE, grads))
+    if kinds.count(kinds[0]) == len(kinds) and kinds[0] in _CODE:  # one dtype, the usual case
+        return [_CODE[kinds[0]]] * len(kinds)
+    codes = list(map(_CODE.get, kinds))
     if None in codes:
-        raise RuntimeError(f"unsupported dtype {grads[codes.index(None)].dtype}: the kernels take bfloat16 or float32")
+        raise RuntimeError(f"unsupported dtype {kinds[codes.index(None)]}: the kernels take bfloat16 or float32")
     return codes
 
 
@@ -360,6 +363,10 @@ def _shares_memory(written: list[torch.Tensor], read: list[torch.Tensor]) -> boo
     return False
 
 
+def _tensors_of(grad) -> tuple:
+    return (grad.ids, grad.values) if isinstance(grad, RowGrad) else (grad,) if isinstance(grad, torch.Tensor) else ()
+
+
 def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor], exp_avg_sqs: list[torch.Tensor],
           steps: list[float], *, lr: float, beta1: float, beta2: float, eps: float, weight_decay: float) -> None:
     """One AdamW update of each parameter, in place with its fp32 moments
@@ -376,22 +383,24 @@ def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor],
         return
     if min(steps) < 1:
         raise ValueError("adamw steps count from 1")
-    values = (g.values if isinstance(g, RowGrad) else g for g in grads)
-    if has_tangent(t for t in chain(params, values, exp_avgs, exp_avg_sqs) if isinstance(t, torch.Tensor)):
+    written = [*params, *exp_avgs, *exp_avg_sqs]
+    if in_dual_level() and has_tangent(chain(written, chain.from_iterable(map(_tensors_of, grads)))):
         raise RuntimeError("adamw has no forward-mode derivative")
+    dense = False
     for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
         if isinstance(g, RowGrad):
             continue  # checked by the engine
+        dense = True
         if not isinstance(g, torch.Tensor) or g.layout is not torch.strided or g.shape != p.shape:
             raise RuntimeError("adamw takes a dense gradient of its parameter's shape, or a RowGrad")
         if any(t.dtype != torch.float32 or t.shape != p.shape or not t.is_contiguous() for t in (m, v)):
             raise RuntimeError("AdamW moments must be contiguous float32 tensors of their parameter's shape")
     index = device_index(params[0])
-    reads = chain.from_iterable((g.ids, g.values) if isinstance(g, RowGrad) else (g,) for g in grads)
-    if _shares_memory([*params, *exp_avgs, *exp_avg_sqs], [t for t in reads if t.is_contiguous()]):  # others are copied
-        raise ValueError("adamw parameters and moments must be distinct: no two of them, and no gradient, may share "
-                         "memory")
-    dense = not all(isinstance(g, RowGrad) for g in grads)
+    if dense or len(params) > 1:  # the tensors of one row update are checked by the library
+        reads = chain.from_iterable(map(_tensors_of, grads))
+        if _shares_memory(written, [t for t in reads if t.is_contiguous()]):  # others are copied
+            raise ValueError("adamw parameters and moments must be distinct: no two of them, and no gradient, may "
+                             "share memory")
     items = list(map(AdamItem, params, grads, exp_avgs, exp_avg_sqs, map(float, steps)))
 
     def call():
@@ -402,4 +411,4 @@ def adamw(params: list[torch.Tensor], grads: list, exp_avgs: list[torch.Tensor],
                                                    eps=float(eps), weight_decay=float(weight_decay))
 
     on_device(index, call)
-    increment_version([*params, *exp_avgs, *exp_avg_sqs])
+    increment_version(written)

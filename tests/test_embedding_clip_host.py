@@ -12,6 +12,7 @@ from torch.autograd import forward_ad as fw
 
 from opendm_b200 import embedding as E
 from opendm_b200 import optimizer as O
+from opendm_b200.build import build
 from opendm_b200.engine import CudaMuonEngine
 from opendm_b200.optimizer import functional
 from opendm_b200.optimizer import MuonAdamW, mark_muon_parameters
@@ -329,3 +330,26 @@ def test_adamw_of_dense_gradients_is_not_captured(adam_items, monkeypatch):
     with pytest.raises(RuntimeError, match="captured"):
         O.adamw([p, q], [rows, g], [m, n], [v, w], [1, 1], **ADAM)
     assert len(adam_items) == 1
+
+
+def test_row_update_buffers_may_not_share_memory():
+    build()
+    lib = E.N.lib()
+    at = {"param": 1 << 20, "exp_avg": 2 << 20, "exp_avg_sq": 3 << 20, "ids": 4 << 20, "values": 5 << 20,
+          "count": 6 << 20}
+
+    def refused(scale=7 << 20, **moved):
+        seg = E.N.AdamwRowsSeg(**(at | {"rows": 4, "dim": 8, "cap": 2, "param_dtype": E.N.MUON_F32,
+                                        "grad_dtype": E.N.MUON_F32} | moved))
+        code = lib.muon_adamw_rows(ctypes.byref(seg), 0.9, 0.95, 1e-8, 1.0, scale, None)
+        return code == E.N.MUON_ERR_ARG and "share memory" in E.N.last_error()
+
+    for written in ("param", "exp_avg", "exp_avg_sq"):  # 4 x 8 fp32 each
+        for other, size in (("param", 128), ("exp_avg", 128), ("exp_avg_sq", 128), ("ids", 16), ("values", 64),
+                            ("count", 8)):
+            if other != written:
+                assert refused(**{other: at[written] + 120}) and refused(**{other: at[written] - size + 8})
+        assert refused(scale=at[written] + 124)
+    seg = E.N.AdamwRowsSeg(**(at | {"rows": 4, "dim": 1 << 30, "cap": (1 << 31) - 1, "param_dtype": E.N.MUON_F32,
+                                    "grad_dtype": E.N.MUON_F32}))
+    assert lib.muon_adamw_rows(ctypes.byref(seg), 0.9, 0.95, 1e-8, 1.0, None, None) == E.N.MUON_ERR_ARG

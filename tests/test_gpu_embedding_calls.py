@@ -245,3 +245,24 @@ def test_adamw_rows_in_a_captured_graph():
     adamw([want[0]], [embedding_row_grad(grad, ids, 300)], [want[1]], [want[2]], [1], **kw)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip((p, m, v), want))
+
+
+def test_neighbours_in_one_buffer_are_updated():
+    """Parameter, moments and rows that touch, as views of one buffer, and one element of overlap."""
+    from opendm_b200.embedding import RowGrad
+    from opendm_b200.optimizer import adamw
+
+    dev = _dev()
+    kw = dict(lr=0.02, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0)
+    buf = torch.ones(7, 4, 8, device=dev)
+    p, m, v, values = buf[1], buf[2], buf[3], buf[4, :2]
+    ids = torch.tensor([0, 3], device=dev)
+    want = [t.clone() for t in (p, m, v)]
+    adamw([want[0]], [RowGrad(4, ids, values)], [want[1]], [want[2]], [1], **kw)
+    adamw([p], [RowGrad(4, ids, values)], [m], [v], [1], **kw)
+    assert all(torch.equal(a, b) for a, b in zip((p, m, v), want))
+    assert bool((buf[[0, 4, 5, 6]] == 1).all())
+    flat = buf.view(-1)
+    for k in (1, 31):
+        with pytest.raises(RuntimeError, match="share memory"):
+            adamw([p], [RowGrad(4, ids, values)], [flat[32 + k:64 + k].view(4, 8)], [buf[6]], [1], **kw)
