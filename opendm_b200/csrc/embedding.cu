@@ -24,6 +24,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "common.cuh"
 #include "internal.h"
@@ -144,7 +145,6 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_kernel(const W* __restrict_
   const uint32_t col0 = uint32_t(base - row0 * groups);
   const int64_t left = tokens * groups - base;
   uint4 raw[LK_PER][kWords];
-  uint32_t bad = 0;  // a bit a group
 #pragma unroll
   for (int i = 0; i < LK_PER; ++i) {
     const uint32_t o = i * LK_THREADS + threadIdx.x, c = col0 + o, over = c / groups;
@@ -152,7 +152,6 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_kernel(const W* __restrict_
     const uint32_t group = c - over * groups;
     const int64_t id = load_id(ids, wide, row0 + over);
     if (id < 0 || id >= rows) {
-      bad |= 1u << i;
 #pragma unroll
       for (int q = 0; q < kWords; ++q) raw[i][q] = make_uint4(0, 0, 0, 0);
       if (group == 0) record_error(err, MUON_DEV_BAD_INDEX);
@@ -166,22 +165,28 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_kernel(const W* __restrict_
   for (int i = 0; i < LK_PER; ++i) {
     const uint32_t o = i * LK_THREADS + threadIdx.x;
     if (o >= left) continue;
-    const float by = bad >> i & 1u ? 0.f : scale;  // zeros times an infinite scale would be NaN
     float v[kVec];
     load_group<kVec>(reinterpret_cast<const W*>(raw[i]), v);
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) v[k] *= by;
+    for (int k = 0; k < kVec; ++k) v[k] *= scale;
     store_group<kVec>(out + (base + o) * kVec, v);
   }
 }
 
 // Other rows: a warp takes up to 1024 columns of one token, eight elements a
 // lane at a time in groups of kE (4, 2 or 1): no division per element. The
-// fp32 32003 x 1001 table with 40961 tokens takes 30 us: its 164 MB of fp32
-// rows and 82 MB of results all cross L2, in part sectors.
+// fp32 32003 x 1001 table with 40961 tokens into bf16 takes 31.5 us on the
+// device and 33.5 a call, against 18.7 of its bytes: loads of 4 and stores of 2
+// bytes a lane, so the lines of 164 MB of rows and 82 MB of results cross L2 in
+// part sectors. The result is one contiguous array; aligned 16-byte groups over
+// two tokens, with the rows read through shared memory, were not tried.
 constexpr int LK_COLS = 1024;
 
-template <int kE, typename W, typename O>
+// kAnyScale: the scale may be infinite or NaN, which a bad id's zeros must not
+// be multiplied by. Looking for that in every call cost up to 11% (20000 x 2052
+// bf16 27.7 -> 31.0 us, 2048 fp32 into bf16 28.8 -> 30.7), so such a scale has a
+// kernel of its own.
+template <int kE, bool kAnyScale, typename W, typename O>
 __global__ void __launch_bounds__(LK_THREADS) lookup_rows_kernel(const W* __restrict__ weight, int64_t rows,
                                                                  int64_t ld, const void* __restrict__ ids, bool wide,
                                                                  int64_t tokens, int64_t dim, int64_t parts,
@@ -193,7 +198,7 @@ __global__ void __launch_bounds__(LK_THREADS) lookup_rows_kernel(const W* __rest
   if (t >= tokens) return;
   const int64_t id = load_id(ids, wide, t);
   const bool ok = id >= 0 && id < rows;
-  const float by = ok ? scale : 0.f;  // as above
+  const float by = kAnyScale && !ok ? 0.f : scale;
   if (!ok && part == 0 && lane == 0) record_error(err, MUON_DEV_BAD_INDEX);
   const int64_t c0 = part * LK_COLS;
   const int n = static_cast<int>(min(int64_t(LK_COLS), dim - c0)) - lane * kE;  // columns from this lane's first on
@@ -220,7 +225,7 @@ template <typename W, typename O>
 int run_lookup(const void* weight, int64_t rows, int64_t dim, int64_t ld, const void* ids, bool wide, int64_t tokens,
                float scale, void* out, int* err, cudaStream_t stream) {
   const int width = group_width(dim, ld, weight, sizeof(W), out, sizeof(O));
-  const bool flat = width == kVec;
+  const bool finite = std::isfinite(scale), flat = finite && width == kVec;
   const int64_t groups = dim / kVec, parts = (dim + LK_COLS - 1) / LK_COLS;
   const int64_t units = flat ? tokens * groups : tokens * parts, per = flat ? LK_THREADS * LK_PER : LK_THREADS / 32;
   const int64_t blocks = (units + per - 1) / per;
@@ -234,12 +239,14 @@ int run_lookup(const void* weight, int64_t rows, int64_t dim, int64_t ld, const 
   if (flat)
     lookup_kernel<W, O><<<grid, LK_THREADS, 0, stream>>>(w, rows, ld, ids, wide, tokens,
                                                          static_cast<uint32_t>(groups), scale, o, err);
+  else if (!finite)
+    by_rows(lookup_rows_kernel<1, true, W, O>);
   else if (width == 4)
-    by_rows(lookup_rows_kernel<4, W, O>);
+    by_rows(lookup_rows_kernel<4, false, W, O>);
   else if (width == 2)
-    by_rows(lookup_rows_kernel<2, W, O>);
+    by_rows(lookup_rows_kernel<2, false, W, O>);
   else
-    by_rows(lookup_rows_kernel<1, W, O>);
+    by_rows(lookup_rows_kernel<1, false, W, O>);
   return check_cuda(cudaGetLastError(), "embedding launch");
 }
 
