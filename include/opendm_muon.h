@@ -483,7 +483,10 @@ int muon_embedding(const void* weight, int weight_dtype, int64_t rows, int64_t d
  * With no tokens, rows or columns the ids are not read (and *count is 0).
  * workspace: muon_embedding_grad_workspace_bytes() bytes, 256-byte aligned
  * (-1 for sizes the call refuses: tokens or rows >= 2^31 - 1). One workspace
- * serves one call at a time. */
+ * serves one call at a time. What is written (out, out_ids, count, workspace)
+ * shares memory with nothing else, as does muon_embedding's out. The cost of
+ * the sort grows with tokens up to some ten million and with their square
+ * above: split longer lists. */
 int64_t muon_embedding_grad_workspace_bytes(int64_t tokens, int64_t rows, int64_t dim);
 int muon_embedding_grad(const void* grad, int grad_dtype, const void* ids, int ids_dtype, int64_t tokens,
                         int64_t rows, int64_t dim, int64_t padding_idx, float scale, void* out, int out_dtype,

@@ -229,9 +229,11 @@ constexpr int ROWS_CHUNK = ADAM_THREADS * ADAM_VEC * ROWS_ITERS;  // 4096 elemen
 // may span rows. kGradVector: they never do, and rows of values are aligned too.
 // 151936 x 2048 bf16, 16384 tokens: 999 us (6.26 TB/s of 6.55 measured); with
 // 8192 elements a block 991, with 2048 1079, with six blocks an SM 1034. An fp32
-// 32003 x 257: 54 us with 2048 or 4096, 57 with 8192. With zero moments in the
-// 97% of its rows no token names (the start of a run) the first takes 680 us,
-// the dense kernel, whose divisions are then slow ones, 1407.
+// 32003 x 257: 54 us with 2048 or 4096, 57 with 8192; a division of integers and
+// a slot lookup for each group of four, and 2009 blocks in 1184 places, are what
+// it has over the first. With zero moments in the 95% of its rows no token names
+// (the start of a run) the first takes 694 us, the dense kernel, whose divisions
+// are then slow ones, 1382.
 template <typename P, typename G, bool kVector, bool kGradVector>
 __global__ void __launch_bounds__(ADAM_THREADS, ROWS_BLOCKS)
     adamw_rows_kernel(P* __restrict__ param, const G* __restrict__ values, const AdamwRowsArgs a) {

@@ -282,9 +282,17 @@ __device__ __forceinline__ uint32_t token_key(const TokenSource& s, int64_t t, i
 // Most of the GPU idles while a block or a cluster sorts. In the dense form,
 // extra blocks of that kernel write zeros over the last rows of the result; the
 // sum writes those of them that have tokens and leaves the rest. 48 MB by 64
-// blocks took the gradient of 16384 tokens (151936 x 2048 bf16) from 120 to 115
-// us; by 32 blocks 126, by 128 118 (they slow the sort), with 64 or 80 MB 117-119.
-// The rows past the count of the row form gained nothing so.
+// blocks beside a cluster, 8 MB beside one block, against none (us a call):
+//   151936 x 2048 bf16  512 tokens 95.4 / 96.4, 2049 101.9 / 102.7, 4096 105.5 /
+//     107.3, 8192 109.1 / 111.3, 16384 117.4 / 123.2, 32768 140.1 / 143.9
+//   32003 x 1024 fp32   2049 37.9 / 39.8, 16384 51.7 / 58.1, 32768 73.2 / 78.4
+//   151936 x 256 bf16   2049 29.6 / 29.7, 8192 31.7 / 32.9, 32768 46.0 / 50.2
+// A result little larger than the 48 MB gains at 16384 tokens (50000 x 512 bf16
+// 33.3 / 35.8) and loses about 1 us from 3000 to 8192 (30.7 / 29.5); one of 25 MB
+// (12000 x 1024 bf16) is between 2 us faster (3000, 8192) and 2 us slower (32768).
+// By 32 blocks 16384 tokens of the first took 126 us, by 128 118 (they slow the
+// sort), with 64 or 80 MB 117-119. The rows past the count of the row form gained
+// nothing so.
 struct Fill {
   char* from;  // 16-byte aligned
   int64_t vectors;
@@ -566,7 +574,12 @@ __global__ void __cluster_dims__(CL_BLOCKS, 1, 1) __launch_bounds__(RS_THREADS)
 // Larger sorts: digit counts of every tile for the first pass, then one
 // scatter a pass. A scatter block adds the tiles' counts itself (its first
 // positions are the sums over the smaller digits and the tiles before it)
-// and counts the next pass's digits by destination tile as it writes.
+// and counts the next pass's digits by destination tile as it writes. Reading
+// all tiles' counts in every block is quadratic, 2 KB x tiles^2 a pass, and next
+// to nothing at the sizes of a training batch: a whole call of two fp32 columns
+// takes 69 us at 131072 tokens, 126 at 400000, 300 at a million, 1420 at four
+// million and 8010 at sixteen. Far above that it rules (a pass over 2^31 tokens
+// would read 560 TB): split such a list.
 constexpr int RS_PER = 8;
 constexpr int RS_TILE = RS_THREADS * RS_PER;
 
@@ -605,8 +618,8 @@ __global__ void __launch_bounds__(RS_THREADS) radix_scatter_kernel(TokenSource s
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   clear_counts(counts);
   wait_previous();
-  // this tile's first position of every digit, a thread a digit (before the keys are asked for: behind them the
-  // sort of 400000 tokens took 59 us, not 44)
+  // this tile's first position of every digit, a thread a digit (before the keys are asked for: behind them a call
+  // of 400000 tokens x 2 took 139 us, not 126)
   uint32_t before = 0, total = 0;
 #pragma unroll 16
   for (int64_t t = 0; t < tiles; ++t) {
@@ -864,8 +877,8 @@ __device__ __forceinline__ void copy_async_wait() {
 // rows of dY come through a ring in shared memory (4 KB a warp, filled by
 // asynchronous copies that each lane makes and reads for itself), so few
 // registers are held; single bf16 elements, too small for such copies, are
-// loaded two rows at a time instead (six blocks an SM: 50000 x 1001 137 us, with
-// four rows 144, with five blocks 151). 131072 x 2560 bf16 into rows: 184 us,
+// loaded two rows at a time instead (six blocks an SM: a call of 50000 x 1001 146
+// us, with four rows 150, with five blocks 161). 131072 x 2560 bf16 into rows: 184 us,
 // 6.6 TB/s of DRAM traffic.
 // A small batch is bound by the issue slots and its one wave of blocks: 16384 x
 // 2048 24 us; 16 columns a lane cost it 3 us more. The blocks behind sum_blocks
@@ -1082,8 +1095,10 @@ int bits_for(int64_t rows) {  // keys 0 .. rows
 
 // Chunk length: long chunks leave fewer partial rows to join, short ones give
 // more warps (counted in whole slices: a warp of a narrow row does little).
-// 16384 tokens x 2048 (bf16): 26.3 us with 32, 26-28 with 16, 33 with 8; 131072
-// x 64: 36 us with 32, 34 with 16, 42 with 8 (long runs then have 950 parts).
+// Calls with at least 32 / 16 / 8 positions: 9000 x 250 (bf16) 31.0 / 29.0 / 28.0
+// us, 131072 x 64 65 / 69 / 80, 400000 x 2 (fp32) 108 / 126 / 167 (long runs then
+// have ever more parts); 16384 x 2048 takes 48 with 32 whichever is the least. So 16
+// above 8192 tokens costs narrow rows of many tokens 4 to 17% and gains 6% at 9000.
 int chunk_for(int64_t tokens, int64_t dim) {
   const int least = tokens > 8192 ? 16 : 8;
   int chunk = kMaxChunk;
