@@ -73,15 +73,17 @@ def _steps(a: torch.Tensor, b: torch.Tensor) -> list[tuple[int, int, int]]:
     return [(stride, *reach[stride]) for stride in sorted(reach, reverse=True)]
 
 
-def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether elements of two strided tensors share memory, or, of a tensor and itself, two different ones.
+def _meet(a: torch.Tensor, b: torch.Tensor | None = None) -> bool:
+    """Whether elements of two strided tensors share memory, or, of one alone, two different elements.
 
     Elements i of a and j of b do where the distance of their addresses,
     b - a + sum of (steps x stride), lies in (-size of b's, size of a's): a
     search over the steps of each stride, widest first, that drops what the
     narrower ones cannot bring back. Views of one buffer leave it two or three
     choices a stride; past 10000 it gives up and answers yes."""
-    steps, same, left = _steps(a, b), a is b, 10000
+    same = b is None
+    b = a if same else b
+    steps, left = _steps(a, b), 10000
     if same and (sum(n > 1 for n in a.shape) > len(steps) or steps and steps[-1][0] == 0):
         return True  # two dimensions of one stride, or one that does not move
     narrower = [(0, 0)]  # what the strides behind each one reach
@@ -112,7 +114,7 @@ def _check_overlap(outs: list[torch.Tensor]) -> None:
     spans = []  # address behind the last byte, tensor; of those before that may still be met
     for t in sorted((t for t in outs if t.numel()), key=_POINTER):
         begin = t.data_ptr()
-        if not t.is_contiguous() and _meet(t, t):
+        if not t.is_contiguous() and _meet(t):
             raise RuntimeError("a tensor whose elements overlap in memory cannot be clipped into")
         spans = [(end, other) for end, other in spans if end > begin]
         if any(_meet(other, t) for _, other in spans):
