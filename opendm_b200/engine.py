@@ -903,6 +903,9 @@ def engine_for(device: torch.device, precision: str, ns_algo: str = "auto") -> C
     idx = device.index if device.index is not None else torch.cuda.current_device()
     key = (idx, precision, ns_algo)
     if key not in _ENGINES:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first call on a device allocates its engine: make one call before capturing a "
+                               "graph")
         _ENGINES[key] = CudaMuonEngine(torch.device("cuda", idx), precision, ns_algo)
     return _ENGINES[key]
 

@@ -354,3 +354,17 @@ def test_row_update_buffers_may_not_share_memory():
     seg = E.N.AdamwRowsSeg(**(at | {"rows": 4, "dim": 1 << 30, "cap": (1 << 31) - 1, "param_dtype": E.N.MUON_F32,
                                     "grad_dtype": E.N.MUON_F32}))
     assert lib.muon_adamw_rows(ctypes.byref(seg), 0.9, 0.95, 1e-8, 1.0, None, None) == E.N.MUON_ERR_ARG
+
+
+def test_an_engine_is_not_made_inside_a_capture(monkeypatch):
+    from opendm_b200 import engine
+
+    monkeypatch.setattr(engine, "_ENGINES", {})
+    monkeypatch.setattr(engine, "CudaMuonEngine", lambda *_: "engine")
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before capturing"):
+        engine.engine_for(torch.device("cuda", 0), "fp16")
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert engine.engine_for(torch.device("cuda", 0), "fp16") == "engine"
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    assert engine.engine_for(torch.device("cuda", 0), "fp16") == "engine"
