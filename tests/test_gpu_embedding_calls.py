@@ -266,3 +266,41 @@ def test_neighbours_in_one_buffer_are_updated():
     for k in (1, 31):
         with pytest.raises(RuntimeError, match="share memory"):
             adamw([p], [RowGrad(4, ids, values)], [flat[32 + k:64 + k].view(4, 8)], [buf[6]], [1], **kw)
+
+
+def test_sparse_backward_captured_into_a_graph():
+    """Forward and sparse backward, captured with the AdamW of its rows and replayed with other tokens."""
+    from opendm_b200.embedding import check_errors, embedding
+    from opendm_b200.optimizer import adamw
+    from opendm_b200.optimizer.functional import rows_of
+
+    dev = _dev()
+    kw = dict(lr=0.02, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0)
+    ids = torch.randint(300, (600,), device=dev, generator=_gen(1))
+    coef = torch.randn(600, 24, device=dev, generator=_gen(2))
+    weight = torch.nn.Parameter(torch.randn(300, 24, device=dev, generator=_gen(3)))
+    m, v = torch.zeros_like(weight), torch.zeros_like(weight)
+
+    def step(w, m, v):
+        w.grad = None
+        (embedding(ids, w, sparse=True) * coef).sum().backward()
+        adamw([w], [rows_of(w.grad)], [m], [v], [1], **kw)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(weight, m, v)
+        weight.grad = None
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(weight, m, v)
+    for seed in (4, 5):
+        ids.copy_(torch.randint(300, (600,), device=dev, generator=_gen(seed)))
+        want = [torch.nn.Parameter(weight.detach().clone()), m.clone(), v.clone()]
+        graph.replay()
+        torch.cuda.synchronize()
+        step(*want)
+        assert torch.equal(weight, want[0]) and torch.equal(m, want[1]) and torch.equal(v, want[2])
+    check_errors()
